@@ -106,7 +106,7 @@ TTAMD_API int rt_memset(void *dst, int value, size_t bytes, void *stream);
 
 /* Code objects.  rt_module_load takes a gfx950 code object image in memory
  * (device.load_library, backend/driver.py:72); rt_builtin_module returns one of
- * the images embedded in this library ("elementwise", "gemm", "attention", "reduce"). */
+ * the images embedded in this library ("elementwise", "gemm", "attention", "reduce", "paged"). */
 TTAMD_API int rt_module_load(const void *image, size_t bytes, rt_module *out);
 TTAMD_API int rt_module_unload(rt_module m);
 TTAMD_API int rt_builtin_module(const char *which, rt_module *out);
@@ -351,6 +351,71 @@ TTAMD_API int tt_attn_fwd(float sm_scale, float *M, int32_t Z, int32_t H, const 
                 const tt_desc2d *desc_k, const tt_desc2d *desc_v, const tt_desc2d *desc_o,
                 int32_t N_CTX, int32_t HEAD_DIM, int32_t BLOCK_M, int32_t BLOCK_N,
                 int32_t STAGE, const uint32_t grid[3], void *stream);
+
+/* ----------------------------------------------------------------------- */
+/* A paged key/value cache in 8 bits (no counterpart in the reference)      */
+/* ----------------------------------------------------------------------- */
+
+/* The cache of one layer: for K and for V, e4m3 codes [num_pages, heads, page_size, head_dim] and one scale for each
+ * (page, head), held as its exponent: code s (a byte, 0..254) stands for 2^(s - 127), and a cached value is its code
+ * times its page's scale.  Strides are in elements, of dimensions page, head and token (codes; the last dimension is
+ * contiguous) and page and head (scales).  A sequence's tokens lie in the pages its row of the block table names:
+ * position p in page table[p / page_size], row p % page_size.
+ * All strides must be >= 0; num_pages, heads, page_size, head_dim >= 1, num_pages * page_size < 2^31. */
+typedef struct tt_paged_cache {
+  void *k, *v;
+  void *k_scale, *v_scale;
+  int64_t k_strides[3], v_strides[3];
+  int64_t k_scale_strides[2], v_scale_strides[2];
+  int32_t num_pages, heads, page_size, head_dim;
+} tt_paged_cache;
+
+/* Block tables and slot maps from request lengths, on the device and in one launch.
+ * Sequence b holds ctx_lens[b] tokens and gets new_lens[b] more (either may be 0; a negative value counts as 0, and
+ * what does not fit the table's width of max_pages pages, or max_tokens in all, is dropped from the sequences' ends).
+ *   cu_new[b]   first row of sequence b among the packed new tokens; cu_new[B] = their number
+ *   lens[b]     ctx_lens[b] + the new tokens that were taken
+ *   block_table entries for the pages that ctx_lens[b] does not reach yet are taken from free_pages in sequence order,
+ *               from index *free_start (null: 0); earlier entries are read and stay as they are
+ *   slot_map[t] page * page_size + row of new token t; -1 for t >= cu_new[B] and for tokens without a page
+ *   free_end[0] *free_start + the pages that were needed; more than num_free says that the list ran out (the entries
+ *               and slots it could not fill are -1)
+ * The outputs must not overlap the inputs or each other.  grid = (B, 1, 1). */
+TTAMD_API int tt_paged_plan(const int32_t *ctx_lens, const int32_t *new_lens, int32_t *block_table,
+                  int64_t table_stride, int32_t B, int32_t max_pages, const int32_t *free_pages,
+                  int32_t num_free, const int32_t *free_start, int32_t page_size, int32_t max_tokens,
+                  int32_t *lens, int32_t *cu_new, int32_t *slot_map, int32_t *free_end,
+                  const uint32_t grid[3], void *stream);
+
+/* Writes new tokens into the cache: k, v [tokens, heads, head_dim] of dtype TT_BF16 or TT_F16 (strides of token and
+ * head in elements, the last dimension contiguous) at slot_map[t]; a slot outside the cache is skipped.
+ * A page's scale is the smallest power of two under which its largest finite magnitude is at most 448; tokens of the
+ * page before the first new one are kept, and rounded again where the scale grows, rows behind the new ones are left
+ * as they are.  A run that starts a page (row 0) starts its scale anew.  Codes are rounded to nearest even;
+ * infinities saturate, NaN stays NaN, and neither decides a scale.
+ * The slots of a page must be consecutive and in order in slot_map (as tt_paged_plan makes them), and a page may
+ * occur in one such run only: what two runs in one page leave there is undefined.  grid = (tokens, 1, 1). */
+TTAMD_API int tt_paged_write(const void *k, const void *v, const int64_t k_strides[2], const int64_t v_strides[2],
+                   const int32_t *slot_map, int32_t tokens, const tt_paged_cache *cache, int32_t dtype,
+                   const uint32_t grid[3], void *stream);
+
+/* Attention of packed queries q [tokens, heads_q, head_dim] (TT_BF16 or TT_F16; strides of token and head) over the
+ * cache: rows cu_q[b] .. cu_q[b+1]-1 belong to sequence b, which holds lens[b] keys.  heads_q is a multiple of
+ * cache->heads; query head h reads cache head h / (heads_q / heads).  With causal, query i of n attends the keys at
+ * positions <= lens[b] - n + i, otherwise all lens[b] keys; keys on a page outside the cache count as absent.  A query
+ * that attends no key gives 0 and lse = -inf.  o (strides as q's) has q's type; lse (null, or [tokens, heads_q]
+ * contiguous fp32) is the base-2 log-sum-exp of the scaled scores.  Rows outside every sequence are left as they are.
+ * max_q is an upper bound of the queries of one sequence; the rows of a sequence that has more are undefined.
+ * Scores, softmax and sums are fp32; the probabilities are rounded to fp16 for the product with V.
+ * workspace: tt_paged_attn_workspace(...) bytes, 16-byte aligned (null if that is 0), used by this call only until the
+ * stream has run it: calls that may overlap need one each.  grid = (tokens, heads_q, 1). */
+TTAMD_API int tt_paged_attn_workspace(int32_t B, int32_t max_pages, int32_t tokens, int32_t heads_q, int32_t max_q,
+                            const tt_paged_cache *cache, size_t *bytes);
+TTAMD_API int tt_paged_attn(const void *q, const int64_t q_strides[2], const tt_paged_cache *cache,
+                  const int32_t *block_table, int64_t table_stride, int32_t B, int32_t max_pages,
+                  const int32_t *lens, const int32_t *cu_q, int32_t tokens, int32_t heads_q, int32_t max_q,
+                  float sm_scale, int32_t causal, int32_t dtype, void *o, const int64_t o_strides[2],
+                  float *lse, void *workspace, size_t workspace_bytes, const uint32_t grid[3], void *stream);
 
 /* Diagnostic, no counterpart in the reference: what core clock does the part grant under the 16-bit macro-tile GEMM?
  * arm != 0 makes the NEXT launch of that kernel (tt_matmul_kernel_tma / _fused on a shape of whole 256x256x128 macro

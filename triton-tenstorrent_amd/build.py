@@ -23,9 +23,9 @@ LIB = PKG / "lib" / "libttamd_rt.so"
 CPUABI_LIB = PKG / "lib" / "libttamd_cpuabi.so"
 ARCH = "gfx950"
 
-CODE_OBJECTS = ["elementwise", "gemm", "attention", "reduce"]
+CODE_OBJECTS = ["elementwise", "gemm", "attention", "reduce", "paged"]
 RT_SOURCES = ["ttamd_rt.cpp", "tt_elementwise.cpp", "tt_gemm.cpp", "tt_attention.cpp", "tt_reduce.cpp",
-              "tt_reduce_static.hip"]
+              "tt_reduce_static.hip", "tt_paged.cpp"]
 
 # -packed-fp32-ops off: the compiler must not form v_pk_*_f32 on this target
 DEVICE_FLAGS = ["-O3", f"--offload-arch={ARCH}", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",

@@ -1,0 +1,303 @@
+// A paged key/value cache in 8 bits for gfx950: its plan (block tables and slot maps from request lengths), its
+// quantising write, and attention over it (paged_attn*.h).
+//
+// Cache: e4m3 codes [pages, heads, page_size, head_dim] for K and for V, and one scale for each (page, head), held as
+// its exponent: code s stands for 2^(s - 127).  A power of two costs e4m3 nothing (a floating-point code has the same
+// precision at every scale) and makes the change of a page's scale exact but for codes that become subnormal.
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "paged_args.h"
+
+namespace {
+
+constexpr int kMinScale = 27; // 2^-100: the scale of a page of zeros
+
+// ---------------------------------------------------------------------------
+// plan
+// ---------------------------------------------------------------------------
+// Inclusive scan over the 1024 threads of the workgroup; `add` is associative with identity 0.
+template <typename F> __device__ __forceinline__ uint32_t scan1024(uint32_t v, uint32_t *part, F add) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const uint32_t o = __shfl_up(v, d);
+    if (lane >= d) v = add(o, v);
+  }
+  __syncthreads(); // `part` may still be read from an earlier scan
+  if (lane == 63) part[wave] = v;
+  __syncthreads();
+  uint32_t before = 0;
+  for (int w = 0; w < wave; ++w) before = add(before, part[w]);
+  return add(before, v);
+}
+
+__device__ __forceinline__ int32_t clampi(int32_t v, int32_t lo, int32_t hi) { return v < lo ? lo : v > hi ? hi : v; }
+
+} // namespace
+
+// Every workgroup scans all sequences (the lengths are a few KB that the L2 holds) and then does its share of the
+// tokens, so that no workgroup waits for another.  Thread i owns `per` consecutive sequences; two scans, the tokens'
+// (saturating at max_tokens) and the pages'.  A new token at the start of a page writes that page's table entry.
+extern "C" __global__ __launch_bounds__(1024) void paged_plan(PagedPlanArgs a) {
+  __shared__ uint32_t part[16];
+  __shared__ int32_t tok0[1025], page0[1024]; // first token / first new page of thread i's sequences
+  const int tid = threadIdx.x;
+  const uint32_t cap = (uint32_t)a.max_tokens;
+  const int32_t P = a.page_size, width = a.max_pages * P;
+  const int per = (a.b + 1023) / 1024;
+  const int b0 = min(tid * per, a.b), b1 = min(b0 + per, a.b);
+  auto sat = [cap](uint32_t x, uint32_t y) { return min(x + y, cap); };
+  auto plus = [](uint32_t x, uint32_t y) { return x + y; };
+  auto ctx_of = [&](int b) { return clampi(a.ctx_lens[b], 0, width); };
+  auto fits_of = [&](int b, int32_t ctx) { return min((uint32_t)max(a.new_lens[b], 0), (uint32_t)(width - ctx)); };
+  auto pages_of = [P](int32_t n) { return (int32_t)(((uint32_t)n + (uint32_t)P - 1) / (uint32_t)P); };
+
+  uint32_t mine = 0;
+  for (int b = b0; b < b1; ++b) mine = sat(mine, min(fits_of(b, ctx_of(b)), cap));
+  const uint32_t incl = scan1024(mine, part, sat);
+  uint32_t total = 0;
+  for (int w = 0; w < 16; ++w) total = sat(total, part[w]);
+  // (saturated sums cannot be subtracted: the exclusive value comes from the left neighbour)
+  __syncthreads();
+  tok0[tid + 1] = (int32_t)incl;
+  if (tid == 0) tok0[0] = 0;
+  __syncthreads();
+  uint32_t cu = (uint32_t)tok0[tid];
+  const uint32_t cu_first = cu;
+  uint32_t fresh = 0;
+  for (int b = b0; b < b1; ++b) {
+    const int32_t ctx = ctx_of(b);
+    const uint32_t next = sat(cu, min(fits_of(b, ctx), cap));
+    fresh += (uint32_t)(pages_of(ctx + (int32_t)(next - cu)) - pages_of(ctx));
+    cu = next;
+  }
+  const uint32_t pincl = scan1024(fresh, part, plus);
+  const int32_t start = a.free_start ? a.free_start[0] : 0;
+  const int32_t pg = start + (int32_t)(pincl - fresh);
+  page0[tid] = pg;
+  __syncthreads();
+
+  if (blockIdx.x == 0) {
+    cu = cu_first;
+    for (int b = b0; b < b1; ++b) {
+      const int32_t ctx = ctx_of(b);
+      const uint32_t next = sat(cu, min(fits_of(b, ctx), cap));
+      a.cu_new[b] = (int32_t)cu;
+      a.lens[b] = ctx + (int32_t)(next - cu);
+      cu = next;
+    }
+    if (tid == 1023) {
+      a.cu_new[a.b] = (int32_t)total;
+      a.free_end[0] = start + (int32_t)pincl;
+    }
+  }
+
+  for (int64_t t64 = (int64_t)blockIdx.x * 1024 + tid; t64 < a.max_tokens; t64 += (int64_t)gridDim.x * 1024) {
+    const int32_t t = (int32_t)t64;
+    int32_t slot = -1;
+    if ((uint32_t)t < total) {
+      int lo = 0, hi = 1023; // the last thread whose first token is at most t
+      while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (tok0[mid] <= t) lo = mid; else hi = mid - 1;
+      }
+      int32_t c = tok0[lo], page = page0[lo];
+      int b = min(lo * per, a.b);
+      int32_t ctx = 0, n = 0;
+      const int be = min(b + per, a.b);
+      for (; b < be; ++b) {
+        ctx = ctx_of(b);
+        n = (int32_t)(sat((uint32_t)c, min(fits_of(b, ctx), cap)) - (uint32_t)c);
+        if (t < c + n) break;
+        c += n;
+        page += pages_of(ctx + n) - pages_of(ctx);
+      }
+      const int32_t pos = ctx + (t - c), blk = (int32_t)((uint32_t)pos / (uint32_t)P), had = pages_of(ctx);
+      int32_t *entry = a.table + (int64_t)b * a.table_stride + blk;
+      int32_t id;
+      if (blk >= had) {
+        const int32_t at = page + (blk - had);
+        id = at >= 0 && at < a.num_free ? a.free_pages[at] : -1;
+        if (pos == blk * P) *entry = id;
+      } else {
+        id = *entry;
+      }
+      const int64_t s = (int64_t)id * P + (pos - blk * P);
+      slot = id >= 0 && s <= INT32_MAX ? (int32_t)s : -1;
+    }
+    a.slots[t] = slot;
+  }
+}
+
+// ---------------------------------------------------------------------------
+// write
+// ---------------------------------------------------------------------------
+namespace {
+
+struct Bf16 {
+  static __device__ __forceinline__ float get(uint16_t h) { return __builtin_bit_cast(float, (uint32_t)h << 16); }
+};
+struct Fp16 {
+  static __device__ __forceinline__ float get(uint16_t h) { return (float)__builtin_bit_cast(_Float16, h); }
+};
+
+// bits of |x|, 0 for infinities and NaN: what does not decide a scale
+__device__ __forceinline__ uint32_t finite_mag(float x) {
+  const uint32_t u = __builtin_bit_cast(uint32_t, x) & 0x7fffffffu;
+  return u < 0x7f800000u ? u : 0u;
+}
+// smallest scale code s with amax <= 448 * 2^(s-127) = 1.75 * 2^(s-119), from the bits of amax
+__device__ __forceinline__ int scale_for(uint32_t amax) {
+  return max((int)(amax >> 23) - 8 + ((amax & 0x7fffffu) > 0x600000u ? 1 : 0), kMinScale);
+}
+__device__ __forceinline__ float pow2_code(int s) { return __builtin_bit_cast(float, (uint32_t)s << 23); }
+// saturating (an infinity becomes +-448), NaN stays NaN
+__device__ __forceinline__ float sat448(float y) { return y != y ? y : fminf(fmaxf(y, -448.0f), 448.0f); }
+__device__ __forceinline__ uint32_t max64(uint32_t v) {
+#pragma unroll
+  for (int d = 32; d; d >>= 1) v = max(v, (uint32_t)__shfl_xor((int)v, d));
+  return v;
+}
+
+// One wavefront writes the runs that begin among its `tile` tokens, for one head of K or of V.  A run is a stretch of
+// tokens whose slots follow one another inside one page: it has one scale.  Whatever the alignment: one element per
+// lane and step.
+template <typename E> __device__ __forceinline__ void write_any(const PagedWriteArgs &a) {
+  const int lane = threadIdx.x & 63;
+  const int64_t unit = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const bool isv = unit & 1;
+  const int head = (int)((unit >> 1) % a.c.heads);
+  const int64_t first = (unit >> 1) / a.c.heads * a.tile;
+  const int P = a.c.page_size, D = a.c.head_dim;
+  const int64_t nslots = (int64_t)a.c.pages * P;
+  const uint16_t *x = (isv ? a.v : a.k) + head * (isv ? a.v_head : a.k_head);
+  const int64_t x_tok = isv ? a.v_tok : a.k_tok;
+  for (int64_t t = first; t < min(first + a.tile, (int64_t)a.tokens); ++t) {
+    const int32_t slot = a.slots[t];
+    if (slot < 0 || slot >= nslots) continue;
+    const int row = slot % P;
+    const int64_t page = slot / P;
+    if (row && t && a.slots[t - 1] == slot - 1) continue; // inside a run that began before
+    int n = 1;
+    while (row + n < P && t + n < a.tokens && a.slots[t + n] == slot + n) ++n;
+    uint8_t *sp = (isv ? a.c.vs + page * a.c.vs_page + head * a.c.vs_head : a.c.ks + page * a.c.ks_page + head * a.c.ks_head);
+    uint8_t *base = isv ? a.c.v + page * a.c.v_page + head * a.c.v_head : a.c.k + page * a.c.k_page + head * a.c.k_head;
+    const int64_t c_tok = isv ? a.c.v_tok : a.c.k_tok;
+    uint32_t amax = 0;
+    for (int i = lane; i < n * D; i += 64) amax = max(amax, finite_mag(E::get(x[(t + i / D) * x_tok + i % D])));
+    amax = max64(amax);
+    int s = scale_for(amax);
+    if (row) {
+      const int old = *sp;
+      if (s > old) { // the tokens before the run go to the larger scale
+        const float f = pow2_code(max(127 + old - s, 0));
+        for (int i = lane; i < row * D; i += 64) {
+          uint8_t *p = base + (i / D) * c_tok + i % D;
+          const float y = __builtin_amdgcn_cvt_f32_fp8(*p, 0) * f;
+          *p = (uint8_t)__builtin_amdgcn_cvt_pk_fp8_f32(y, y, 0, false);
+        }
+      }
+      s = max(s, old);
+    }
+    const float inv = pow2_code(254 - s);
+    for (int i = lane; i < n * D; i += 64) {
+      const float y = sat448(E::get(x[(t + i / D) * x_tok + i % D]) * inv);
+      base[(row + i / D) * c_tok + i % D] = (uint8_t)__builtin_amdgcn_cvt_pk_fp8_f32(y, y, 0, false);
+    }
+    if (lane == 0) *sp = (uint8_t)s;
+  }
+}
+
+} // namespace
+
+extern "C" __global__ __launch_bounds__(256) void paged_write_any_bf16(PagedWriteArgs a) { write_any<Bf16>(a); }
+extern "C" __global__ __launch_bounds__(256) void paged_write_any_f16(PagedWriteArgs a) { write_any<Fp16>(a); }
+
+// ---------------------------------------------------------------------------
+// attention, any shape
+// ---------------------------------------------------------------------------
+namespace {
+
+// The sequence that owns packed row t, or -1: the last b with cu[b] <= t, if t is before its end.
+__device__ __forceinline__ int owner_of(const int32_t *cu, int b, int32_t t) {
+  int lo = 0, hi = b - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (cu[mid] <= t) lo = mid; else hi = mid - 1;
+  }
+  return cu[lo] <= t && t < cu[lo + 1] ? lo : -1;
+}
+
+// One wavefront per (row, query head): lane = key for the scores of 64 keys, lane = head dims lane, lane + 64, ... for
+// the sum over V.  Any page size, strides and head dim up to 256; everything in fp32.
+template <typename E> __device__ __forceinline__ void attn_any(const PagedAttnArgs &a, float *qs, uint16_t (*to_out)(float)) {
+  const int lane = threadIdx.x;
+  const int t = blockIdx.x, hq = blockIdx.y, D = a.c.head_dim, P = a.c.page_size, hk = hq / a.group;
+  const int b = owner_of(a.cu_q, a.b, t);
+  if (b < 0) return;
+  const int32_t len = min(max(a.lens[b], 0), (int32_t)min((int64_t)a.max_pages * P, (int64_t)INT32_MAX));
+  // keys the query sees: all, or those up to its own position len - n_q + (t - cu)
+  const int64_t last = a.causal ? (int64_t)len - ((int64_t)a.cu_q[b + 1] - t) : (int64_t)len - 1;
+  for (int d = lane; d < D; d += 64) qs[d] = E::get(a.q[t * a.q_tok + hq * a.q_head + d]) * a.qk_scale;
+  __syncthreads();
+  const int32_t *table = a.table + b * a.table_stride;
+  float m = -__builtin_inff(), l = 0.0f, acc[4] = {0, 0, 0, 0};
+  bool seen = false;
+  for (int64_t k0 = 0; k0 <= last; k0 += 64) {
+    const int64_t key = k0 + lane;
+    int32_t page = -1;
+    if (key <= last) page = table[key / P];
+    const bool live = page >= 0 && page < a.c.pages;
+    float s = -__builtin_inff(), vscale = 0.0f;
+    if (live) {
+      const uint8_t *kr = a.c.k + page * a.c.k_page + hk * a.c.k_head + (key % P) * a.c.k_tok;
+      float dot = 0.0f;
+      for (int d = 0; d < D; ++d) dot = fmaf(qs[d], __builtin_amdgcn_cvt_f32_fp8(kr[d], 0), dot);
+      s = dot * pow2_code(a.c.ks[page * a.c.ks_page + hk * a.c.ks_head]);
+      vscale = pow2_code(a.c.vs[page * a.c.vs_page + hk * a.c.vs_head]);
+    }
+    float top = s;
+#pragma unroll
+    for (int d = 32; d; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
+    if (!__any(live)) continue;
+    seen = true;
+    const float m_new = fmaxf(m, top);
+    const float p = live ? __builtin_amdgcn_exp2f(s - m_new) : 0.0f;
+    const float alpha = __builtin_amdgcn_exp2f(m - m_new);
+    l = l * alpha + p;
+    m = m_new;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) acc[r] *= alpha;
+    const int n = (int)min((int64_t)64, last - k0 + 1);
+    for (int j = 0; j < n; ++j) {
+      const int32_t pj = __shfl(page, j);
+      if (pj < 0 || pj >= a.c.pages) continue;
+      const float w = __shfl(p, j) * __shfl(vscale, j);
+      const uint8_t *vr = a.c.v + pj * a.c.v_page + hk * a.c.v_head + ((k0 + j) % P) * a.c.v_tok;
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        if (lane + r * 64 < D) acc[r] = fmaf(w, __builtin_amdgcn_cvt_f32_fp8(vr[lane + r * 64], 0), acc[r]);
+    }
+  }
+#pragma unroll
+  for (int d = 32; d; d >>= 1) l += __shfl_xor(l, d);
+#pragma unroll
+  for (int r = 0; r < 4; ++r)
+    if (lane + r * 64 < D) a.o[t * a.o_tok + hq * a.o_head + lane + r * 64] = to_out(seen ? acc[r] / l : 0.0f);
+  if (a.lse && lane == 0) a.lse[(int64_t)t * a.heads_q + hq] = seen ? m + __builtin_log2f(l) : -__builtin_inff();
+}
+
+__device__ __forceinline__ uint16_t out_bf16(float f) { return __builtin_bit_cast(uint16_t, (__bf16)f); }
+__device__ __forceinline__ uint16_t out_f16(float f) { return __builtin_bit_cast(uint16_t, (_Float16)f); }
+
+} // namespace
+
+extern "C" __global__ __launch_bounds__(64) void paged_attn_any_bf16(PagedAttnArgs a) {
+  __shared__ float qs[256];
+  attn_any<Bf16>(a, qs, out_bf16);
+}
+extern "C" __global__ __launch_bounds__(64) void paged_attn_any_f16(PagedAttnArgs a) {
+  __shared__ float qs[256];
+  attn_any<Fp16>(a, qs, out_f16);
+}

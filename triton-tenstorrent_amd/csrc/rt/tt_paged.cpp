@@ -1,0 +1,145 @@
+// tt_paged_plan, tt_paged_write, tt_paged_attn: launch validation and kernel selection for the paged 8-bit cache.
+#include <algorithm>
+#include <cmath>
+#include <cstring>
+
+#include "tt_internal.h"
+#include "../kernels/paged_args.h"
+
+using namespace ttamd;
+
+namespace {
+bool aligned(const void *p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
+
+int check_cache(const char *who, const tt_paged_cache *c, PagedCacheArgs *out) {
+  if (!c || !c->k || !c->v || !c->k_scale || !c->v_scale) return fail(RT_ERR_INVALID, "%s: null cache or cache pointer", who);
+  if (c->num_pages <= 0 || c->heads <= 0 || c->page_size <= 0 || c->head_dim <= 0)
+    return fail(RT_ERR_INVALID, "%s: cache of %d pages, %d heads, page size %d, head dim %d", who, c->num_pages, c->heads,
+                c->page_size, c->head_dim);
+  if ((int64_t)c->num_pages * c->page_size > INT32_MAX)
+    return fail(RT_ERR_UNSUPPORTED, "%s: num_pages * page_size exceeds int32", who);
+  if (c->head_dim > 256) return fail(RT_ERR_UNSUPPORTED, "%s: head dim %d (at most 256)", who, c->head_dim);
+  for (int i = 0; i < 3; ++i)
+    if (c->k_strides[i] < 0 || c->v_strides[i] < 0) return fail(RT_ERR_INVALID, "%s: negative cache stride", who);
+  for (int i = 0; i < 2; ++i)
+    if (c->k_scale_strides[i] < 0 || c->v_scale_strides[i] < 0) return fail(RT_ERR_INVALID, "%s: negative scale stride", who);
+  *out = {(uint8_t *)c->k, (uint8_t *)c->v, (uint8_t *)c->k_scale, (uint8_t *)c->v_scale,
+          c->k_strides[0], c->k_strides[1], c->k_strides[2], c->v_strides[0], c->v_strides[1], c->v_strides[2],
+          c->k_scale_strides[0], c->k_scale_strides[1], c->v_scale_strides[0], c->v_scale_strides[1],
+          c->num_pages, c->heads, c->page_size, c->head_dim};
+  return RT_OK;
+}
+
+int check_grid(const char *who, const uint32_t grid[3], int32_t x, int32_t y) {
+  if (!grid) return fail(RT_ERR_INVALID, "%s: null grid", who);
+  if (grid[0] != (uint32_t)x || grid[1] != (uint32_t)y || grid[2] != 1)
+    return fail(RT_ERR_INVALID, "%s: grid (%u,%u,%u), expected (%d,%d,1)", who, grid[0], grid[1], grid[2], x, y);
+  return RT_OK;
+}
+} // namespace
+
+extern "C" int tt_paged_plan(const int32_t *ctx_lens, const int32_t *new_lens, int32_t *block_table, int64_t table_stride,
+                             int32_t B, int32_t max_pages, const int32_t *free_pages, int32_t num_free,
+                             const int32_t *free_start, int32_t page_size, int32_t max_tokens, int32_t *lens,
+                             int32_t *cu_new, int32_t *slot_map, int32_t *free_end, const uint32_t grid[3], void *stream) {
+  const char *who = "paged_plan";
+  if (!props()) return fail(RT_ERR_NOT_INIT, "%s: call rt_init first", who);
+  if (B <= 0 || max_pages <= 0 || page_size <= 0 || num_free < 0 || max_tokens < 0)
+    return fail(RT_ERR_INVALID, "%s: B %d, max_pages %d, page_size %d, num_free %d, max_tokens %d", who, B, max_pages,
+                page_size, num_free, max_tokens);
+  if (!ctx_lens || !new_lens || !block_table || (num_free && !free_pages) || !lens || !cu_new || (max_tokens && !slot_map) ||
+      !free_end)
+    return fail(RT_ERR_INVALID, "%s: null pointer", who);
+  if (table_stride < max_pages) return fail(RT_ERR_INVALID, "%s: table stride %lld, %d entries", who, (long long)table_stride, max_pages);
+  if ((int64_t)max_pages * page_size > INT32_MAX) return fail(RT_ERR_UNSUPPORTED, "%s: max_pages * page_size exceeds int32", who);
+  if (B > (1 << 20)) return fail(RT_ERR_UNSUPPORTED, "%s: %d sequences (at most 2^20)", who, B);
+  for (const void *p : {(const void *)ctx_lens, (const void *)new_lens, (const void *)block_table, (const void *)free_pages,
+                        (const void *)free_start, (const void *)lens, (const void *)cu_new, (const void *)slot_map,
+                        (const void *)free_end})
+    if (!aligned(p, 4)) return fail(RT_ERR_INVALID, "%s: pointer not aligned to 4 bytes", who);
+  int rc;
+  if ((rc = check_grid(who, grid, B, 1))) return rc;
+  PagedPlanArgs a{ctx_lens, new_lens, block_table, free_pages, free_start, lens, cu_new, slot_map, free_end,
+                  table_stride, B, max_pages, num_free, page_size, max_tokens};
+  const uint32_t wgs = (uint32_t)std::clamp<int64_t>(cdiv64(max_tokens, 1024), 1, props()->multiprocessor_count);
+  void *args[] = {&a};
+  return launch("paged", "paged_plan", dim3(wgs), dim3(1024), 0, stream, args, 1);
+}
+
+extern "C" int tt_paged_write(const void *k, const void *v, const int64_t k_strides[2], const int64_t v_strides[2],
+                              const int32_t *slot_map, int32_t tokens, const tt_paged_cache *cache, int32_t dtype,
+                              const uint32_t grid[3], void *stream) {
+  const char *who = "paged_write";
+  if (!props()) return fail(RT_ERR_NOT_INIT, "%s: call rt_init first", who);
+  PagedWriteArgs a;
+  memset(&a, 0, sizeof(a));
+  int rc;
+  if ((rc = check_cache(who, cache, &a.c))) return rc;
+  if (dtype != TT_BF16 && dtype != TT_F16) return fail(RT_ERR_UNSUPPORTED, "%s: dtype %d (bf16 and fp16 are supported)", who, dtype);
+  if (tokens <= 0) return fail(RT_ERR_INVALID, "%s: %d tokens", who, tokens);
+  if (!k || !v || !k_strides || !v_strides || !slot_map) return fail(RT_ERR_INVALID, "%s: null pointer", who);
+  for (int i = 0; i < 2; ++i)
+    if (k_strides[i] < 0 || v_strides[i] < 0) return fail(RT_ERR_INVALID, "%s: negative stride", who);
+  if (!aligned(k, 2) || !aligned(v, 2) || !aligned(slot_map, 4)) return fail(RT_ERR_INVALID, "%s: misaligned pointer", who);
+  if ((rc = check_grid(who, grid, tokens, 1))) return rc;
+  a.k = (const uint16_t *)k; a.v = (const uint16_t *)v; a.slots = slot_map;
+  a.k_tok = k_strides[0]; a.k_head = k_strides[1]; a.v_tok = v_strides[0]; a.v_head = v_strides[1];
+  a.tokens = tokens;
+  a.tile = 1;
+  const int64_t units = cdiv64(tokens, a.tile) * a.c.heads * 2;
+  if (cdiv64(units, 4) > INT32_MAX) return fail(RT_ERR_UNSUPPORTED, "%s: tokens * heads exceeds the grid", who);
+  void *args[] = {&a};
+  return launch("paged", dtype == TT_BF16 ? "paged_write_any_bf16" : "paged_write_any_f16", dim3((uint32_t)cdiv64(units, 4)),
+                dim3(256), 0, stream, args, 1);
+}
+
+extern "C" int tt_paged_attn_workspace(int32_t B, int32_t max_pages, int32_t tokens, int32_t heads_q, int32_t max_q,
+                                       const tt_paged_cache *cache, size_t *bytes) {
+  const char *who = "paged_attn_workspace";
+  if (!props()) return fail(RT_ERR_NOT_INIT, "%s: call rt_init first", who);
+  if (!bytes) return fail(RT_ERR_INVALID, "%s: null out pointer", who);
+  PagedCacheArgs c;
+  int rc;
+  if ((rc = check_cache(who, cache, &c))) return rc;
+  if (B <= 0 || max_pages <= 0 || tokens <= 0 || heads_q <= 0 || max_q <= 0 || heads_q % c.heads)
+    return fail(RT_ERR_INVALID, "%s: B %d, max_pages %d, tokens %d, heads %d over %d, max_q %d", who, B, max_pages, tokens,
+                heads_q, c.heads, max_q);
+  *bytes = 0;
+  return RT_OK;
+}
+
+extern "C" int tt_paged_attn(const void *q, const int64_t q_strides[2], const tt_paged_cache *cache, const int32_t *block_table,
+                             int64_t table_stride, int32_t B, int32_t max_pages, const int32_t *lens, const int32_t *cu_q,
+                             int32_t tokens, int32_t heads_q, int32_t max_q, float sm_scale, int32_t causal, int32_t dtype,
+                             void *o, const int64_t o_strides[2], float *lse, void *workspace, size_t workspace_bytes,
+                             const uint32_t grid[3], void *stream) {
+  const char *who = "paged_attn";
+  if (!props()) return fail(RT_ERR_NOT_INIT, "%s: call rt_init first", who);
+  PagedAttnArgs a;
+  memset(&a, 0, sizeof(a));
+  size_t need = 0;
+  int rc;
+  if ((rc = check_cache(who, cache, &a.c))) return rc;
+  if ((rc = tt_paged_attn_workspace(B, max_pages, tokens, heads_q, max_q, cache, &need))) return rc;
+  if (dtype != TT_BF16 && dtype != TT_F16) return fail(RT_ERR_UNSUPPORTED, "%s: dtype %d (bf16 and fp16 are supported)", who, dtype);
+  if (!q || !q_strides || !o || !o_strides || !block_table || !lens || !cu_q) return fail(RT_ERR_INVALID, "%s: null pointer", who);
+  if (table_stride < max_pages) return fail(RT_ERR_INVALID, "%s: table stride %lld, %d entries", who, (long long)table_stride, max_pages);
+  if ((int64_t)max_pages * a.c.page_size > INT32_MAX) return fail(RT_ERR_UNSUPPORTED, "%s: max_pages * page_size exceeds int32", who);
+  for (int i = 0; i < 2; ++i)
+    if (q_strides[i] < 0 || o_strides[i] < 0) return fail(RT_ERR_INVALID, "%s: negative stride", who);
+  if (!aligned(q, 2) || !aligned(o, 2) || !aligned(block_table, 4) || !aligned(lens, 4) || !aligned(cu_q, 4) || !aligned(lse, 4))
+    return fail(RT_ERR_INVALID, "%s: misaligned pointer", who);
+  if (!std::isfinite(sm_scale)) return fail(RT_ERR_INVALID, "%s: sm_scale is not finite", who);
+  if (need && (!workspace || workspace_bytes < need || !aligned(workspace, 16)))
+    return fail(RT_ERR_INVALID, "%s: a 16-byte aligned workspace of %zu bytes is needed, got %zu", who, need, workspace ? workspace_bytes : 0);
+  if ((rc = check_grid(who, grid, tokens, heads_q))) return rc;
+  if (heads_q > 65535) return fail(RT_ERR_UNSUPPORTED, "%s: %d query heads (at most 65535)", who, heads_q);
+  a.q = (const uint16_t *)q; a.o = (uint16_t *)o; a.lse = lse;
+  a.table = block_table; a.lens = lens; a.cu_q = cu_q; a.table_stride = table_stride;
+  a.q_tok = q_strides[0]; a.q_head = q_strides[1]; a.o_tok = o_strides[0]; a.o_head = o_strides[1];
+  a.b = B; a.max_pages = max_pages; a.tokens = tokens; a.heads_q = heads_q; a.group = heads_q / a.c.heads;
+  a.causal = causal != 0; a.qk_scale = sm_scale * 1.44269504f;
+  void *args[] = {&a};
+  return launch("paged", dtype == TT_BF16 ? "paged_attn_any_bf16" : "paged_attn_any_f16",
+                dim3((uint32_t)tokens, (uint32_t)heads_q), dim3(64), 0, stream, args, 1);
+}

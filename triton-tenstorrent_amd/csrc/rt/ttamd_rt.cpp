@@ -38,6 +38,7 @@ TTAMD_EMBED(ttamd_co_elementwise, "elementwise.hsaco")
 TTAMD_EMBED(ttamd_co_gemm, "gemm.hsaco")
 TTAMD_EMBED(ttamd_co_attention, "attention.hsaco")
 TTAMD_EMBED(ttamd_co_reduce, "reduce.hsaco")
+TTAMD_EMBED(ttamd_co_paged, "paged.hsaco")
 
 struct rt_module_s {
   hipModule_t mod = nullptr;
@@ -160,7 +161,8 @@ int rt_init(int device) {
   const Img imgs[] = {{"elementwise", ttamd_co_elementwise_begin, ttamd_co_elementwise_end},
                       {"gemm", ttamd_co_gemm_begin, ttamd_co_gemm_end},
                       {"attention", ttamd_co_attention_begin, ttamd_co_attention_end},
-                      {"reduce", ttamd_co_reduce_begin, ttamd_co_reduce_end}};
+                      {"reduce", ttamd_co_reduce_begin, ttamd_co_reduce_end},
+                      {"paged", ttamd_co_paged_begin, ttamd_co_paged_end}};
   for (const Img &im : imgs) {
     auto *m = new rt_module_s();
     hipError_t e = hipModuleLoadData(&m->mod, im.b);

@@ -9,8 +9,13 @@ in the same order; host wrappers mirror the reference's own
 """
 from __future__ import annotations
 
+import ctypes
+import functools
+from typing import NamedTuple
 
 import torch
+
+from . import runtime as rt
 
 from .jit import Config, PrebuiltKernel
 from .tensor_descriptor import TensorDescriptor, is_tensor_descriptor
@@ -356,3 +361,95 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, causal: bool, s
                     HEAD_DIM=HEAD_DIM_K, FP8_OUTPUT=False, STAGE=stage, warp_specialize=warp_specialize,
                     IS_HOPPER=False, **meta)
     return (o, M) if return_lse else o
+
+
+# ---- a paged key/value cache in 8 bits --------------------------------------
+class PagedCache(NamedTuple):
+    """The cache of one layer.  ``k``, ``v``: e4m3 codes [pages, heads, page_size, head_dim] (any strides, the last
+    dimension contiguous); ``k_scale``, ``v_scale``: uint8 [pages, heads], exponents: code s stands for 2^(s - 127), and
+    a cached value is its code times its page's scale."""
+    k: torch.Tensor
+    v: torch.Tensor
+    k_scale: torch.Tensor
+    v_scale: torch.Tensor
+
+
+class PagedPlan(NamedTuple):
+    """What :func:`paged_plan` makes: ``lens`` [B] (cached + new tokens), ``cu_new`` [B+1] (rows of the packed new
+    tokens), ``slot_map`` [max_tokens] (page * page_size + row, -1 = none), ``free_end`` [1]."""
+    lens: torch.Tensor
+    cu_new: torch.Tensor
+    slot_map: torch.Tensor
+    free_end: torch.Tensor
+
+
+paged_plan_kernel = PrebuiltKernel("paged_plan_kernel", ["ctx_lens", "new_lens", "block_table", "free_pages", "free_start", "lens",
+                                                         "cu_new", "slot_map", "free_end", "PAGE_SIZE"], ["PAGE_SIZE"])
+paged_write_kernel = PrebuiltKernel("paged_write_kernel", ["k", "v", "slot_map", "k_cache", "v_cache", "k_scale", "v_scale"], [])
+paged_attn_kernel = PrebuiltKernel("paged_attn_kernel", ["q", "k_cache", "v_cache", "k_scale", "v_scale", "block_table", "lens",
+                                                         "cu_q", "out", "lse", "workspace", "sm_scale", "max_q", "CAUSAL"], ["CAUSAL"])
+
+
+def paged_cache(num_pages: int, heads: int, head_dim: int, page_size: int = 64, device="cuda") -> PagedCache:
+    """An empty cache.  Its codes start as they lie in memory: a page means something once :func:`paged_write` has
+    written it from its first row."""
+    shape = (num_pages, heads, page_size, head_dim)
+    return PagedCache(*(torch.empty(shape, dtype=torch.float8_e4m3fn, device=device) for _ in range(2)),
+                      *(torch.zeros(shape[:2], dtype=torch.uint8, device=device) for _ in range(2)))
+
+
+def paged_plan(ctx_lens: torch.Tensor, new_lens: torch.Tensor, block_table: torch.Tensor, free_pages: torch.Tensor,
+               page_size: int, max_tokens: int, free_start: torch.Tensor | None = None) -> PagedPlan:
+    """Plan one step on the GPU: sequence b holds ``ctx_lens[b]`` tokens and gets ``new_lens[b]`` more (int32 [B]).
+    ``block_table`` (int32 [B, max_pages]) is extended in place with pages from ``free_pages`` (int32), taken in sequence
+    order from index ``free_start`` (int32 [1]; None: 0).  ``max_tokens`` is the size of the slot map, at least the sum of
+    ``new_lens``; with a larger one the surplus slots are -1, so that a captured step serves batches of several sizes.
+    ``free_end`` is where the next step's ``free_start`` begins; past ``len(free_pages)`` it says that pages ran out."""
+    B = block_table.shape[0]
+    i32 = dict(dtype=torch.int32, device=block_table.device)
+    plan = PagedPlan(torch.empty(B, **i32), torch.empty(B + 1, **i32), torch.empty(max_tokens, **i32), torch.empty(1, **i32))
+    paged_plan_kernel[(B, )](ctx_lens, new_lens, block_table, free_pages, free_start, *plan, PAGE_SIZE=page_size)
+    return plan
+
+
+def paged_write(k: torch.Tensor, v: torch.Tensor, slot_map: torch.Tensor, cache: PagedCache) -> PagedCache:
+    """Quantise new tokens ``k``, ``v`` ([tokens, heads, head_dim], bf16 or fp16) into ``cache`` at ``slot_map``, in place.
+    A page's scale is the smallest power of two under which its largest magnitude is at most 448; where a new token makes
+    it grow, the page's earlier tokens are put to the new scale.  Slots of a page must be consecutive and in order, and
+    a page may occur once (as :func:`paged_plan` makes them); slots outside the cache are skipped."""
+    if k.shape[0]:
+        paged_write_kernel[(k.shape[0], )](k, v, slot_map, *cache)
+    return cache
+
+
+@functools.lru_cache(maxsize=256)
+def _paged_attn_workspace(device: int, B: int, max_pages: int, tokens: int, heads_q: int, max_q: int, shape: tuple) -> int:
+    n = ctypes.c_size_t()
+    lib = rt.init(device)
+    # (pointers and strides do not enter)
+    rt.check(lib.tt_paged_attn_workspace(B, max_pages, tokens, heads_q, max_q, rt.pack_paged_cache(1, 1, 1, 1, *([0] * 10), *shape),
+                                         ctypes.byref(n)))
+    return n.value
+
+
+def paged_attention(q: torch.Tensor, cache: PagedCache, block_table: torch.Tensor, lens: torch.Tensor, cu_q: torch.Tensor,
+                    sm_scale: float, max_q: int | None = None, causal: bool = True, return_lse: bool = False,
+                    out: torch.Tensor | None = None):
+    """Attention of packed queries ``q`` [tokens, heads_q, head_dim] (bf16 or fp16) over the cache.  Rows
+    ``cu_q[b]:cu_q[b+1]`` belong to sequence b with ``lens[b]`` keys (the new ones among them: write first, then attend).
+    ``causal``: query i of n attends the keys at positions <= lens[b] - n + i; otherwise all (an encoder's states).
+    ``heads_q`` is a multiple of the cache's heads.  ``max_q``: an upper bound of the queries of one sequence (None: the
+    number of rows); 1 for a decode step takes the kernel for single tokens.  A query without a key gives 0 (lse -inf);
+    rows outside every sequence are left as they are in ``out``.  Returns ``out``, or (``out``, lse [tokens, heads_q] in
+    base 2) with ``return_lse``."""
+    out = torch.empty(q.shape, dtype=q.dtype, device=q.device) if out is None else out
+    tokens, heads_q = q.shape[0], q.shape[1]
+    lse = torch.empty((tokens, heads_q), dtype=torch.float32, device=q.device) if return_lse else None
+    B, max_pages = block_table.shape
+    if tokens and B:
+        max_q = tokens if max_q is None else max_q
+        need = _paged_attn_workspace(q.get_device(), B, max_pages, tokens, heads_q, max_q, tuple(cache.k.shape)) if q.is_cuda else 0
+        workspace = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+        paged_attn_kernel[(tokens, heads_q)](q, *cache, block_table, lens, cu_q, out, lse, workspace, float(sm_scale), max_q,
+                                             CAUSAL=bool(causal))
+    return (out, lse) if return_lse else out

@@ -6,6 +6,7 @@ device is present, every entry point raises.
 from __future__ import annotations
 
 import ctypes as C
+import struct
 import threading
 from pathlib import Path
 
@@ -66,6 +67,12 @@ Grid3 = C.c_uint32 * 3
 _vp, _i32, _f32 = C.c_void_p, C.c_int32, C.c_float
 _DP = C.POINTER(tt_desc2d)
 _G = C.POINTER(C.c_uint32)
+_i64 = C.c_int64
+# a tt_paged_cache and arrays of strides are handed over as packed bytes (built in one call, where filling a ctypes
+# structure field by field costs several microseconds a launch)
+pack_paged_cache = struct.Struct("=4Q10q4i").pack     # k, v, k_scale, v_scale; page, head, token strides of k and v, page
+#                                                       and head strides of the scales; pages, heads, page size, head dim
+pack_strides2 = struct.Struct("=2q").pack
 SYMBOLS = {
     "rt_init": (C.c_int, [C.c_int]),
     "rt_device_count": (C.c_int, [C.POINTER(C.c_int)]),
@@ -103,6 +110,11 @@ SYMBOLS = {
     "tt_matmul_kernel_tma_fp8_scaled": (C.c_int, [_DP, _DP, _DP, _i32, _i32, _i32, _f32, _f32, _i32, _i32, _i32, _i32, _G, _vp]),
     "tt_matmul_kernel": (C.c_int, [_vp, _vp, _vp, _i32, _i32, _i32] + [C.c_int64] * 6 + [_i32] * 6 + [_G, _vp]),
     "tt_attn_fwd": (C.c_int, [_f32, _vp, _i32, _i32, _DP, _DP, _DP, _DP, _i32, _i32, _i32, _i32, _i32, _G, _vp]),
+    "tt_paged_plan": (C.c_int, [_vp, _vp, _vp, _i64, _i32, _i32, _vp, _i32, _vp, _i32, _i32, _vp, _vp, _vp, _vp, _G, _vp]),
+    "tt_paged_write": (C.c_int, [_vp, _vp, _vp, _vp, _vp, _i32, _vp, _i32, _G, _vp]),
+    "tt_paged_attn_workspace": (C.c_int, [_i32, _i32, _i32, _i32, _i32, _vp, C.POINTER(C.c_size_t)]),
+    "tt_paged_attn": (C.c_int, [_vp, _vp, _vp, _vp, _i64, _i32, _i32, _vp, _vp, _i32, _i32, _i32, _f32, _i32, _i32, _vp, _vp,
+                                _vp, _vp, C.c_size_t, _G, _vp]),
     "tt_last_kernel_name": (C.c_char_p, []),
     "rt_gemm_clock_probe": (C.c_int, [_i32, C.POINTER(C.c_uint64)]),
 }
