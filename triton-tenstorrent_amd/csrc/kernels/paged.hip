@@ -301,3 +301,5 @@ extern "C" __global__ __launch_bounds__(64) void paged_attn_any_f16(PagedAttnArg
   __shared__ float qs[256];
   attn_any<Fp16>(a, qs, out_f16);
 }
+
+#include "paged_attn_one.h"

@@ -39,4 +39,8 @@ struct PagedAttnArgs {
   int32_t b, max_pages, tokens, heads_q, group; // group = heads_q / heads
   int32_t causal;
   float qk_scale;    // sm_scale * log2(e)
+  uint64_t page_magic;  // ceil(2^36 / (page_size / 16)): n / (page_size / 16) = (n * page_magic) >> 36 for n < 2^27,
+                        // page_size <= 8192
+  float *part;          // partial results of split sequences
+  int32_t split_groups; // workgroups of the launch that left them
 };

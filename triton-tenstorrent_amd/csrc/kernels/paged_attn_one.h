@@ -1,0 +1,489 @@
+// Attention over the paged cache, one query of each sequence (decode).
+//
+// What bounds it: one pass over the cached codes, HBM.  A wavefront owns all query heads of one cache head (rows of an
+// MFMA tile; a group of fewer than 16 leaves rows empty, which costs nothing here) and streams keys from global memory
+// into registers, with no LDS between: every code is used once, by one wavefront.
+//   S^T[key, q] = K . Q^T       v_mfma_f32_16x16x32, A = 16 rows of K, B = Q; lane l ends with query l%16, keys (l/16)*4+r
+//   O^T[d, q]  += V^T . P^T     B = P^T is what the lane already holds; A = V^T, whose lane needs 8 keys of one d: it loads
+//                               D/16 consecutive codes of each of its keys and pairs neighbouring keys' bytes with
+//                               v_perm_b32, one for two conversions.  MFMA number i takes the lanes' i-th code, so its
+//                               row l%16 stands for d = (l%16) * D/16 + i.
+// e4m3 -> 16 bits is v_cvt_scalef32_pk_{bf16,f16}_fp8 (exact): K without its scale, which joins the factor on the scores;
+// V with its page's scale relative to the largest met so far (`eref`, the accumulator follows when it grows), in fp16,
+// like the probabilities: 11 bits where bf16 has 8, and the accumulator's power of two keeps the range.
+//
+// Split: the keys of all sequences, in units of 64 * NS, are dealt evenly to the workgroups of a grid that fills the chip
+// once, whatever the lengths: workgroup i takes units [i U / G, (i+1) U / G) and meets at most two (sequence, head)
+// pairs that it does not have whole, the first and the last.  Those leave partial results (fp32 sum, reference, sum of
+// probabilities) in the workspace and paged_attn_join adds them in order, so results do not change from run to run.
+#pragma once
+
+namespace one {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+
+constexpr float kLift = 8.0f;  // probabilities are held times 2^8: fp16 then reaches down to 2^-32 of the reference
+constexpr float kLazy = 7.0f;  // the reference follows a row's maximum when that is 2^7 above it: at most 2^15 < 65504
+constexpr float kInf = __builtin_inff();
+
+template <int D, int MT> constexpr int subtiles() { return D * MT >= 256 ? 2 : 4; } // of 16 keys, per wavefront and step
+
+// Units of work of sequence b: n = 0 where it is not this kernel's (no query, or several).
+struct Seq { int32_t len, units; };
+template <int UK> __device__ __forceinline__ Seq seq_of(const PagedAttnArgs &a, int b) {
+  const int32_t q0 = a.cu_q[b], q1 = a.cu_q[b + 1];
+  const int32_t len = clampi(a.lens[b], 0, a.max_pages * a.c.page_size);
+  const bool mine = q1 - q0 == 1 && q0 >= 0 && q0 < a.tokens;
+  return {len, mine ? max((len + UK - 1) / UK, 1) : 0};
+}
+
+// Prefix sums of the units of all sequences, in LDS: base[i] = units before thread i's `per` consecutive sequences.
+template <int UK> __device__ __forceinline__ int scan_units(const PagedAttnArgs &a, int32_t *base, int32_t *part) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, per = (a.b + 255) / 256;
+  int32_t n = 0;
+  for (int b = min(tid * per, a.b); b < min(tid * per + per, a.b); ++b) n += seq_of<UK>(a, b).units;
+  int32_t v = n;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int32_t o = __shfl_up(v, d);
+    if (lane >= d) v += o;
+  }
+  if (lane == 63) part[wave] = v;
+  __syncthreads();
+  for (int w = 0; w < wave; ++w) v += part[w];
+  base[tid] = v - n;
+  const int total = part[0] + part[1] + part[2] + part[3];
+  __syncthreads();
+  return total;
+}
+
+struct Bf {
+  typedef bf16x8 frag;
+  static __device__ __forceinline__ f32x4 mfma(frag x, frag y, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, y, c, 0, 0, 0); }
+  static __device__ __forceinline__ frag codes(uint32_t lo, uint32_t hi) {
+    const u32x4 r = {__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, false)),
+                     __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, true)),
+                     __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, false)),
+                     __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, true))};
+    return __builtin_bit_cast(frag, r);
+  }
+  static __device__ __forceinline__ uint16_t out(float f) { return out_bf16(f); }
+};
+struct Hf {
+  typedef f16x8 frag;
+  static __device__ __forceinline__ f32x4 mfma(frag x, frag y, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(x, y, c, 0, 0, 0); }
+  static __device__ __forceinline__ frag codes(uint32_t lo, uint32_t hi) {
+    const u32x4 r = {__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.0f, false)),
+                     __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.0f, true)),
+                     __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.0f, false)),
+                     __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.0f, true))};
+    return __builtin_bit_cast(frag, r);
+  }
+  static __device__ __forceinline__ uint16_t out(float f) { return out_f16(f); }
+};
+
+__device__ __forceinline__ int64_t uniform64(int64_t v) {
+  return (int64_t)(((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32) |
+                   (uint32_t)__builtin_amdgcn_readfirstlane((int)v));
+}
+__device__ __forceinline__ int64_t lane64(int32_t lo, int32_t hi, int lane) {
+  return (int64_t)(((uint64_t)(uint32_t)__builtin_amdgcn_readlane(hi, lane) << 32) | (uint32_t)__builtin_amdgcn_readlane(lo, lane));
+}
+
+// Partial result p of the workspace: rows * D sums, then rows pairs (reference, sum), then the sums' exponent.
+template <int D, int MT> constexpr int part_floats() { return 16 * MT * D + 32 * MT + 4; }
+
+template <class E, int D, int MT>
+__device__ __forceinline__ void body(const PagedAttnArgs &a, float *lds) {
+  constexpr int NS = subtiles<D, MT>(), UK = 64 * NS, KL = D / 64, VW = D / 64; // 16-byte loads of K, dwords of V per row
+  constexpr int VB = D / 16, IB = 64 / NS, LD = D + 4;                      // LD: padded LDS row of the merge
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int c16 = lane & 15, g = lane >> 4;
+  int32_t *base = (int32_t *)lds, *part = base + 256;
+  const int64_t U = (int64_t)scan_units<UK>(a, base, part) * a.c.heads;
+  const int64_t G = min((int64_t)gridDim.x, U); // fewer units than workgroups: one each
+  if (blockIdx.x >= G) return;
+  int64_t u = blockIdx.x * U / G;
+  const int64_t u_end = (blockIdx.x + 1) * U / G, u_first = u;
+
+  // the sequence that holds unit u
+  const int per = (a.b + 255) / 256;
+  int lo = 0, hi = 255;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if ((int64_t)base[mid] * a.c.heads <= u) lo = mid; else hi = mid - 1;
+  }
+  int b = __builtin_amdgcn_readfirstlane(min(lo * per, a.b - 1));
+  int64_t before = uniform64((int64_t)base[lo] * a.c.heads);
+  __syncthreads(); // `base` shares its LDS with the merge
+  Seq sq = seq_of<UK>(a, b);
+  while (before + (int64_t)sq.units * a.c.heads <= u) {
+    before += (int64_t)sq.units * a.c.heads;
+    sq = seq_of<UK>(a, ++b);
+  }
+
+  const uint32_t klane = (uint32_t)(c16 * a.c.k_tok + g * 16);
+  uint32_t vlane[4];
+#pragma unroll
+  for (int r = 0; r < 4; ++r) vlane[r] = (uint32_t)((g * 4 + r) * a.c.v_tok + c16 * VB);
+
+  while (u < u_end) {
+    while (sq.units == 0 || before + (int64_t)sq.units * a.c.heads <= u) { // (u < U: ends before b does)
+      before += (int64_t)sq.units * a.c.heads;
+      sq = seq_of<UK>(a, ++b);
+    }
+    const int32_t len = sq.len, units = sq.units;
+    const int hk = (int)((u - before) / units);
+    const int c0 = (int)(u - before - (int64_t)hk * units);
+    const int n = (int)min((int64_t)(units - c0), u_end - u);
+    const int32_t t = a.cu_q[b];
+    const int32_t *table = a.table + (int64_t)b * a.table_stride;
+    const uint8_t *kh = a.c.k + hk * a.c.k_head, *vh = a.c.v + hk * a.c.v_head;
+
+    typename E::frag qf[MT][2 * KL];
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+      const int row = m * 16 + c16;
+      const uint16_t *qr = a.q + t * a.q_tok + (hk * a.group + row) * a.q_head + g * 16;
+#pragma unroll
+      for (int s = 0; s < 2 * KL; ++s) {
+        u32x4 z = {0, 0, 0, 0};
+        if (row < a.group) z = *(const u32x4 *)(qr + (s >> 1) * 64 + (s & 1) * 8);
+        qf[m][s] = __builtin_bit_cast(typename E::frag, z);
+      }
+    }
+
+    f32x4 acc[MT][VB];
+    float mref[MT], lsum[MT];
+    int eref = 0;
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+      mref[m] = -kInf;
+      lsum[m] = 0.0f;
+#pragma unroll
+      for (int i = 0; i < VB; ++i) acc[m][i] = (f32x4){0, 0, 0, 0};
+    }
+
+    // What lane (it % IB) * NS + s knows of subtile s of step it: where its rows lie, how many count, its scales.
+    int32_t ko_lo, ko_hi, vo_lo, vo_hi, live, vcode;
+    float kscale;
+    auto batch = [&](int it0) {
+      const int64_t key = (int64_t)(c0 + it0 + lane / NS) * UK + wave * (16 * NS) + (lane % NS) * 16;
+      const uint32_t sub = (uint32_t)(key >> 4);
+      const uint32_t blk = (uint32_t)(((uint64_t)sub * a.page_magic) >> 36);
+      int32_t page = key < len ? table[blk] : -1;
+      const bool ok = page >= 0 && page < a.c.pages;
+      page = ok ? page : 0;
+      const int64_t row = ok ? ((int64_t)sub - (int64_t)blk * (a.c.page_size >> 4)) * 16 : 0;
+      const int64_t ko = page * a.c.k_page + row * a.c.k_tok, vo = page * a.c.v_page + row * a.c.v_tok;
+      ko_lo = (int32_t)ko; ko_hi = (int32_t)(ko >> 32); vo_lo = (int32_t)vo; vo_hi = (int32_t)(vo >> 32);
+      live = ok ? (int32_t)min((int64_t)len - key, (int64_t)16) : 0;
+      kscale = pow2_code(a.c.ks[page * a.c.ks_page + hk * a.c.ks_head]) * a.qk_scale;
+      vcode = ok ? a.c.vs[page * a.c.vs_page + hk * a.c.vs_head] : 0;
+    };
+
+    u32x4 kr[NS][KL];
+    uint32_t vr[NS][4][VW];
+    auto load_k = [&](int it) {
+#pragma unroll
+      for (int s = 0; s < NS; ++s) {
+        const uint8_t *kp = kh + lane64(ko_lo, ko_hi, (it % IB) * NS + s);
+#pragma unroll
+        for (int h = 0; h < KL; ++h) kr[s][h] = *(const u32x4 *)(kp + klane + h * 64);
+      }
+    };
+    auto load_v = [&](int it) {
+#pragma unroll
+      for (int s = 0; s < NS; ++s) {
+        const uint8_t *vp = vh + lane64(vo_lo, vo_hi, (it % IB) * NS + s);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          if constexpr (VW == 1) vr[s][r][0] = *(const uint32_t *)(vp + vlane[r]);
+          if constexpr (VW == 2) {
+            const u32x2 x = *(const u32x2 *)(vp + vlane[r]);
+            vr[s][r][0] = x[0]; vr[s][r][1] = x[1];
+          }
+          if constexpr (VW == 4) {
+            const u32x4 x = *(const u32x4 *)(vp + vlane[r]);
+            vr[s][r][0] = x[0]; vr[s][r][1] = x[1]; vr[s][r][2] = x[2]; vr[s][r][3] = x[3];
+          }
+        }
+      }
+    };
+
+    // one set of registers each for K and V: a step's loads go out as soon as the step before has used them up
+    batch(0);
+    load_k(0);
+    load_v(0);
+    for (int it = 0; it < n; ++it) {
+      int nv[NS], vc[NS];
+      float ks[NS];
+      int nmin = 16, emax = 0;
+#pragma unroll
+      for (int s = 0; s < NS; ++s) {
+        const int src = (it % IB) * NS + s;
+        nv[s] = __builtin_amdgcn_readlane(live, src);
+        vc[s] = __builtin_amdgcn_readlane(vcode, src);
+        ks[s] = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, kscale), src));
+        nmin = min(nmin, nv[s]);
+        emax = max(emax, vc[s]);
+      }
+      // scores
+      f32x4 st[MT][NS];
+#pragma unroll
+      for (int s = 0; s < NS; ++s) {
+#pragma unroll
+        for (int m = 0; m < MT; ++m) st[m][s] = (f32x4){0, 0, 0, 0};
+#pragma unroll
+        for (int h = 0; h < KL; ++h)
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            const typename E::frag kf = E::codes(kr[s][h][2 * c], kr[s][h][2 * c + 1]);
+#pragma unroll
+            for (int m = 0; m < MT; ++m) st[m][s] = E::mfma(kf, qf[m][h * 2 + c], st[m][s]);
+          }
+#pragma unroll
+        for (int m = 0; m < MT; ++m) st[m][s] *= ks[s];
+      }
+      if (it + 1 < n) {
+        if ((it + 1) % IB == 0) batch(it + 1);
+        load_k(it + 1);
+      }
+      if (nmin < 16) { // rows behind the end or on no page: their scores count for nothing, their V must not be NaN
+#pragma unroll
+        for (int s = 0; s < NS; ++s)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const bool in = g * 4 + r < nv[s];
+#pragma unroll
+            for (int m = 0; m < MT; ++m) st[m][s][r] = in ? st[m][s][r] : -kInf;
+#pragma unroll
+            for (int w = 0; w < VW; ++w) vr[s][r][w] = in ? vr[s][r][w] : 0;
+          }
+      }
+      // the reference, and the largest V scale
+      float top[MT];
+      bool grow = false;
+#pragma unroll
+      for (int m = 0; m < MT; ++m) {
+        top[m] = -kInf;
+#pragma unroll
+        for (int s = 0; s < NS; ++s)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) top[m] = fmaxf(top[m], st[m][s][r]);
+        grow |= top[m] > mref[m] + kLazy;
+      }
+      if (__any(grow) || emax > eref) {
+        const float ve = __builtin_amdgcn_ldexpf(1.0f, min(eref - emax, 0));
+        eref = max(eref, emax);
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+          float x = fmaxf(top[m], __shfl_xor(top[m], 16));
+          x = fmaxf(x, __shfl_xor(x, 32));
+          const float mn = fmaxf(mref[m], x);
+          const float al = mn == -kInf ? 1.0f : __builtin_amdgcn_exp2f(mref[m] - mn);
+          mref[m] = mn;
+          lsum[m] *= al;
+#pragma unroll
+          for (int i = 0; i < VB; ++i) acc[m][i] *= al * ve;
+        }
+      }
+      f16x8 pf[MT][NS / 2];
+#pragma unroll
+      for (int m = 0; m < MT; ++m) {
+        const float ref = (mref[m] == -kInf ? 0.0f : mref[m]) - kLift;
+#pragma unroll
+        for (int s = 0; s < NS; ++s)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const float p = __builtin_amdgcn_exp2f(st[m][s][r] - ref);
+            lsum[m] += p;
+            pf[m][s >> 1][(s & 1) * 4 + r] = (_Float16)p;
+          }
+      }
+      // the sum over V
+      float vs[NS];
+#pragma unroll
+      for (int s = 0; s < NS; ++s) vs[s] = __builtin_bit_cast(float, (uint32_t)max(vc[s] - eref + 127, 0) << 23);
+#pragma unroll
+      for (int p = 0; p < NS / 2; ++p)
+#pragma unroll
+        for (int w = 0; w < VW; ++w) {
+          uint32_t f[4][4]; // [code of the dword][pair of keys]
+#pragma unroll
+          for (int j = 0; j < 4; ++j) { // pairs: rows 0-1 and 2-3 of subtile 2p, then of 2p + 1
+            const int s = 2 * p + (j >> 1), r = (j & 1) * 2;
+            const uint32_t x = __builtin_amdgcn_perm(vr[s][r + 1][w], vr[s][r][w], 0x05010400);
+            const uint32_t y = __builtin_amdgcn_perm(vr[s][r + 1][w], vr[s][r][w], 0x07030602);
+            f[0][j] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x, vs[s], false));
+            f[1][j] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x, vs[s], true));
+            f[2][j] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(y, vs[s], false));
+            f[3][j] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(y, vs[s], true));
+          }
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const u32x4 x = {f[i][0], f[i][1], f[i][2], f[i][3]};
+#pragma unroll
+            for (int m = 0; m < MT; ++m)
+              acc[m][w * 4 + i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, x), pf[m][p], acc[m][w * 4 + i], 0, 0, 0);
+          }
+        }
+      if (it + 1 < n) load_v(it + 1);
+    }
+
+    // ---- merge the four wavefronts ----
+    float *wo = lds, *wml = lds + 4 * 16 * MT * LD;   // sums [wave][row][LD], (reference, sum) [wave][row], exponents [wave]
+    int32_t *we = (int32_t *)(wml + 4 * 16 * MT * 2);
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+      float l = lsum[m];
+      l += __shfl_xor(l, 16);
+      l += __shfl_xor(l, 32);
+      const int row = wave * 16 * MT + m * 16 + c16;
+      if (g == 0) { wml[row * 2] = mref[m]; wml[row * 2 + 1] = l; }
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int i = 0; i < VB; i += 4)
+          *(f32x4 *)(wo + row * LD + (g * 4 + r) * VB + i) = (f32x4){acc[m][i][r], acc[m][i + 1][r], acc[m][i + 2][r], acc[m][i + 3][r]};
+    }
+    if (lane == 0) we[wave] = eref;
+    __syncthreads();
+    const bool whole = c0 == 0 && n == units;
+    const int e = max(max(we[0], we[1]), max(we[2], we[3]));
+    // (the first segment of this workgroup takes slot 0, a later one that is not whole can only be its last: slot 1)
+    float *slot = a.part + (2 * (int64_t)blockIdx.x + (u == u_first ? 0 : 1)) * part_floats<D, MT>();
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+      const int row = m * 16 + (tid >> 4), d0 = (tid & 15) * VB;
+      float mx = -kInf;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) mx = fmaxf(mx, wml[(w * 16 * MT + row) * 2]);
+      const float mm = mx == -kInf ? 0.0f : mx;
+      float l = 0.0f, o[VB];
+#pragma unroll
+      for (int i = 0; i < VB; ++i) o[i] = 0.0f;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const float mw = wml[(w * 16 * MT + row) * 2];
+        const float f = mw == -kInf ? 1.0f : __builtin_amdgcn_exp2f(mw - mm); // (a row of NaN scores has reference -inf)
+        l += wml[(w * 16 * MT + row) * 2 + 1] * f;
+        const float fe = f * __builtin_amdgcn_ldexpf(1.0f, we[w] - e);
+#pragma unroll
+        for (int i = 0; i < VB; ++i) o[i] += wo[(w * 16 * MT + row) * LD + d0 + i] * fe;
+      }
+      if (whole) {
+        if (row < a.group) {
+          const int hq = hk * a.group + row;
+          const bool none = l == 0.0f && mx == -kInf;
+          const float inv = none ? 0.0f : 1.0f / l;
+          uint16_t *op = a.o + t * a.o_tok + hq * a.o_head + d0;
+#pragma unroll
+          for (int i = 0; i < VB; i += 2)
+            *(uint32_t *)(op + i) = (uint32_t)E::out(__builtin_amdgcn_ldexpf(o[i] * inv, e - 127)) |
+                                    (uint32_t)E::out(__builtin_amdgcn_ldexpf(o[i + 1] * inv, e - 127)) << 16;
+          if (a.lse && d0 == 0) a.lse[(int64_t)t * a.heads_q + hq] = none ? -kInf : mx - kLift + __builtin_log2f(l);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < VB; i += 4) *(f32x4 *)(slot + row * D + d0 + i) = (f32x4){o[i], o[i + 1], o[i + 2], o[i + 3]};
+        if (d0 == 0) {
+          slot[16 * MT * D + row * 2] = mx;
+          slot[16 * MT * D + row * 2 + 1] = l;
+          if (row == 0) ((int32_t *)slot)[16 * MT * D + 32 * MT] = e;
+        }
+      }
+    }
+    __syncthreads();
+    u += n;
+  }
+}
+
+// Joins the partial results of one (sequence, head): grid (b, heads).
+template <class E, int D, int MT> __device__ __forceinline__ void join(const PagedAttnArgs &a, int32_t *base) {
+  constexpr int NS = subtiles<D, MT>(), UK = 64 * NS, VB = D / 16;
+  const int b = blockIdx.x, hk = blockIdx.y, tid = threadIdx.x;
+  const Seq sq = seq_of<UK>(a, b);
+  if (sq.units <= 1) return; // one unit, or none, is never split
+  const int64_t U = (int64_t)scan_units<UK>(a, base, base + 256) * a.c.heads;
+  const int64_t G = min((int64_t)a.split_groups, U);
+  const int per = (a.b + 255) / 256, th = b / per;
+  int64_t first = base[th];
+  for (int x = th * per; x < b; ++x) first += seq_of<UK>(a, x).units;
+  first = first * a.c.heads + (int64_t)hk * sq.units;
+  // the workgroups that own its first and its last unit
+  auto owner = [&](int64_t u) { return ((u + 1) * G + U - 1) / U - 1; };
+  const int64_t i0 = owner(first), i1 = owner(first + sq.units - 1);
+  if (i0 == i1) return;
+  const int64_t s0 = 2 * i0 + (i0 * U / G < first ? 1 : 0);
+  auto slot = [&](int64_t i) { return a.part + (i == i0 ? s0 : 2 * i) * part_floats<D, MT>(); };
+  const int32_t t = a.cu_q[b];
+#pragma unroll
+  for (int m = 0; m < MT; ++m) {
+    const int row = m * 16 + (tid >> 4), d0 = (tid & 15) * VB;
+    if (row >= a.group) continue;
+    float mx = -kInf;
+    int e = 0;
+    for (int64_t i = i0; i <= i1; ++i) {
+      mx = fmaxf(mx, slot(i)[16 * MT * D + row * 2]);
+      e = max(e, ((const int32_t *)slot(i))[16 * MT * D + 32 * MT]);
+    }
+    const float mm = mx == -kInf ? 0.0f : mx;
+    float l = 0.0f, o[VB];
+#pragma unroll
+    for (int i = 0; i < VB; ++i) o[i] = 0.0f;
+    for (int64_t i = i0; i <= i1; ++i) {
+      const float *p = slot(i);
+      const float mw = p[16 * MT * D + row * 2];
+      const float f = mw == -kInf ? 1.0f : __builtin_amdgcn_exp2f(mw - mm);
+      l += p[16 * MT * D + row * 2 + 1] * f;
+      const float fe = f * __builtin_amdgcn_ldexpf(1.0f, ((const int32_t *)p)[16 * MT * D + 32 * MT] - e);
+#pragma unroll
+      for (int j = 0; j < VB; j += 4) {
+        const f32x4 x = *(const f32x4 *)(p + row * D + d0 + j);
+        o[j] += x[0] * fe; o[j + 1] += x[1] * fe; o[j + 2] += x[2] * fe; o[j + 3] += x[3] * fe;
+      }
+    }
+    const int hq = hk * a.group + row;
+    const bool none = l == 0.0f && mx == -kInf;
+    const float inv = none ? 0.0f : 1.0f / l;
+    uint16_t *op = a.o + t * a.o_tok + hq * a.o_head + d0;
+#pragma unroll
+    for (int i = 0; i < VB; i += 2)
+      *(uint32_t *)(op + i) = (uint32_t)E::out(__builtin_amdgcn_ldexpf(o[i] * inv, e - 127)) |
+                              (uint32_t)E::out(__builtin_amdgcn_ldexpf(o[i + 1] * inv, e - 127)) << 16;
+    if (a.lse && d0 == 0) a.lse[(int64_t)t * a.heads_q + hq] = none ? -kInf : mx - kLift + __builtin_log2f(l);
+  }
+}
+
+template <int D, int MT> constexpr int lds_floats() {
+  return 4 * 16 * MT * (D + 4) + 4 * 16 * MT * 2 + 4 > 264 ? 4 * 16 * MT * (D + 4) + 4 * 16 * MT * 2 + 4 : 264;
+}
+
+} // namespace one
+
+#define PAGED_ONE(T, E, D, MT)                                                                                \
+  extern "C" __global__ __launch_bounds__(256, 2) void paged_attn_one_##T##_d##D##_r##MT(PagedAttnArgs a) {    \
+    __shared__ __align__(16) float lds[one::lds_floats<D, MT>()];                                             \
+    one::body<one::E, D, MT>(a, lds);                                                                         \
+  }                                                                                                           \
+  extern "C" __global__ __launch_bounds__(256) void paged_attn_join_##T##_d##D##_r##MT(PagedAttnArgs a) {      \
+    __shared__ int32_t base[264];                                                                             \
+    one::join<one::E, D, MT>(a, base);                                                        \
+  }
+PAGED_ONE(bf16, Bf, 64, 1)
+PAGED_ONE(bf16, Bf, 64, 2)
+PAGED_ONE(bf16, Bf, 128, 1)
+PAGED_ONE(bf16, Bf, 128, 2)
+PAGED_ONE(bf16, Bf, 256, 1)
+PAGED_ONE(f16, Hf, 64, 1)
+PAGED_ONE(f16, Hf, 64, 2)
+PAGED_ONE(f16, Hf, 128, 1)
+PAGED_ONE(f16, Hf, 128, 2)
+PAGED_ONE(f16, Hf, 256, 1)
+#undef PAGED_ONE

@@ -1,6 +1,7 @@
 // tt_paged_plan, tt_paged_write, tt_paged_attn: launch validation and kernel selection for the paged 8-bit cache.
 #include <algorithm>
 #include <cmath>
+#include <cstdio>
 #include <cstring>
 
 #include "tt_internal.h"
@@ -35,6 +36,29 @@ int check_grid(const char *who, const uint32_t grid[3], int32_t x, int32_t y) {
   if (grid[0] != (uint32_t)x || grid[1] != (uint32_t)y || grid[2] != 1)
     return fail(RT_ERR_INVALID, "%s: grid (%u,%u,%u), expected (%d,%d,1)", who, grid[0], grid[1], grid[2], x, y);
   return RT_OK;
+}
+// How tt_paged_attn runs a call of these sizes.
+struct Route {
+  bool one = false;       // single tokens: paged_attn_one_*
+  int rows = 1;           // its 16-row tiles of query heads
+  uint32_t groups = 0;    // its workgroups
+  bool join = false;      // sequences may be split: partial results, joined by a second launch
+  size_t workspace = 0;
+};
+Route route_of(const PagedCacheArgs &c, int32_t B, int32_t max_pages, int32_t tokens, int32_t heads_q, int32_t max_q) {
+  Route r;
+  const int D = c.head_dim, group = heads_q / c.heads;
+  if (max_q > 1 || (D != 64 && D != 128 && D != 256) || c.page_size % 16 || c.page_size > 8192) return r;
+  if (group > (D == 256 ? 16 : 32)) return r;
+  r.one = true;
+  r.rows = group > 16 ? 2 : 1;
+  const int64_t unit = D * r.rows >= 256 ? 128 : 256;
+  const int64_t most = std::max<int64_t>(cdiv64((int64_t)max_pages * c.page_size, unit), 1);
+  const int64_t units = most * c.heads * std::min(B, tokens);
+  r.groups = (uint32_t)std::min<int64_t>(units, 2 * props()->multiprocessor_count);
+  r.join = most > 1 && r.groups > 1;
+  if (r.join) r.workspace = 2 * (size_t)r.groups * (16 * r.rows * D + 32 * r.rows + 4) * sizeof(float);
+  return r;
 }
 } // namespace
 
@@ -104,7 +128,7 @@ extern "C" int tt_paged_attn_workspace(int32_t B, int32_t max_pages, int32_t tok
   if (B <= 0 || max_pages <= 0 || tokens <= 0 || heads_q <= 0 || max_q <= 0 || heads_q % c.heads)
     return fail(RT_ERR_INVALID, "%s: B %d, max_pages %d, tokens %d, heads %d over %d, max_q %d", who, B, max_pages, tokens,
                 heads_q, c.heads, max_q);
-  *bytes = 0;
+  *bytes = route_of(c, B, max_pages, tokens, heads_q, max_q).workspace;
   return RT_OK;
 }
 
@@ -140,6 +164,24 @@ extern "C" int tt_paged_attn(const void *q, const int64_t q_strides[2], const tt
   a.b = B; a.max_pages = max_pages; a.tokens = tokens; a.heads_q = heads_q; a.group = heads_q / a.c.heads;
   a.causal = causal != 0; a.qk_scale = sm_scale * 1.44269504f;
   void *args[] = {&a};
+  const char *type = dtype == TT_BF16 ? "bf16" : "f16";
+  char name[64];
+  const Route r = route_of(a.c, B, max_pages, tokens, heads_q, max_q);
+  // 16-byte loads of the cache and of q, pairs of results, and offsets inside 16 rows that fit 32 bits
+  const PagedCacheArgs &c = a.c;
+  const bool al = aligned16(c.k) && aligned16(c.v) && (c.k_page | c.k_head | c.k_tok | c.v_page | c.v_head | c.v_tok) % 16 == 0 &&
+                  std::max(c.k_tok, c.v_tok) < (1 << 26) && aligned16(a.q) && (a.q_tok | a.q_head) % 8 == 0 &&
+                  aligned(a.o, 4) && (a.o_tok | a.o_head) % 2 == 0;
+  if (r.one && al) {
+    const uint64_t per = (uint64_t)c.page_size / 16;
+    a.page_magic = ((1ull << 36) + per - 1) / per;
+    a.part = (float *)workspace;
+    a.split_groups = (int32_t)r.groups;
+    snprintf(name, sizeof(name), "paged_attn_one_%s_d%d_r%d", type, c.head_dim, r.rows);
+    if ((rc = launch("paged", name, dim3(r.groups), dim3(256), 0, stream, args, 1)) || !r.join) return rc;
+    snprintf(name, sizeof(name), "paged_attn_join_%s_d%d_r%d", type, c.head_dim, r.rows);
+    return launch("paged", name, dim3((uint32_t)B, (uint32_t)c.heads), dim3(256), 0, stream, args, 1);
+  }
   return launch("paged", dtype == TT_BF16 ? "paged_attn_any_bf16" : "paged_attn_any_f16",
                 dim3((uint32_t)tokens, (uint32_t)heads_q), dim3(64), 0, stream, args, 1);
 }
