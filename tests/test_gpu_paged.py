@@ -2,7 +2,9 @@
 
 Plan and write are compared bit for bit.  Attention: with u = 2^-24, n keys, head dim D, a score (base 2) is off by at
 most (D + 4) u reach, a probability by the relative ln 2 times that, one exp2 (2 u) and n u for the sums, twice for
-numerator and denominator; the probabilities and the output are rounded to 11 or 8 bits at half a step each."""
+numerator and denominator; the weights and the output are rounded to 11 or 8 bits at half a step each.  A V scale of code
+e enters as score + (e - 121), one more rounding of a sum of magnitude reach + |e - 121|, and leaves the same way in the
+log-sum-exp (codes here are within 54 of 121)."""
 import numpy as np
 import pytest
 import torch
@@ -202,11 +204,11 @@ def compare(o, lse, want, n, D, dtype):
     rows = ~np.isnan(wl)
     assert np.array_equal(np.isneginf(lse[rows]), np.isneginf(wl[rows]))
     fine = rows & np.isfinite(wl)
-    ds = (D + 4) * U * reach
+    ds = (D + 5) * U * reach + 54 * U
     rel = 2 * (np.log(2.0) * ds + 2 * U + n * U)
     tol = spread * (2.0**-11 + rel[..., None]) + torch.finfo(dtype).eps / 2 * (np.abs(wo) + spread * 2.0**-10) + 2.0**-24
     assert (np.abs(o - wo)[fine] <= tol[fine]).all(), np.nanmax((np.abs(o - wo) / tol)[fine])
-    ltol = ds + (n + 4) * U / np.log(2.0) + 2 * U * np.abs(np.where(fine, wl, 0.0)) + 2 * U
+    ltol = ds + (n + 4) * U / np.log(2.0) + 2 * U * np.abs(np.where(fine, wl, 0.0)) + 64 * U
     assert (np.abs(lse - np.where(fine, wl, 0.0))[fine] <= ltol[fine]).all()
     none = rows & np.isneginf(wl)
     assert (o[none] == 0).all()

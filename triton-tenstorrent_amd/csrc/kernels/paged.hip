@@ -303,3 +303,4 @@ extern "C" __global__ __launch_bounds__(64) void paged_attn_any_f16(PagedAttnArg
 }
 
 #include "paged_attn_one.h"
+#include "paged_attn_rows.h"

@@ -8,9 +8,11 @@
 //                               D/16 consecutive codes of each of its keys and pairs neighbouring keys' bytes with
 //                               v_perm_b32, one for two conversions.  MFMA number i takes the lanes' i-th code, so its
 //                               row l%16 stands for d = (l%16) * D/16 + i.
-// e4m3 -> 16 bits is v_cvt_scalef32_pk_{bf16,f16}_fp8 (exact): K without its scale, which joins the factor on the scores;
-// V with its page's scale relative to the largest met so far (`eref`, the accumulator follows when it grows), in fp16,
-// like the probabilities: 11 bits where bf16 has 8, and the accumulator's power of two keeps the range.
+// e4m3 -> 16 bits is v_cvt_scalef32_pk_{bf16,f16}_fp8 (exact), K and V without their scales.  K's joins the factor on the
+// scores.  V's, a power of two 2^(e - 127), joins the exponent: with x = score + e - 121 the weight w = 2^(x - ref) is what
+// a key contributes relative to the row's largest contribution, the sum over V takes w and the sum of probabilities
+// w 2^(121 - e).  So weights can be held in fp16 (11 bits where bf16 has 8) whatever the scales' range: fp16 flushes
+// below 2^-32 of the largest contribution.
 //
 // Split: the keys of all sequences, in units of 64 * NS, are dealt evenly to the workgroups of a grid that fills the chip
 // once, whatever the lengths: workgroup i takes units [i U / G, (i+1) U / G) and meets at most two (sequence, head)
@@ -27,8 +29,12 @@ typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
-constexpr float kLift = 8.0f;  // probabilities are held times 2^8: fp16 then reaches down to 2^-32 of the reference
+constexpr float kLift = 8.0f;  // weights are held times 2^8: fp16 then reaches down to 2^-32 of the reference
 constexpr float kLazy = 7.0f;  // the reference follows a row's maximum when that is 2^7 above it: at most 2^15 < 65504
+constexpr int kBase = 121;     // scale code that leaves x = score: that of a page of magnitudes up to 4 .. 7
+// what brings a page's weights back to probabilities, 2^(kBase - e)
+__device__ __forceinline__ float unweight(int e) { return __builtin_bit_cast(float, (uint32_t)max(kBase + 127 - e, 1) << 23); }
+constexpr float kOut = 0x1p-6f; // 2^(kBase - 127): V of scale code kBase
 constexpr float kInf = __builtin_inff();
 
 template <int D, int MT> constexpr int subtiles() { return D * MT >= 256 ? 2 : 4; } // of 16 keys, per wavefront and step
@@ -95,8 +101,8 @@ __device__ __forceinline__ int64_t lane64(int32_t lo, int32_t hi, int lane) {
   return (int64_t)(((uint64_t)(uint32_t)__builtin_amdgcn_readlane(hi, lane) << 32) | (uint32_t)__builtin_amdgcn_readlane(lo, lane));
 }
 
-// Partial result p of the workspace: rows * D sums, then rows pairs (reference, sum), then the sums' exponent.
-template <int D, int MT> constexpr int part_floats() { return 16 * MT * D + 32 * MT + 4; }
+// Partial result p of the workspace: rows * D sums, then rows pairs (reference, sum).
+template <int D, int MT> constexpr int part_floats() { return 16 * MT * D + 32 * MT; }
 
 template <class E, int D, int MT>
 __device__ __forceinline__ void body(const PagedAttnArgs &a, float *lds) {
@@ -160,7 +166,6 @@ __device__ __forceinline__ void body(const PagedAttnArgs &a, float *lds) {
 
     f32x4 acc[MT][VB];
     float mref[MT], lsum[MT];
-    int eref = 0;
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
       mref[m] = -kInf;
@@ -223,7 +228,7 @@ __device__ __forceinline__ void body(const PagedAttnArgs &a, float *lds) {
     for (int it = 0; it < n; ++it) {
       int nv[NS], vc[NS];
       float ks[NS];
-      int nmin = 16, emax = 0;
+      int nmin = 16;
 #pragma unroll
       for (int s = 0; s < NS; ++s) {
         const int src = (it % IB) * NS + s;
@@ -231,7 +236,6 @@ __device__ __forceinline__ void body(const PagedAttnArgs &a, float *lds) {
         vc[s] = __builtin_amdgcn_readlane(vcode, src);
         ks[s] = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, kscale), src));
         nmin = min(nmin, nv[s]);
-        emax = max(emax, vc[s]);
       }
       // scores
       f32x4 st[MT][NS];
@@ -248,7 +252,9 @@ __device__ __forceinline__ void body(const PagedAttnArgs &a, float *lds) {
             for (int m = 0; m < MT; ++m) st[m][s] = E::mfma(kf, qf[m][h * 2 + c], st[m][s]);
           }
 #pragma unroll
-        for (int m = 0; m < MT; ++m) st[m][s] *= ks[s];
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) st[m][s][r] = fmaf(st[m][s][r], ks[s], (float)(vc[s] - kBase));
       }
       if (it + 1 < n) {
         if ((it + 1) % IB == 0) batch(it + 1);
@@ -266,7 +272,7 @@ __device__ __forceinline__ void body(const PagedAttnArgs &a, float *lds) {
             for (int w = 0; w < VW; ++w) vr[s][r][w] = in ? vr[s][r][w] : 0;
           }
       }
-      // the reference, and the largest V scale
+      // the reference
       float top[MT];
       bool grow = false;
 #pragma unroll
@@ -278,9 +284,7 @@ __device__ __forceinline__ void body(const PagedAttnArgs &a, float *lds) {
           for (int r = 0; r < 4; ++r) top[m] = fmaxf(top[m], st[m][s][r]);
         grow |= top[m] > mref[m] + kLazy;
       }
-      if (__any(grow) || emax > eref) {
-        const float ve = __builtin_amdgcn_ldexpf(1.0f, min(eref - emax, 0));
-        eref = max(eref, emax);
+      if (__any(grow)) {
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
           float x = fmaxf(top[m], __shfl_xor(top[m], 16));
@@ -290,7 +294,7 @@ __device__ __forceinline__ void body(const PagedAttnArgs &a, float *lds) {
           mref[m] = mn;
           lsum[m] *= al;
 #pragma unroll
-          for (int i = 0; i < VB; ++i) acc[m][i] *= al * ve;
+          for (int i = 0; i < VB; ++i) acc[m][i] *= al;
         }
       }
       f16x8 pf[MT][NS / 2];
@@ -298,18 +302,17 @@ __device__ __forceinline__ void body(const PagedAttnArgs &a, float *lds) {
       for (int m = 0; m < MT; ++m) {
         const float ref = (mref[m] == -kInf ? 0.0f : mref[m]) - kLift;
 #pragma unroll
-        for (int s = 0; s < NS; ++s)
+        for (int s = 0; s < NS; ++s) {
+          float w[4];
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            const float p = __builtin_amdgcn_exp2f(st[m][s][r] - ref);
-            lsum[m] += p;
-            pf[m][s >> 1][(s & 1) * 4 + r] = (_Float16)p;
+            w[r] = __builtin_amdgcn_exp2f(st[m][s][r] - ref);
+            pf[m][s >> 1][(s & 1) * 4 + r] = (_Float16)w[r];
           }
+          lsum[m] = fmaf((w[0] + w[1]) + (w[2] + w[3]), unweight(vc[s]), lsum[m]);
+        }
       }
       // the sum over V
-      float vs[NS];
-#pragma unroll
-      for (int s = 0; s < NS; ++s) vs[s] = __builtin_bit_cast(float, (uint32_t)max(vc[s] - eref + 127, 0) << 23);
 #pragma unroll
       for (int p = 0; p < NS / 2; ++p)
 #pragma unroll
@@ -320,10 +323,10 @@ __device__ __forceinline__ void body(const PagedAttnArgs &a, float *lds) {
             const int s = 2 * p + (j >> 1), r = (j & 1) * 2;
             const uint32_t x = __builtin_amdgcn_perm(vr[s][r + 1][w], vr[s][r][w], 0x05010400);
             const uint32_t y = __builtin_amdgcn_perm(vr[s][r + 1][w], vr[s][r][w], 0x07030602);
-            f[0][j] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x, vs[s], false));
-            f[1][j] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x, vs[s], true));
-            f[2][j] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(y, vs[s], false));
-            f[3][j] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(y, vs[s], true));
+            f[0][j] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x, 1.0f, false));
+            f[1][j] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x, 1.0f, true));
+            f[2][j] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(y, 1.0f, false));
+            f[3][j] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(y, 1.0f, true));
           }
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
@@ -337,8 +340,7 @@ __device__ __forceinline__ void body(const PagedAttnArgs &a, float *lds) {
     }
 
     // ---- merge the four wavefronts ----
-    float *wo = lds, *wml = lds + 4 * 16 * MT * LD;   // sums [wave][row][LD], (reference, sum) [wave][row], exponents [wave]
-    int32_t *we = (int32_t *)(wml + 4 * 16 * MT * 2);
+    float *wo = lds, *wml = lds + 4 * 16 * MT * LD;   // sums [wave][row][LD], (reference, sum) [wave][row]
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
       float l = lsum[m];
@@ -352,10 +354,8 @@ __device__ __forceinline__ void body(const PagedAttnArgs &a, float *lds) {
         for (int i = 0; i < VB; i += 4)
           *(f32x4 *)(wo + row * LD + (g * 4 + r) * VB + i) = (f32x4){acc[m][i][r], acc[m][i + 1][r], acc[m][i + 2][r], acc[m][i + 3][r]};
     }
-    if (lane == 0) we[wave] = eref;
     __syncthreads();
     const bool whole = c0 == 0 && n == units;
-    const int e = max(max(we[0], we[1]), max(we[2], we[3]));
     // (the first segment of this workgroup takes slot 0, a later one that is not whole can only be its last: slot 1)
     float *slot = a.part + (2 * (int64_t)blockIdx.x + (u == u_first ? 0 : 1)) * part_floats<D, MT>();
 #pragma unroll
@@ -373,20 +373,19 @@ __device__ __forceinline__ void body(const PagedAttnArgs &a, float *lds) {
         const float mw = wml[(w * 16 * MT + row) * 2];
         const float f = mw == -kInf ? 1.0f : __builtin_amdgcn_exp2f(mw - mm); // (a row of NaN scores has reference -inf)
         l += wml[(w * 16 * MT + row) * 2 + 1] * f;
-        const float fe = f * __builtin_amdgcn_ldexpf(1.0f, we[w] - e);
 #pragma unroll
-        for (int i = 0; i < VB; ++i) o[i] += wo[(w * 16 * MT + row) * LD + d0 + i] * fe;
+        for (int i = 0; i < VB; ++i) o[i] += wo[(w * 16 * MT + row) * LD + d0 + i] * f;
       }
       if (whole) {
         if (row < a.group) {
           const int hq = hk * a.group + row;
           const bool none = l == 0.0f && mx == -kInf;
-          const float inv = none ? 0.0f : 1.0f / l;
+          const float inv = none ? 0.0f : kOut / l;
           uint16_t *op = a.o + t * a.o_tok + hq * a.o_head + d0;
 #pragma unroll
           for (int i = 0; i < VB; i += 2)
-            *(uint32_t *)(op + i) = (uint32_t)E::out(__builtin_amdgcn_ldexpf(o[i] * inv, e - 127)) |
-                                    (uint32_t)E::out(__builtin_amdgcn_ldexpf(o[i + 1] * inv, e - 127)) << 16;
+            *(uint32_t *)(op + i) = (uint32_t)E::out(o[i] * inv) |
+                                    (uint32_t)E::out(o[i + 1] * inv) << 16;
           if (a.lse && d0 == 0) a.lse[(int64_t)t * a.heads_q + hq] = none ? -kInf : mx - kLift + __builtin_log2f(l);
         }
       } else {
@@ -395,7 +394,6 @@ __device__ __forceinline__ void body(const PagedAttnArgs &a, float *lds) {
         if (d0 == 0) {
           slot[16 * MT * D + row * 2] = mx;
           slot[16 * MT * D + row * 2 + 1] = l;
-          if (row == 0) ((int32_t *)slot)[16 * MT * D + 32 * MT] = e;
         }
       }
     }
@@ -428,11 +426,7 @@ template <class E, int D, int MT> __device__ __forceinline__ void join(const Pag
     const int row = m * 16 + (tid >> 4), d0 = (tid & 15) * VB;
     if (row >= a.group) continue;
     float mx = -kInf;
-    int e = 0;
-    for (int64_t i = i0; i <= i1; ++i) {
-      mx = fmaxf(mx, slot(i)[16 * MT * D + row * 2]);
-      e = max(e, ((const int32_t *)slot(i))[16 * MT * D + 32 * MT]);
-    }
+    for (int64_t i = i0; i <= i1; ++i) mx = fmaxf(mx, slot(i)[16 * MT * D + row * 2]);
     const float mm = mx == -kInf ? 0.0f : mx;
     float l = 0.0f, o[VB];
 #pragma unroll
@@ -442,27 +436,26 @@ template <class E, int D, int MT> __device__ __forceinline__ void join(const Pag
       const float mw = p[16 * MT * D + row * 2];
       const float f = mw == -kInf ? 1.0f : __builtin_amdgcn_exp2f(mw - mm);
       l += p[16 * MT * D + row * 2 + 1] * f;
-      const float fe = f * __builtin_amdgcn_ldexpf(1.0f, ((const int32_t *)p)[16 * MT * D + 32 * MT] - e);
 #pragma unroll
       for (int j = 0; j < VB; j += 4) {
         const f32x4 x = *(const f32x4 *)(p + row * D + d0 + j);
-        o[j] += x[0] * fe; o[j + 1] += x[1] * fe; o[j + 2] += x[2] * fe; o[j + 3] += x[3] * fe;
+        o[j] += x[0] * f; o[j + 1] += x[1] * f; o[j + 2] += x[2] * f; o[j + 3] += x[3] * f;
       }
     }
     const int hq = hk * a.group + row;
     const bool none = l == 0.0f && mx == -kInf;
-    const float inv = none ? 0.0f : 1.0f / l;
+    const float inv = none ? 0.0f : kOut / l;
     uint16_t *op = a.o + t * a.o_tok + hq * a.o_head + d0;
 #pragma unroll
     for (int i = 0; i < VB; i += 2)
-      *(uint32_t *)(op + i) = (uint32_t)E::out(__builtin_amdgcn_ldexpf(o[i] * inv, e - 127)) |
-                              (uint32_t)E::out(__builtin_amdgcn_ldexpf(o[i + 1] * inv, e - 127)) << 16;
+      *(uint32_t *)(op + i) = (uint32_t)E::out(o[i] * inv) |
+                              (uint32_t)E::out(o[i + 1] * inv) << 16;
     if (a.lse && d0 == 0) a.lse[(int64_t)t * a.heads_q + hq] = none ? -kInf : mx - kLift + __builtin_log2f(l);
   }
 }
 
 template <int D, int MT> constexpr int lds_floats() {
-  return 4 * 16 * MT * (D + 4) + 4 * 16 * MT * 2 + 4 > 264 ? 4 * 16 * MT * (D + 4) + 4 * 16 * MT * 2 + 4 : 264;
+  return 4 * 16 * MT * (D + 4) + 4 * 16 * MT * 2;
 }
 
 } // namespace one

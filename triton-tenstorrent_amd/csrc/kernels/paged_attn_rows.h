@@ -1,0 +1,457 @@
+// Attention over the paged cache, several queries of a sequence (prompts, pieces of prompts, verification).
+//
+// A workgroup owns 128 rows of one (sequence, cache head): row r is query r / group, query head r % group of the head's
+// group, so that the heads that share keys share the keys' conversion and LDS tile.  Each of its four wavefronts has 32
+// rows and computes both products transposed, so that a row's statistics stay in the two lanes that own it:
+//   S^T[key, row] = K . Q^T      v_mfma_f32_32x32x16, A = 32 rows of K, B = Q
+//   O^T[d, row]  += V^T . P^T    A = V^T, B = P^T straight from the registers of S^T
+// Keys come in tiles of 64.  Wavefront w stages the tile's 16 keys 16 w .. 16 w + 15 (they share a page): codes are loaded
+// two tiles ahead, turned to 16 bits on the way into LDS, V transposed there (v_perm_b32 pairs neighbouring keys' bytes
+// before the conversion, as in paged_attn_one.h), K and V without their scales, which join the scores as there.  LDS
+// holds two tiles; one barrier a tile.
+// Bound: MFMA and the exponentials (32 v_exp_f32 a lane and tile against 32 MFMAs of 32 cycles), LDS reads behind them.
+//
+// Where the rows are too few to fill the chip the keys are split `splits` ways and paged_attn_rows_join adds the parts.
+#pragma once
+
+namespace rows {
+
+using one::f16x8;
+using one::kBase;
+using one::kInf;
+using one::kLazy;
+using one::kLift;
+using one::kOut;
+using one::unweight;
+using one::u32x2;
+using one::u32x4;
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+struct Bf : one::Bf {
+  static __device__ __forceinline__ f32x16 mfma32(frag x, frag y, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, y, c, 0, 0, 0); }
+};
+struct Hf : one::Hf {
+  static __device__ __forceinline__ f32x16 mfma32(frag x, frag y, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(x, y, c, 0, 0, 0); }
+};
+
+constexpr int kRows = 128;
+
+struct Seq { int32_t q0, n, len, units; }; // first packed row, queries, keys, tiles of 128 rows
+__device__ __forceinline__ Seq seq_of(const PagedAttnArgs &a, int b) {
+  const int32_t q0 = clampi(a.cu_q[b], 0, a.tokens), q1 = clampi(a.cu_q[b + 1], q0, a.tokens);
+  const int32_t n = q1 - q0 >= a.rows_min ? q1 - q0 : 0;
+  return {q0, n, clampi(a.lens[b], 0, a.max_pages * a.c.page_size), (int32_t)(((int64_t)n * a.group + kRows - 1) / kRows)};
+}
+
+__device__ __forceinline__ int scan_units(const PagedAttnArgs &a, int32_t *base, int32_t *part) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, per = (a.b + 255) / 256;
+  int32_t n = 0;
+  for (int b = min(tid * per, a.b); b < min(tid * per + per, a.b); ++b) n += seq_of(a, b).units;
+  int32_t v = n;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int32_t o = __shfl_up(v, d);
+    if (lane >= d) v += o;
+  }
+  if (lane == 63) part[wave] = v;
+  __syncthreads();
+  for (int w = 0; w < wave; ++w) v += part[w];
+  base[tid] = v - n;
+  const int total = part[0] + part[1] + part[2] + part[3];
+  __syncthreads();
+  return total;
+}
+
+// The sequence that holds row tile u, and the tile's number in it.
+struct Item { int b, tile; Seq sq; };
+__device__ __forceinline__ Item item_of(const PagedAttnArgs &a, const int32_t *base, int u) {
+  const int per = (a.b + 255) / 256;
+  int lo = 0, hi = 255;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (base[mid] <= u) lo = mid; else hi = mid - 1;
+  }
+  int b = __builtin_amdgcn_readfirstlane(min(lo * per, a.b - 1));
+  int before = __builtin_amdgcn_readfirstlane(base[lo]);
+  Seq sq = seq_of(a, b);
+  while (before + sq.units <= u) {
+    before += sq.units;
+    sq = seq_of(a, ++b);
+  }
+  return {b, u - before, sq};
+}
+
+// Last key that query i of the sequence attends (-1: none).
+__device__ __forceinline__ int32_t last_key(const PagedAttnArgs &a, const Seq &sq, int32_t i) {
+  return a.causal ? max(sq.len - sq.n + i, -1) : sq.len - 1;
+}
+
+// A tile's steps of 64 keys, and split s of them.
+__device__ __forceinline__ int steps_of(const PagedAttnArgs &a, const Seq &sq, int tile) {
+  const int32_t r1 = (int32_t)min((int64_t)(tile + 1) * kRows, (int64_t)sq.n * a.group) - 1;
+  return (last_key(a, sq, r1 / a.group) + 64) / 64;
+}
+
+// Floats of one part: 128 rows of D sums, then (reference, sum) of each row.
+template <int D> constexpr int part_floats() { return kRows * D + 2 * kRows; }
+
+// K tile, V^T tile, flags (32 bytes), and where V holds NaN: a bit for each code, 16 bits for each (key, staging thread)
+template <int D> constexpr int stage_bytes() { return (64 * D * 2 * 2 + 32 + 64 * 16 * 2 + 511) / 512 * 512; }
+template <int D> constexpr int lds_bytes() { return 2 * stage_bytes<D>(); }
+
+template <class E, int D>
+__device__ __forceinline__ void body(const PagedAttnArgs &a, uint8_t *lds) {
+  constexpr int DK = D / 16, DT = D / 32, KB = D / 4, VB = D / 16, KW = KB / 16, VW = VB / 4;
+  constexpr int KROW = D * 2, VOFF = 64 * KROW, FOFF = 2 * VOFF;
+  constexpr int KMASK = D == 64 ? 7 : 15, KSH = D == 64 ? 1 : 0; // chunk swizzle of K rows
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int c32 = lane & 31, hi = lane >> 5;
+  int32_t *base = (int32_t *)lds, *part = base + 256;
+  const int total = scan_units(a, base, part);
+
+  const int heads = a.c.heads, splits = a.splits;
+  const int hk = blockIdx.x % heads, rest = blockIdx.x / heads, split = rest % splits;
+  const int u = total - 1 - rest / splits; // late rows, which attend most keys, first
+  if (u < 0) return;
+  const Item item = item_of(a, base, u);
+  __syncthreads(); // `base` shares its LDS with the tiles
+  const Seq sq = item.sq;
+  const int R = sq.n * a.group, row0 = item.tile * kRows;
+  const int nsteps = steps_of(a, sq, item.tile);
+  const int k_lo = (int)((int64_t)split * nsteps / splits), k_hi = (int)((int64_t)(split + 1) * nsteps / splits);
+  if (splits > 1 && k_lo >= k_hi && !(nsteps == 0 && split == 0)) return; // (an item without a key writes its zeros once)
+
+  const int row = row0 + wave * 32 + c32;
+  const int qi = min(row, R - 1) / a.group, qg = min(row, R - 1) % a.group;
+  const int64_t t = sq.q0 + qi;
+  const int hq = hk * a.group + qg;
+  const int32_t limit = last_key(a, sq, qi);
+  const bool alive = row0 + wave * 32 < R;  // the wavefront has rows
+  // keys that all rows of the workgroup attend end here; the wavefront's own rows see nothing from `wave_end` on
+  const int32_t all_to = last_key(a, sq, row0 / a.group);
+  const int32_t wave_last = __builtin_amdgcn_readfirstlane(last_key(a, sq, min(row0 + wave * 32 + 31, R - 1) / a.group));
+
+  typename E::frag qf[DK];
+  {
+    const uint16_t *qr = a.q + t * a.q_tok + hq * a.q_head + hi * 8;
+#pragma unroll
+    for (int s = 0; s < DK; ++s) qf[s] = __builtin_bit_cast(typename E::frag, *(const u32x4 *)(qr + s * 16));
+  }
+  f32x16 acc[DT];
+#pragma unroll
+  for (int i = 0; i < DT; ++i) acc[i] = (f32x16){0};
+  float mref = -kInf, lsum = 0.0f;
+
+  const int32_t *table = a.table + (int64_t)item.b * a.table_stride;
+  const uint8_t *kh = a.c.k + hk * a.c.k_head, *vh = a.c.v + hk * a.c.v_head;
+  // staging: K row tid / 4 of the tile, KB codes from column (tid % 4) * KB; V keys 4 (tid / 16) .. + 3, VB codes from
+  // column (tid % 16) * VB.  Both lie in the wavefront's 16 keys.
+  const uint32_t kvo = (uint32_t)(((tid >> 2) & 15) * a.c.k_tok + (tid & 3) * KB);
+  uint32_t vvo[4];
+#pragma unroll
+  for (int r = 0; r < 4; ++r) vvo[r] = (uint32_t)(((((tid >> 4) & 3) * 4 + r)) * a.c.v_tok + (tid & 15) * VB);
+
+  // What lane (k % 16) * 4 + s knows of subtile s of step k (16 steps at a time).
+  int32_t ko_lo, ko_hi, vo_lo, vo_hi, live, vcode;
+  float kscale;
+  auto batch = [&](int k0) {
+    const int64_t key = (int64_t)(k0 + (lane >> 2)) * 64 + (lane & 3) * 16;
+    const uint32_t sub = (uint32_t)(key >> 4);
+    const uint32_t blk = (uint32_t)(((uint64_t)sub * a.page_magic) >> 36);
+    int32_t page = key < sq.len ? table[blk] : -1;
+    const bool ok = page >= 0 && page < a.c.pages;
+    page = ok ? page : 0;
+    const int64_t prow = ok ? ((int64_t)sub - (int64_t)blk * (a.c.page_size >> 4)) * 16 : 0;
+    const int64_t ko = page * a.c.k_page + prow * a.c.k_tok, vo = page * a.c.v_page + prow * a.c.v_tok;
+    ko_lo = (int32_t)ko; ko_hi = (int32_t)(ko >> 32); vo_lo = (int32_t)vo; vo_hi = (int32_t)(vo >> 32);
+    live = ok ? (int32_t)min((int64_t)sq.len - key, (int64_t)16) : 0;
+    kscale = pow2_code(a.c.ks[page * a.c.ks_page + hk * a.c.ks_head]) * a.qk_scale;
+    vcode = ok ? a.c.vs[page * a.c.vs_page + hk * a.c.vs_head] : 0;
+  };
+  u32x4 kr[KW];
+  uint32_t vr[4][VW];
+  struct Meta { float ks[4]; int nv[4], vc[4]; };
+  Meta staged; // of the codes in kr and vr
+  auto load = [&](int k, int k_first) {
+    const int at = ((k - k_first) & 15) * 4;
+    if (((k - k_first) & 15) == 0) batch(k);
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      staged.ks[s] = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, kscale), at + s));
+      staged.nv[s] = __builtin_amdgcn_readlane(live, at + s);
+      staged.vc[s] = __builtin_amdgcn_readlane(vcode, at + s);
+    }
+    const uint8_t *kp = kh + one::lane64(ko_lo, ko_hi, at + wave), *vp = vh + one::lane64(vo_lo, vo_hi, at + wave);
+#pragma unroll
+    for (int i = 0; i < KW; ++i) kr[i] = *(const u32x4 *)(kp + kvo + i * 16);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      if constexpr (VW == 1) vr[r][0] = *(const uint32_t *)(vp + vvo[r]);
+      if constexpr (VW == 2) {
+        const u32x2 x = *(const u32x2 *)(vp + vvo[r]);
+        vr[r][0] = x[0]; vr[r][1] = x[1];
+      }
+      if constexpr (VW == 4) {
+        const u32x4 x = *(const u32x4 *)(vp + vvo[r]);
+        vr[r][0] = x[0]; vr[r][1] = x[1]; vr[r][2] = x[2]; vr[r][3] = x[3];
+      }
+    }
+  };
+  // LDS addresses.  16-byte chunk c of K row r lies at c ^ (r / (256 / KROW) & KMASK), chunk c of V^T row d at
+  // c ^ swz(d), which spreads what one instruction touches over the banks; a tile begins on 512 bytes, so that every
+  // address below is one of four lane constants ^ a compile-time constant + another.
+  auto swz = [](int d) { return ((d >> 1) ^ (d >> 4)) & 7; };
+  const uint32_t k_rd = c32 * KROW + ((hi ^ ((c32 >> KSH) & KMASK)) << 4);
+  const uint32_t v_rd = VOFF + c32 * 128 + ((hi ^ swz(c32)) << 4);
+  const uint32_t k_wr = (tid >> 2) * KROW + ((((tid & 3) * (KB / 8)) ^ (((tid >> 2) >> KSH) & KMASK)) << 4);
+  const uint32_t v_wr = VOFF + (tid & 15) * VB * 128 + (((wave * 2 + ((tid >> 4) & 1)) ^ swz((tid & 15) * VB)) << 4) + ((tid >> 5) & 1) * 8;
+  // codes in registers -> tile in LDS.  `edge`: some row does not attend some of these keys, so a NaN in V must be told
+  // from the others' results (found here, handled by the readers).
+  auto store = [&](uint32_t buf, bool edge) {
+    const uint32_t kw = buf + k_wr, vw = buf + v_wr;
+#pragma unroll
+    for (int i = 0; i < KW; ++i)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        *(u32x4 *)(lds + (kw ^ ((i * 2 + h) << 4))) = __builtin_bit_cast(u32x4, E::codes(kr[i][2 * h], kr[i][2 * h + 1]));
+    const int nv = wave == 0 ? staged.nv[0] : wave == 1 ? staged.nv[1] : wave == 2 ? staged.nv[2] : staged.nv[3];
+    const int mm = (tid >> 4) & 3; // 4-key group of the 16
+    if (nv < 16) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int w = 0; w < VW; ++w) vr[r][w] = mm * 4 + r < nv ? vr[r][w] : 0;
+    }
+    if (edge) {
+      uint32_t nan[4][VW], any = 0;
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int w = 0; w < VW; ++w) {
+          nan[r][w] = ((vr[r][w] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+          any |= nan[r][w];
+        }
+      const bool found = __any(any != 0);
+      if (lane == 0) *(int32_t *)(lds + buf + FOFF + wave * 4) = found;
+      if (found) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          uint32_t bits = 0;
+#pragma unroll
+          for (int w = 0; w < VW; ++w) {
+            // bits 7, 15, 23, 31 -> 0 .. 3
+            bits |= (((nan[r][w] >> 7) * 0x00204081u) >> 21 & 15u) << (w * 4);
+            vr[r][w] &= ~((nan[r][w] >> 7) * 0xffu);
+          }
+          ((uint16_t *)(lds + buf + FOFF + 32))[(wave * 16 + mm * 4 + r) * 16 + (tid & 15)] = (uint16_t)bits;
+        }
+      }
+    }
+#pragma unroll
+    for (int w = 0; w < VW; ++w) {
+      const uint32_t x0 = __builtin_amdgcn_perm(vr[1][w], vr[0][w], 0x05010400), x1 = __builtin_amdgcn_perm(vr[3][w], vr[2][w], 0x05010400);
+      const uint32_t y0 = __builtin_amdgcn_perm(vr[1][w], vr[0][w], 0x07030602), y1 = __builtin_amdgcn_perm(vr[3][w], vr[2][w], 0x07030602);
+      const u32x2 f[4] = {{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x0, 1.0f, false)),
+                           __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x1, 1.0f, false))},
+                          {__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x0, 1.0f, true)),
+                           __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x1, 1.0f, true))},
+                          {__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(y0, 1.0f, false)),
+                           __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(y1, 1.0f, false))},
+                          {__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(y0, 1.0f, true)),
+                           __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(y1, 1.0f, true))}};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) *(u32x2 *)(lds + (vw ^ (((w * 4 + i) >> 1) << 4)) + (w * 4 + i) * 128) = f[i];
+    }
+  };
+  auto edge_of = [&](int k) { return k * 64 + 63 > all_to; };
+
+  if (k_lo < k_hi) {
+    load(k_lo, k_lo);
+    store(0, edge_of(k_lo));
+  }
+  Meta now = staged; // of the tile in LDS that is computed
+  if (k_lo + 1 < k_hi) load(k_lo + 1, k_lo);
+  __syncthreads();
+  for (int k = k_lo; k < k_hi; ++k) {
+    const uint32_t buf = ((k - k_lo) & 1) * stage_bytes<D>(), next = stage_bytes<D>() - buf;
+    Meta after = staged;
+    if (k + 1 < k_hi) {
+      store(next, edge_of(k + 1));
+      if (k + 2 < k_hi) load(k + 2, k_lo);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    if (alive && k * 64 <= wave_last) {
+      const uint32_t kb = buf + k_rd, vb = buf + v_rd;
+      f32x16 st[2] = {(f32x16){0}, (f32x16){0}};
+#pragma unroll
+      for (int s = 0; s < DK; ++s)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const u32x4 x = *(const u32x4 *)(lds + (kb ^ (s << 5)) + j * 32 * KROW);
+          st[j] = E::mfma32(__builtin_bit_cast(typename E::frag, x), qf[s], st[j]);
+        }
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) st[j][r] = fmaf(st[j][r], now.ks[j * 2 + (r >> 3)], (float)(now.vc[j * 2 + (r >> 3)] - kBase));
+      const bool edge = edge_of(k);
+      if (edge || !(now.nv[0] && now.nv[1] && now.nv[2] && now.nv[3])) {
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+          const int32_t rel = now.nv[s] ? limit - k * 64 - s * 16 - hi * 4 : -1; // (keys past the end are past the limit)
+#pragma unroll
+          for (int r = 0; r < 8; ++r) {
+            const float x = st[s >> 1][(s & 1) * 8 + r];
+            st[s >> 1][(s & 1) * 8 + r] = (r >> 2) * 8 + (r & 3) <= rel ? x : -kInf;
+          }
+        }
+      }
+      float top = -kInf;
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) top = fmaxf(top, st[j][r]);
+      if (__any(top > mref + kLazy)) {
+        const float mn = fmaxf(mref, fmaxf(top, __shfl_xor(top, 32)));
+        const float al = mn == -kInf ? 1.0f : __builtin_amdgcn_exp2f(mref - mn);
+        mref = mn;
+        lsum *= al;
+#pragma unroll
+        for (int i = 0; i < DT; ++i)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) acc[i][r] *= al;
+      }
+      const float ref = (mref == -kInf ? 0.0f : mref) - kLift;
+      f16x8 pf[4];
+#pragma unroll
+      for (int s = 0; s < 4; ++s) {
+        float sum = 0.0f;
+#pragma unroll
+        for (int r = 0; r < 8; ++r) {
+          const float w = __builtin_amdgcn_exp2f(st[s >> 1][(s & 1) * 8 + r] - ref);
+          sum += w;
+          pf[s][r] = (_Float16)w;
+        }
+        lsum = fmaf(sum, unweight(now.vc[s]), lsum);
+      }
+#pragma unroll
+      for (int s = 0; s < 4; ++s)
+#pragma unroll
+        for (int i = 0; i < DT; ++i) {
+          const u32x4 x = *(const u32x4 *)(lds + (vb ^ ((s ^ (i & 3)) << 5)) + i * 32 * 128);
+          acc[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, x), pf[s], acc[i], 0, 0, 0);
+        }
+      if (edge) { // NaN in V, taken out of the tile: it reaches the rows that attend its key
+        for (int s = 0; s < 4; ++s) {
+          if (!__builtin_amdgcn_readfirstlane(*(const int32_t *)(lds + buf + FOFF + s * 4))) continue;
+          for (int j = 0; j < 16; ++j) {
+            if (k * 64 + s * 16 + j > limit) continue;
+            const uint16_t *bits = (const uint16_t *)(lds + buf + FOFF + 32) + (s * 16 + j) * 16;
+#pragma unroll
+            for (int i = 0; i < DT; ++i)
+#pragma unroll
+              for (int r = 0; r < 16; ++r) {
+                const int d = i * 32 + (r >> 2) * 8 + hi * 4 + (r & 3);
+                if (bits[d / VB] >> (d % VB) & 1) acc[i][r] = __builtin_nanf("");
+              }
+          }
+        }
+      }
+    }
+    now = after;
+    __syncthreads();
+  }
+
+  lsum += __shfl_xor(lsum, 32);
+  if (!alive || row >= R) return;
+  if (splits == 1) {
+    const bool none = lsum == 0.0f && mref == -kInf;
+    const float inv = none ? 0.0f : kOut / lsum;
+    uint16_t *op = a.o + t * a.o_tok + hq * a.o_head + hi * 4;
+#pragma unroll
+    for (int i = 0; i < DT; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        uint16_t x[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[j] = E::out(acc[i][r * 4 + j] * inv);
+        *(u32x2 *)(op + i * 32 + r * 8) = (u32x2){(uint32_t)x[0] | (uint32_t)x[1] << 16, (uint32_t)x[2] | (uint32_t)x[3] << 16};
+      }
+    if (a.lse && hi == 0) a.lse[t * a.heads_q + hq] = none ? -kInf : mref - kLift + __builtin_log2f(lsum);
+  } else {
+    float *p = a.part + (((int64_t)u * heads + hk) * splits + split) * part_floats<D>();
+    const int lr = wave * 32 + c32;
+#pragma unroll
+    for (int i = 0; i < DT; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        *(f32x4 *)(p + lr * D + i * 32 + r * 8 + hi * 4) = (f32x4){acc[i][r * 4], acc[i][r * 4 + 1], acc[i][r * 4 + 2], acc[i][r * 4 + 3]};
+    if (hi == 0) { p[kRows * D + lr * 2] = mref; p[kRows * D + lr * 2 + 1] = lsum; }
+  }
+}
+
+// Adds the parts of one row tile: grid (row tiles, heads).
+template <class E, int D> __device__ __forceinline__ void join(const PagedAttnArgs &a, int32_t *base) {
+  constexpr int VB = D / 16;
+  const int total = scan_units(a, base, base + 256), u = blockIdx.x, hk = blockIdx.y, tid = threadIdx.x, splits = a.splits;
+  if (u >= total) return;
+  const Item item = item_of(a, base, u);
+  const Seq sq = item.sq;
+  const int R = sq.n * a.group, row0 = item.tile * kRows, nsteps = steps_of(a, sq, item.tile);
+  auto has = [&](int s) { return (int64_t)(s + 1) * nsteps / splits > (int64_t)s * nsteps / splits || (nsteps == 0 && s == 0); };
+  const float *p0 = a.part + ((int64_t)u * a.c.heads + hk) * splits * part_floats<D>();
+  for (int lr = tid >> 4; lr < min(R - row0, kRows); lr += 16) {
+    const int d0 = (tid & 15) * VB;
+    float mx = -kInf;
+    for (int s = 0; s < splits; ++s) {
+      if (has(s)) mx = fmaxf(mx, p0[(int64_t)s * part_floats<D>() + kRows * D + lr * 2]);
+    }
+    const float mm = mx == -kInf ? 0.0f : mx;
+    float l = 0.0f, o[VB];
+#pragma unroll
+    for (int i = 0; i < VB; ++i) o[i] = 0.0f;
+    for (int s = 0; s < splits; ++s) {
+      if (!has(s)) continue;
+      const float *p = p0 + (int64_t)s * part_floats<D>();
+      const float m = p[kRows * D + lr * 2];
+      const float f = m == -kInf ? 1.0f : __builtin_amdgcn_exp2f(m - mm); // (a row of NaN scores has reference -inf)
+      l += p[kRows * D + lr * 2 + 1] * f;
+#pragma unroll
+      for (int j = 0; j < VB; j += 4) {
+        const f32x4 y = *(const f32x4 *)(p + lr * D + d0 + j);
+        o[j] += y[0] * f; o[j + 1] += y[1] * f; o[j + 2] += y[2] * f; o[j + 3] += y[3] * f;
+      }
+    }
+    const int qi = (row0 + lr) / a.group, hq = hk * a.group + (row0 + lr) % a.group;
+    const int64_t t = sq.q0 + qi;
+    const bool none = l == 0.0f && mx == -kInf;
+    const float inv = none ? 0.0f : kOut / l;
+    uint16_t *op = a.o + t * a.o_tok + hq * a.o_head + d0;
+#pragma unroll
+    for (int i = 0; i < VB; i += 2)
+      *(uint32_t *)(op + i) = (uint32_t)E::out(o[i] * inv) |
+                              (uint32_t)E::out(o[i + 1] * inv) << 16;
+    if (a.lse && d0 == 0) a.lse[t * a.heads_q + hq] = none ? -kInf : mx - kLift + __builtin_log2f(l);
+  }
+}
+
+} // namespace rows
+
+#define PAGED_ROWS(T, E, D, OCC)                                                                              \
+  extern "C" __global__ __launch_bounds__(256, OCC) void paged_attn_rows_##T##_d##D(PagedAttnArgs a) {         \
+    __shared__ __align__(512) uint8_t lds[rows::lds_bytes<D>()];                                               \
+    rows::body<rows::E, D>(a, lds);                                                                           \
+  }                                                                                                           \
+  extern "C" __global__ __launch_bounds__(256) void paged_attn_rows_join_##T##_d##D(PagedAttnArgs a) {         \
+    __shared__ int32_t base[264];                                                                             \
+    rows::join<rows::E, D>(a, base);                                                                          \
+  }
+PAGED_ROWS(bf16, Bf, 64, 2)
+PAGED_ROWS(bf16, Bf, 128, 2)
+PAGED_ROWS(bf16, Bf, 256, 1)
+PAGED_ROWS(f16, Hf, 64, 2)
+PAGED_ROWS(f16, Hf, 128, 2)
+PAGED_ROWS(f16, Hf, 256, 1)
+#undef PAGED_ROWS

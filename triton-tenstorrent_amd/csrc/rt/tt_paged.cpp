@@ -39,25 +39,44 @@ int check_grid(const char *who, const uint32_t grid[3], int32_t x, int32_t y) {
 }
 // How tt_paged_attn runs a call of these sizes.
 struct Route {
-  bool one = false;       // single tokens: paged_attn_one_*
-  int rows = 1;           // its 16-row tiles of query heads
-  uint32_t groups = 0;    // its workgroups
-  bool join = false;      // sequences may be split: partial results, joined by a second launch
-  size_t workspace = 0;
+  bool fast = false;
+  // single tokens: paged_attn_one_*, its 16-row tiles of query heads, its workgroups, and whether sequences may be
+  // split (partial results, joined by a second launch)
+  bool one = false, one_join = false;
+  int one_tiles = 1;
+  uint32_t one_groups = 0;
+  // several queries: paged_attn_rows_*, its bound of 128-row tiles and the parts of a tile's keys
+  bool rows = false;
+  int32_t row_tiles = 0, splits = 1;
+  size_t one_bytes = 0, workspace = 0;
 };
 Route route_of(const PagedCacheArgs &c, int32_t B, int32_t max_pages, int32_t tokens, int32_t heads_q, int32_t max_q) {
   Route r;
-  const int D = c.head_dim, group = heads_q / c.heads;
-  if (max_q > 1 || (D != 64 && D != 128 && D != 256) || c.page_size % 16 || c.page_size > 8192) return r;
-  if (group > (D == 256 ? 16 : 32)) return r;
-  r.one = true;
-  r.rows = group > 16 ? 2 : 1;
-  const int64_t unit = D * r.rows >= 256 ? 128 : 256;
-  const int64_t most = std::max<int64_t>(cdiv64((int64_t)max_pages * c.page_size, unit), 1);
-  const int64_t units = most * c.heads * std::min(B, tokens);
-  r.groups = (uint32_t)std::min<int64_t>(units, 2 * props()->multiprocessor_count);
-  r.join = most > 1 && r.groups > 1;
-  if (r.join) r.workspace = 2 * (size_t)r.groups * (16 * r.rows * D + 32 * r.rows + 4) * sizeof(float);
+  const int D = c.head_dim, group = heads_q / c.heads, cus = props()->multiprocessor_count;
+  if ((D != 64 && D != 128 && D != 256) || c.page_size % 16 || c.page_size > 8192) return r;
+  if ((int64_t)tokens * group > INT32_MAX - 256) return r;
+  r.fast = true;
+  const int64_t keys = (int64_t)max_pages * c.page_size;
+  // sequences of one query go to their own kernel where a head group's rows fit it, unless the call has one sequence
+  // of several
+  r.one = group <= (D == 256 ? 16 : 32) && (max_q == 1 || B > 1);
+  r.rows = !r.one || max_q > 1;
+  if (r.one) {
+    r.one_tiles = group > 16 ? 2 : 1;
+    const int64_t unit = D * r.one_tiles >= 256 ? 128 : 256;
+    const int64_t most = std::max<int64_t>(cdiv64(keys, unit), 1);
+    r.one_groups = (uint32_t)std::min<int64_t>(most * c.heads * std::min(B, tokens), 2 * cus);
+    r.one_join = most > 1 && r.one_groups > 1;
+    if (r.one_join) r.one_bytes = 2 * (size_t)r.one_groups * (16 * r.one_tiles * D + 32 * r.one_tiles) * sizeof(float);
+  }
+  r.workspace = r.one_bytes;
+  if (r.rows) {
+    r.row_tiles = (int32_t)((int64_t)tokens * group / 128 + std::min(B, tokens));
+    // two workgroups a CU (one at head dim 256); a part has 256 keys at least
+    const int64_t items = (int64_t)r.row_tiles * c.heads, want = cdiv64((D == 256 ? 1 : 2) * cus, items);
+    r.splits = (int32_t)std::max<int64_t>(std::min(want, cdiv64(keys, 256)), 1);
+    if (r.splits > 1) r.workspace += (size_t)items * r.splits * (128 * D + 256) * sizeof(float);
+  }
   return r;
 }
 } // namespace
@@ -167,20 +186,38 @@ extern "C" int tt_paged_attn(const void *q, const int64_t q_strides[2], const tt
   const char *type = dtype == TT_BF16 ? "bf16" : "f16";
   char name[64];
   const Route r = route_of(a.c, B, max_pages, tokens, heads_q, max_q);
-  // 16-byte loads of the cache and of q, pairs of results, and offsets inside 16 rows that fit 32 bits
+  // 16-byte loads of the cache and of q, 8-byte stores of results, and offsets inside 16 rows that fit 32 bits
   const PagedCacheArgs &c = a.c;
   const bool al = aligned16(c.k) && aligned16(c.v) && (c.k_page | c.k_head | c.k_tok | c.v_page | c.v_head | c.v_tok) % 16 == 0 &&
                   std::max(c.k_tok, c.v_tok) < (1 << 26) && aligned16(a.q) && (a.q_tok | a.q_head) % 8 == 0 &&
-                  aligned(a.o, 4) && (a.o_tok | a.o_head) % 2 == 0;
-  if (r.one && al) {
+                  aligned(a.o, 8) && (a.o_tok | a.o_head) % 4 == 0;
+  if (r.fast && al) {
     const uint64_t per = (uint64_t)c.page_size / 16;
     a.page_magic = ((1ull << 36) + per - 1) / per;
-    a.part = (float *)workspace;
-    a.split_groups = (int32_t)r.groups;
-    snprintf(name, sizeof(name), "paged_attn_one_%s_d%d_r%d", type, c.head_dim, r.rows);
-    if ((rc = launch("paged", name, dim3(r.groups), dim3(256), 0, stream, args, 1)) || !r.join) return rc;
-    snprintf(name, sizeof(name), "paged_attn_join_%s_d%d_r%d", type, c.head_dim, r.rows);
-    return launch("paged", name, dim3((uint32_t)B, (uint32_t)c.heads), dim3(256), 0, stream, args, 1);
+    a.split_groups = (int32_t)r.one_groups;
+    a.splits = r.splits;
+    a.rows_min = r.one ? 2 : 1;
+    if (r.one) {
+      a.part = (float *)workspace;
+      snprintf(name, sizeof(name), "paged_attn_one_%s_d%d_r%d", type, c.head_dim, r.one_tiles);
+      if ((rc = launch("paged", name, dim3(r.one_groups), dim3(256), 0, stream, args, 1))) return rc;
+      if (r.one_join) {
+        snprintf(name, sizeof(name), "paged_attn_join_%s_d%d_r%d", type, c.head_dim, r.one_tiles);
+        if ((rc = launch("paged", name, dim3((uint32_t)B, (uint32_t)c.heads), dim3(256), 0, stream, args, 1))) return rc;
+      }
+    }
+    if (r.rows) {
+      a.part = (float *)((char *)workspace + r.one_bytes);
+      snprintf(name, sizeof(name), "paged_attn_rows_%s_d%d", type, c.head_dim);
+      const int64_t wgs = (int64_t)r.row_tiles * c.heads * r.splits;
+      if (wgs > INT32_MAX) return fail(RT_ERR_UNSUPPORTED, "%s: tokens * heads exceeds the grid", who);
+      if ((rc = launch("paged", name, dim3((uint32_t)wgs), dim3(256), 0, stream, args, 1))) return rc;
+      if (r.splits > 1) {
+        snprintf(name, sizeof(name), "paged_attn_rows_join_%s_d%d", type, c.head_dim);
+        if ((rc = launch("paged", name, dim3((uint32_t)r.row_tiles, (uint32_t)c.heads), dim3(256), 0, stream, args, 1))) return rc;
+      }
+    }
+    return RT_OK;
   }
   return launch("paged", dtype == TT_BF16 ? "paged_attn_any_bf16" : "paged_attn_any_f16",
                 dim3((uint32_t)tokens, (uint32_t)heads_q), dim3(64), 0, stream, args, 1);
