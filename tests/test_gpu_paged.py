@@ -94,6 +94,11 @@ def device_cache(codes, scales, layout="phtd"):
                         *(torch.from_numpy(s.astype(np.uint8)).cuda() for s in scales))
 
 
+def plain(codes):
+    """Codes with one pattern for NaN, whose sign bit means nothing."""
+    return np.where((codes & 127) == 127, 127, codes)
+
+
 def check_write(x, slots, codes, scales, layout="phtd"):
     cache = device_cache(codes, scales, layout)
     K.paged_write(x[0], x[1], i32(slots), cache)
@@ -101,7 +106,8 @@ def check_write(x, slots, codes, scales, layout="phtd"):
         wc, ws = codes[j].copy(), scales[j].copy()
         orc.write(x[j].cpu().double().numpy(), np.asarray(slots), wc, ws)
         assert np.array_equal(s.cpu().numpy(), ws), "scale"
-        assert np.array_equal(c.view(torch.uint8).cpu().numpy(), wc), "codes"
+        bad = np.argwhere(plain(c.view(torch.uint8).cpu().numpy()) != plain(wc))
+        assert len(bad) == 0, f"codes at {bad[:5].tolist()}"
 
 
 def runs(spec, P):
@@ -163,8 +169,17 @@ def test_write_of_strided_inputs(D, pad):
     check_write((k, v), slots, codes, scales)
 
 
-def test_write_grows_scales_token_by_token():
-    H, P, D = 2, 16, 128
+def test_write_keeps_nan_codes_of_earlier_rows():
+    H, P, D = 2, 64, 128
+    codes, scales = filled(3, H, P, D, seed=8)
+    codes[:, :, :, 2, 5], codes[:, :, :, 33, 7] = 0x7F, 0xFF
+    x = (torch.randn(2, 11, H, D) * 3e6).to(torch.bfloat16).cuda()      # every scale grows
+    check_write(x, runs([(0, 40, 10), (2, 63, 1)], P), codes, scales)
+
+
+@pytest.mark.parametrize("D", [64, 128, 256, 48])
+def test_write_grows_scales_token_by_token(D):
+    H, P = 2, 16
     codes, scales = filled(2, H, P, D, seed=6)
     cache = device_cache(codes, scales)
     want = [(codes[j].copy(), scales[j].copy()) for j in range(2)]

@@ -135,11 +135,25 @@ extern "C" __global__ __launch_bounds__(1024) void paged_plan(PagedPlanArgs a) {
 // ---------------------------------------------------------------------------
 namespace {
 
+typedef __bf16 w_bf16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 w_f16x2 __attribute__((ext_vector_type(2)));
+typedef short w_s16x2 __attribute__((ext_vector_type(2)));
+
+// The two input types.  codes2: two values, divided by the power of two `scale` and rounded to nearest even, into the
+// low or high half of c; they must be finite and at most 448 scale (one v_cvt_scalef32_pk_fp8_*).
 struct Bf16 {
+  static constexpr uint32_t kInfinite = 0x7f80;
   static __device__ __forceinline__ float get(uint16_t h) { return __builtin_bit_cast(float, (uint32_t)h << 16); }
+  template <bool HI> static __device__ __forceinline__ w_s16x2 codes2(w_s16x2 c, uint32_t x, float scale) {
+    return __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(c, __builtin_bit_cast(w_bf16x2, x), scale, HI);
+  }
 };
 struct Fp16 {
+  static constexpr uint32_t kInfinite = 0x7c00;
   static __device__ __forceinline__ float get(uint16_t h) { return (float)__builtin_bit_cast(_Float16, h); }
+  template <bool HI> static __device__ __forceinline__ w_s16x2 codes2(w_s16x2 c, uint32_t x, float scale) {
+    return __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(c, __builtin_bit_cast(w_f16x2, x), scale, HI);
+  }
 };
 
 // bits of |x|, 0 for infinities and NaN: what does not decide a scale
@@ -209,8 +223,247 @@ template <typename E> __device__ __forceinline__ void write_any(const PagedWrite
   }
 }
 
+// ---- head dims 64, 128, 256, 16-byte aligned rows ----
+// Bound: HBM, 2 bytes read and 1 written a value.  A lane takes 8 values (16 bytes in, 8 out), so a row is D / 8 lanes and
+// a wavefront step RPS rows.  A workgroup looks at `tile` tokens for one head of K or of V; its wavefronts share the runs
+// that begin there:
+//   - a run of several tokens is one wavefront's, a long one all four's, held in registers between the maximum and the
+//     conversion (one read; twice beyond 16 * RPS tokens);
+//   - single tokens (a decode step) go RPS at a time, one to each group of D / 8 lanes;
+//   - where a scale grows, the whole wavefront moves that page's earlier rows to it.
+typedef uint32_t w_u32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t w_u32x4 __attribute__((ext_vector_type(4)));
+typedef float w_f32x2 __attribute__((ext_vector_type(2)));
+
+typedef uint16_t w_u16x2 __attribute__((ext_vector_type(2)));
+
+// The largest magnitude of 8 values, as the bits of a 16-bit float: they order like the magnitudes.
+__device__ __forceinline__ uint32_t top_of8(w_u32x4 x) {
+  w_u16x2 m = __builtin_bit_cast(w_u16x2, x[0] & 0x7fff7fffu);
+#pragma unroll
+  for (int i = 1; i < 4; ++i) m = __builtin_elementwise_max(m, __builtin_bit_cast(w_u16x2, x[i] & 0x7fff7fffu));
+  return max((uint32_t)m[0], (uint32_t)m[1]);
+}
+// The same among the finite ones: for runs that hold an infinity or NaN.
+template <typename E> __device__ __forceinline__ uint32_t finite_top_of8(w_u32x4 x) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int h = 0; h < 32; h += 16) {
+      const uint32_t u = (x[i] >> h) & 0x7fffu;
+      m = max(m, u < E::kInfinite ? u : 0u);
+    }
+  return m;
+}
+template <typename E> __device__ __forceinline__ int scale_of_top(uint32_t top) {
+  return scale_for(__builtin_bit_cast(uint32_t, E::get((uint16_t)top)));
+}
+template <typename E> __device__ __forceinline__ w_u32x2 codes_of8(w_u32x4 x, int s, bool wild) {
+  w_u32x2 r;
+  if (wild) {
+    const float inv = pow2_code(254 - s);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      int c = __builtin_amdgcn_cvt_pk_fp8_f32(sat448(E::get((uint16_t)x[2 * i]) * inv), sat448(E::get((uint16_t)(x[2 * i] >> 16)) * inv), 0, false);
+      c = __builtin_amdgcn_cvt_pk_fp8_f32(sat448(E::get((uint16_t)x[2 * i + 1]) * inv), sat448(E::get((uint16_t)(x[2 * i + 1] >> 16)) * inv), c, true);
+      r[i] = (uint32_t)c;
+    }
+  } else {
+    const float scale = pow2_code(s);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      w_s16x2 c = {0, 0};
+      c = E::template codes2<false>(c, x[2 * i], scale);
+      c = E::template codes2<true>(c, x[2 * i + 1], scale);
+      r[i] = __builtin_bit_cast(uint32_t, c);
+    }
+  }
+  return r;
+}
+__device__ __forceinline__ w_u32x2 rescale8(w_u32x2 x, float f) {
+  w_u32x2 r;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const w_f32x2 lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)x[i], false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)x[i], true);
+    int c = __builtin_amdgcn_cvt_pk_fp8_f32(lo[0] * f, lo[1] * f, 0, false);
+    r[i] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(hi[0] * f, hi[1] * f, c, true);
+  }
+  return r;
+}
+
+// Rows [0, rows) of a page to the scale 2^(new - old) times larger; the whole wavefront, all arguments uniform.
+template <int D> __device__ __forceinline__ void rescale_rows(uint8_t *base, int64_t tok, int rows, int old, int s) {
+  constexpr int LPR = D / 8, RPS = 64 / LPR, N = 4;
+  const int lane = threadIdx.x & 63, r0 = lane / LPR, col = lane % LPR * 8;
+  const float f = pow2_code(max(127 + old - s, 0));
+  for (int r = r0; r < rows; r += N * RPS) {
+    w_u32x2 x[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (r + i * RPS < rows) x[i] = *(const w_u32x2 *)(base + (r + i * RPS) * tok + col);
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (r + i * RPS < rows) *(w_u32x2 *)(base + (r + i * RPS) * tok + col) = rescale8(x[i], f);
+  }
+}
+
+template <typename E, int D> __device__ __forceinline__ void write_rows(const PagedWriteArgs &a, uint8_t *list, uint32_t *tops) {
+  constexpr int LPR = D / 8, RPS = 64 / LPR, HOLD = 4;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int side = blockIdx.x % (2 * a.c.heads), head = side >> 1; // K or V of one head
+  const bool isv = side & 1;
+  const int64_t first = (int64_t)(blockIdx.x / (2 * a.c.heads)) * a.tile;
+  const int P = a.c.page_size;
+  const int64_t nslots = (int64_t)a.c.pages * P;
+  const uint16_t *x = isv ? a.v + head * a.v_head : a.k + head * a.k_head;
+  const int64_t x_tok = isv ? a.v_tok : a.k_tok, c_tok = isv ? a.c.v_tok : a.c.k_tok;
+  const int64_t c_page = isv ? a.c.v_page : a.c.k_page, s_page = isv ? a.c.vs_page : a.c.ks_page;
+  uint8_t *codes = isv ? a.c.v + head * a.c.v_head : a.c.k + head * a.c.k_head;
+  uint8_t *scales = isv ? a.c.vs + head * a.c.vs_head : a.c.ks + head * a.c.ks_head;
+  const int sub = lane / LPR, col = lane % LPR * 8;
+
+  // the runs that begin in this tile: lane i looks at token first + i (every wavefront comes to the same answer)
+  const int64_t tt = first + lane;
+  int32_t slot = -1;
+  bool leads = false, single = false, goes_on = false;
+  if (lane < a.tile && tt < a.tokens) {
+    slot = a.slots[tt];
+    const int32_t prev = tt ? a.slots[tt - 1] : -1, next = tt + 1 < a.tokens ? a.slots[tt + 1] : -1;
+    if (slot >= 0 && slot < nslots) {
+      const int r = slot % P;
+      goes_on = r && tt && prev == slot - 1;
+      leads = !goes_on;
+      single = leads && !(r + 1 < P && next == slot + 1);
+    }
+  }
+  uint64_t many = __ballot(leads && !single);
+  const uint64_t ones = __ballot(single), rest = __ballot(goes_on);
+
+  for (int turn = 0; many; ++turn, many &= many - 1) {
+    const int src = __builtin_ctzll(many);
+    const int64_t t = first + src;
+    const int32_t s0 = __builtin_amdgcn_readlane(slot, src);
+    const int row = s0 % P;
+    const int64_t page = s0 / P;
+    // the run's tokens: those that go on behind it, past the tile's end if it reaches that
+    int n = 1 + (src == 63 ? 0 : __builtin_ctzll(~(rest >> (src + 1))));
+    while (src + n >= a.tile) {
+      const bool on = row + n + lane < P && t + n + lane < a.tokens && a.slots[t + n + lane] == s0 + n + lane;
+      const uint64_t off = ~__ballot(on);
+      n += off ? __builtin_ctzll(off) : 64;
+      if (off) break;
+    }
+    // a short run is one wavefront's, a long one all four's
+    const bool shared = n > HOLD * RPS;
+    if (!shared && (turn & 3) != wave) continue;
+    const int r0 = shared ? wave * HOLD * RPS : 0, stride = shared ? 4 * HOLD * RPS : HOLD * RPS;
+    uint8_t *base = codes + page * c_page, *sp = scales + page * s_page;
+    const uint16_t *xr = x + t * x_tok + col;
+    const int old = row ? *sp : 0;
+    w_u32x4 hold[HOLD];
+    uint32_t amax = 0;
+    for (int b = r0; b < n; b += stride) {
+#pragma unroll
+      for (int i = 0; i < HOLD; ++i) {
+        const int r = b + i * RPS + sub;
+        hold[i] = (w_u32x4){0, 0, 0, 0};
+        if (r < n) hold[i] = *(const w_u32x4 *)(xr + r * x_tok);
+      }
+#pragma unroll
+      for (int i = 0; i < HOLD; ++i) amax = max(amax, top_of8(hold[i]));
+    }
+    auto over_run = [&](uint32_t m, int at) { // the maximum over all lanes that share the run
+      m = max64(m);
+      if (shared) {
+        if (lane == 0) tops[at + wave] = m;
+        __syncthreads();
+        m = max(max(tops[at], tops[at + 1]), max(tops[at + 2], tops[at + 3]));
+      }
+      return (uint32_t)__builtin_amdgcn_readfirstlane((int)m);
+    };
+    amax = over_run(amax, 0);
+    const bool wild = amax >= E::kInfinite;
+    if (wild) {
+      amax = 0;
+      for (int b = r0 + sub; b < n; b += stride)
+#pragma unroll
+        for (int i = 0; i < HOLD; ++i)
+          if (b + i * RPS < n) amax = max(amax, finite_top_of8<E>(*(const w_u32x4 *)(xr + (b + i * RPS) * x_tok)));
+      amax = over_run(amax, 4);
+    }
+    const int need = scale_of_top<E>(amax), s = row ? max(need, __builtin_amdgcn_readfirstlane(old)) : need;
+    if (row && s > old && (!shared || wave == 0)) rescale_rows<D>(base, c_tok, row, old, s);
+    for (int b = r0; b < n; b += stride) {
+#pragma unroll
+      for (int i = 0; i < HOLD; ++i) {
+        const int r = b + i * RPS + sub;
+        if (r >= n) continue;
+        if (n > stride) hold[i] = *(const w_u32x4 *)(xr + r * x_tok); // a run longer than the registers is read twice
+        *(w_u32x2 *)(base + (row + r) * c_tok + col) = codes_of8<E>(hold[i], s, wild);
+      }
+    }
+    if (shared) __syncthreads(); // (tops; and every wavefront has read the old scale)
+    if (lane == 0 && (!shared || wave == 0)) *sp = (uint8_t)s;
+  }
+
+  // single tokens: list[i] = the lane that found the i-th
+  if (single) list[wave * 64 + __builtin_amdgcn_mbcnt_hi((uint32_t)(ones >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)ones, 0))] = (uint8_t)lane;
+  __builtin_amdgcn_wave_barrier();
+  const int count = __builtin_popcountll(ones);
+  for (int i0 = wave * RPS; i0 < count; i0 += 4 * RPS) {
+    const bool mine = i0 + sub < count;
+    const int src = mine ? list[wave * 64 + i0 + sub] : 0;
+    const int32_t s0 = __shfl(slot, src);
+    const int row = s0 % P;
+    const int64_t page = s0 / P;
+    uint8_t *base = codes + page * c_page, *sp = scales + page * s_page;
+    w_u32x4 v = {0, 0, 0, 0};
+    int old = 0;
+    if (mine) {
+      v = *(const w_u32x4 *)(x + (first + src) * x_tok + col);
+      if (row) old = *sp;
+    }
+    uint32_t amax = top_of8(v);
+#pragma unroll
+    for (int d = 1; d < LPR; d <<= 1) amax = max(amax, (uint32_t)__shfl_xor((int)amax, d));
+    const bool wild = amax >= E::kInfinite;
+    if (__any(wild)) {
+      amax = finite_top_of8<E>(v);
+#pragma unroll
+      for (int d = 1; d < LPR; d <<= 1) amax = max(amax, (uint32_t)__shfl_xor((int)amax, d));
+    }
+    const int need = scale_of_top<E>(amax), s = row ? max(need, old) : need;
+    uint64_t grown = __ballot(mine && row && need > old);
+    while (grown) { // a group of lanes at a time
+      const int l = __builtin_ctzll(grown);
+      grown &= ~((LPR == 64 ? ~0ull : (1ull << LPR) - 1) << l);
+      const int64_t pg = __builtin_amdgcn_readlane((int)page, l);
+      rescale_rows<D>(codes + pg * c_page, c_tok, __builtin_amdgcn_readlane(row, l), __builtin_amdgcn_readlane(old, l),
+                      __builtin_amdgcn_readlane(s, l));
+    }
+    if (mine) {
+      *(w_u32x2 *)(base + row * c_tok + col) = codes_of8<E>(v, s, wild);
+      if (col == 0) *sp = (uint8_t)s;
+    }
+  }
+}
+
+#define PAGED_WRITE(T, E, D)                                                                          \
+  extern "C" __global__ __launch_bounds__(256, 6) void paged_write_##T##_d##D(PagedWriteArgs a) {      \
+    __shared__ uint8_t list[256];                                                                     \
+    __shared__ uint32_t tops[8];                                                                      \
+    write_rows<E, D>(a, list, tops);                                                                     \
+  }
 } // namespace
 
+PAGED_WRITE(bf16, Bf16, 64)
+PAGED_WRITE(bf16, Bf16, 128)
+PAGED_WRITE(bf16, Bf16, 256)
+PAGED_WRITE(f16, Fp16, 64)
+PAGED_WRITE(f16, Fp16, 128)
+PAGED_WRITE(f16, Fp16, 256)
+#undef PAGED_WRITE
 extern "C" __global__ __launch_bounds__(256) void paged_write_any_bf16(PagedWriteArgs a) { write_any<Bf16>(a); }
 extern "C" __global__ __launch_bounds__(256) void paged_write_any_f16(PagedWriteArgs a) { write_any<Fp16>(a); }
 

@@ -26,7 +26,7 @@ struct PagedWriteArgs {
   const int32_t *slots;
   int64_t k_tok, k_head, v_tok, v_head;
   int32_t tokens;
-  int32_t tile;          // consecutive tokens per wavefront
+  int32_t tile;          // consecutive tokens per workgroup (paged_write_any: per wavefront)
 };
 
 struct PagedAttnArgs {

@@ -128,12 +128,26 @@ extern "C" int tt_paged_write(const void *k, const void *v, const int64_t k_stri
   a.k = (const uint16_t *)k; a.v = (const uint16_t *)v; a.slots = slot_map;
   a.k_tok = k_strides[0]; a.k_head = k_strides[1]; a.v_tok = v_strides[0]; a.v_head = v_strides[1];
   a.tokens = tokens;
-  a.tile = 1;
-  const int64_t units = cdiv64(tokens, a.tile) * a.c.heads * 2;
-  if (cdiv64(units, 4) > INT32_MAX) return fail(RT_ERR_UNSUPPORTED, "%s: tokens * heads exceeds the grid", who);
   void *args[] = {&a};
-  return launch("paged", dtype == TT_BF16 ? "paged_write_any_bf16" : "paged_write_any_f16", dim3((uint32_t)cdiv64(units, 4)),
-                dim3(256), 0, stream, args, 1);
+  const PagedCacheArgs &c = a.c;
+  const int D = c.head_dim;
+  const bool al = aligned16(k) && aligned16(v) && (a.k_tok | a.k_head | a.v_tok | a.v_head) % 8 == 0 && aligned(c.k, 8) &&
+                  aligned(c.v, 8) && (c.k_page | c.k_head | c.k_tok | c.v_page | c.v_head | c.v_tok) % 8 == 0;
+  char name[64];
+  int64_t wgs;
+  if (al && (D == 64 || D == 128 || D == 256)) {
+    // Tokens per workgroup.  16 single tokens are what its wavefronts do at once at head dim 128; once that gives more
+    // workgroups than the chip holds (8 a CU), 64 leave fewer that only find out that a run began before them.
+    a.tile = cdiv64(tokens, 16) * c.heads * 2 > 8 * props()->multiprocessor_count ? 64 : 16;
+    wgs = cdiv64(tokens, a.tile) * c.heads * 2;
+    snprintf(name, sizeof(name), "paged_write_%s_d%d", dtype == TT_BF16 ? "bf16" : "f16", D);
+  } else {
+    a.tile = 1;
+    wgs = cdiv64((int64_t)tokens * c.heads * 2, 4);
+    snprintf(name, sizeof(name), "paged_write_any_%s", dtype == TT_BF16 ? "bf16" : "f16");
+  }
+  if (wgs > INT32_MAX) return fail(RT_ERR_UNSUPPORTED, "%s: tokens * heads exceeds the grid", who);
+  return launch("paged", name, dim3((uint32_t)wgs), dim3(256), 0, stream, args, 1);
 }
 
 extern "C" int tt_paged_attn_workspace(int32_t B, int32_t max_pages, int32_t tokens, int32_t heads_q, int32_t max_q,
