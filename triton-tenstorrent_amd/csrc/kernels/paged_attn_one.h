@@ -18,6 +18,7 @@
 // once, whatever the lengths: workgroup i takes units [i U / G, (i+1) U / G) and meets at most two (sequence, head)
 // pairs that it does not have whole, the first and the last.  Those leave partial results (fp32 sum, reference, sum of
 // probabilities) in the workspace and paged_attn_join adds them in order, so results do not change from run to run.
+// While a pair's four wavefronts are merged, the next pair's first loads are under way.
 #pragma once
 
 namespace one {
@@ -37,36 +38,64 @@ __device__ __forceinline__ float unweight(int e) { return __builtin_bit_cast(flo
 constexpr float kOut = 0x1p-6f; // 2^(kBase - 127): V of scale code kBase
 constexpr float kInf = __builtin_inff();
 
-template <int D, int MT> constexpr int subtiles() { return D * MT >= 256 ? 2 : 4; } // of 16 keys, per wavefront and step
+// Subtiles of 16 keys that a wavefront takes in one step.  Two leave room for three workgroups on a CU at head dim 128
+// and make finer units than four (513 keys, 8 heads: 7.2 us against 9.3); at head dim 64 two would be too few bytes in flight.
+template <int D, int MT> constexpr int subtiles() { return D * MT >= 128 ? 2 : 4; }
 
-// Units of work of sequence b: n = 0 where it is not this kernel's (no query, or several).
-struct Seq { int32_t len, units; };
+// Sequence b as this kernel sees it: no units where it is not this kernel's (no query, or several).
+struct Seq { int32_t q0, len, units; };
 template <int UK> __device__ __forceinline__ Seq seq_of(const PagedAttnArgs &a, int b) {
   const int32_t q0 = a.cu_q[b], q1 = a.cu_q[b + 1];
   const int32_t len = clampi(a.lens[b], 0, a.max_pages * a.c.page_size);
   const bool mine = q1 - q0 == 1 && q0 >= 0 && q0 < a.tokens;
-  return {len, mine ? max((len + UK - 1) / UK, 1) : 0};
+  return {q0, len, mine ? max((len + UK - 1) / UK, 1) : 0};
 }
 
-// Prefix sums of the units of all sequences, in LDS: base[i] = units before thread i's `per` consecutive sequences.
-template <int UK> __device__ __forceinline__ int scan_units(const PagedAttnArgs &a, int32_t *base, int32_t *part) {
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, per = (a.b + 255) / 256;
-  int32_t n = 0;
-  for (int b = min(tid * per, a.b); b < min(tid * per + per, a.b); ++b) n += seq_of<UK>(a, b).units;
-  int32_t v = n;
+// Where the units of all sequences lie: every wavefront scans the lengths by itself, lane i the sequences i * per and
+// up.  Up to 64 sequences stay in registers.
+template <int UK> struct Walk {
+  const PagedAttnArgs &a;
+  int per;
+  int32_t base, total;
+  Seq own;
+  __device__ __forceinline__ Walk(const PagedAttnArgs &args) : a(args) {
+    const int lane = threadIdx.x & 63;
+    per = (a.b + 63) / 64;
+    int32_t n = 0;
+    own = {0, 0, 0};
+    for (int b = min(lane * per, a.b); b < min(lane * per + per, a.b); ++b) {
+      own = seq_of<UK>(a, b);
+      n += own.units;
+    }
+    int32_t v = n;
 #pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const int32_t o = __shfl_up(v, d);
-    if (lane >= d) v += o;
+    for (int d = 1; d < 64; d <<= 1) {
+      const int32_t o = __shfl_up(v, d);
+      if (lane >= d) v += o;
+    }
+    base = v - n;
+    total = __builtin_amdgcn_readlane(v, 63);
   }
-  if (lane == 63) part[wave] = v;
-  __syncthreads();
-  for (int w = 0; w < wave; ++w) v += part[w];
-  base[tid] = v - n;
-  const int total = part[0] + part[1] + part[2] + part[3];
-  __syncthreads();
-  return total;
-}
+  __device__ __forceinline__ Seq at(int b) const {
+    if (per != 1) return seq_of<UK>(a, b);
+    return {__builtin_amdgcn_readlane(own.q0, b), __builtin_amdgcn_readlane(own.len, b), __builtin_amdgcn_readlane(own.units, b)};
+  }
+  // the sequence that holds unit u of `heads` times the total, and the units before it
+  __device__ __forceinline__ int find(int64_t u, int heads, int64_t *before, Seq *sq) const {
+    const int l = 63 - __builtin_clzll(__ballot((int64_t)base * heads <= u));
+    int b = l * per;
+    *before = (int64_t)__builtin_amdgcn_readlane(base, l) * heads;
+    *sq = at(b);
+    step(u, heads, &b, before, sq);
+    return b;
+  }
+  __device__ __forceinline__ void step(int64_t u, int heads, int *b, int64_t *before, Seq *sq) const {
+    while (*before + (int64_t)sq->units * heads <= u) { // (u is less than all units: ends before the sequences do)
+      *before += (int64_t)sq->units * heads;
+      *sq = at(++*b);
+    }
+  }
+};
 
 struct Bf {
   typedef bf16x8 frag;
@@ -104,58 +133,104 @@ __device__ __forceinline__ int64_t lane64(int32_t lo, int32_t hi, int lane) {
 // Partial result p of the workspace: rows * D sums, then rows pairs (reference, sum).
 template <int D, int MT> constexpr int part_floats() { return 16 * MT * D + 32 * MT; }
 
+// A pair that is split and whose first units are workgroup i's: the i-th entry behind the partial results.  Its parts are
+// slot 2 i + slot of workgroup i and slot 2 j of workgroups j = i + 1 .. last.
+struct Split { int32_t row, head, last, slot; }; // row: packed row of q, -1 = none
+
 template <class E, int D, int MT>
 __device__ __forceinline__ void body(const PagedAttnArgs &a, float *lds) {
   constexpr int NS = subtiles<D, MT>(), UK = 64 * NS, KL = D / 64, VW = D / 64; // 16-byte loads of K, dwords of V per row
   constexpr int VB = D / 16, IB = 64 / NS, LD = D + 4;                      // LD: padded LDS row of the merge
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c16 = lane & 15, g = lane >> 4;
-  int32_t *base = (int32_t *)lds, *part = base + 256;
-  const int64_t U = (int64_t)scan_units<UK>(a, base, part) * a.c.heads;
+  const Walk<UK> walk(a);
+  const int64_t U = (int64_t)walk.total * a.c.heads;
   const int64_t G = min((int64_t)gridDim.x, U); // fewer units than workgroups: one each
-  if (blockIdx.x >= G) return;
+  Split *split = (Split *)(a.part + 2 * (int64_t)gridDim.x * part_floats<D, MT>()) + blockIdx.x;
+  if (blockIdx.x >= G) {
+    if (a.part && tid == 0) split->row = -1;
+    return;
+  }
   int64_t u = blockIdx.x * U / G;
   const int64_t u_end = (blockIdx.x + 1) * U / G, u_first = u;
-
-  // the sequence that holds unit u
-  const int per = (a.b + 255) / 256;
-  int lo = 0, hi = 255;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if ((int64_t)base[mid] * a.c.heads <= u) lo = mid; else hi = mid - 1;
-  }
-  int b = __builtin_amdgcn_readfirstlane(min(lo * per, a.b - 1));
-  int64_t before = uniform64((int64_t)base[lo] * a.c.heads);
-  __syncthreads(); // `base` shares its LDS with the merge
-  Seq sq = seq_of<UK>(a, b);
-  while (before + (int64_t)sq.units * a.c.heads <= u) {
-    before += (int64_t)sq.units * a.c.heads;
-    sq = seq_of<UK>(a, ++b);
-  }
+  int64_t before;
+  Seq sq;
+  int b = walk.find(u, a.c.heads, &before, &sq);
+  bool noted = false;
 
   const uint32_t klane = (uint32_t)(c16 * a.c.k_tok + g * 16);
   uint32_t vlane[4];
 #pragma unroll
   for (int r = 0; r < 4; ++r) vlane[r] = (uint32_t)((g * 4 + r) * a.c.v_tok + c16 * VB);
 
-  while (u < u_end) {
-    while (sq.units == 0 || before + (int64_t)sq.units * a.c.heads <= u) { // (u < U: ends before b does)
-      before += (int64_t)sq.units * a.c.heads;
-      sq = seq_of<UK>(a, ++b);
-    }
-    const int32_t len = sq.len, units = sq.units;
-    const int hk = (int)((u - before) / units);
-    const int c0 = (int)(u - before - (int64_t)hk * units);
-    const int n = (int)min((int64_t)(units - c0), u_end - u);
-    const int32_t t = a.cu_q[b];
-    const int32_t *table = a.table + (int64_t)b * a.table_stride;
-    const uint8_t *kh = a.c.k + hk * a.c.k_head, *vh = a.c.v + hk * a.c.v_head;
+  // the pair at u: units c0 .. c0 + n of its sq.units
+  int hk, c0, n;
+  const int32_t *table;
+  const uint8_t *kh, *vh;
+  typename E::frag qf[MT][2 * KL];
 
-    typename E::frag qf[MT][2 * KL];
+  // What lane (it % IB) * NS + s knows of subtile s of step it: where its rows lie, how many count, its scales.
+  int32_t ko_lo, ko_hi, vo_lo, vo_hi, live, vcode;
+  float kscale;
+  auto batch = [&](int it0) {
+    const int64_t key = (int64_t)(c0 + it0 + lane / NS) * UK + wave * (16 * NS) + (lane % NS) * 16;
+    const uint32_t sub = (uint32_t)(key >> 4);
+    const uint32_t blk = (uint32_t)(((uint64_t)sub * a.page_magic) >> 36);
+    int32_t page = key < sq.len ? table[blk] : -1;
+    const bool ok = page >= 0 && page < a.c.pages;
+    page = ok ? page : 0;
+    const int64_t row = ok ? ((int64_t)sub - (int64_t)blk * (a.c.page_size >> 4)) * 16 : 0;
+    const int64_t ko = page * a.c.k_page + row * a.c.k_tok, vo = page * a.c.v_page + row * a.c.v_tok;
+    ko_lo = (int32_t)ko; ko_hi = (int32_t)(ko >> 32); vo_lo = (int32_t)vo; vo_hi = (int32_t)(vo >> 32);
+    live = ok ? (int32_t)min((int64_t)sq.len - key, (int64_t)16) : 0;
+    kscale = pow2_code(a.c.ks[page * a.c.ks_page + hk * a.c.ks_head]) * a.qk_scale;
+    vcode = ok ? a.c.vs[page * a.c.vs_page + hk * a.c.vs_head] : 0;
+  };
+
+  u32x4 kr[NS][KL];
+  uint32_t vr[NS][4][VW];
+  auto load_k = [&](int it) {
+#pragma unroll
+    for (int s = 0; s < NS; ++s) {
+      const uint8_t *kp = kh + lane64(ko_lo, ko_hi, (it % IB) * NS + s);
+#pragma unroll
+      for (int h = 0; h < KL; ++h) kr[s][h] = *(const u32x4 *)(kp + klane + h * 64);
+    }
+  };
+  auto load_v = [&](int it) {
+#pragma unroll
+    for (int s = 0; s < NS; ++s) {
+      const uint8_t *vp = vh + lane64(vo_lo, vo_hi, (it % IB) * NS + s);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        if constexpr (VW == 1) vr[s][r][0] = *(const uint32_t *)(vp + vlane[r]);
+        if constexpr (VW == 2) {
+          const u32x2 x = *(const u32x2 *)(vp + vlane[r]);
+          vr[s][r][0] = x[0]; vr[s][r][1] = x[1];
+        }
+        if constexpr (VW == 4) {
+          const u32x4 x = *(const u32x4 *)(vp + vlane[r]);
+          vr[s][r][0] = x[0]; vr[s][r][1] = x[1]; vr[s][r][2] = x[2]; vr[s][r][3] = x[3];
+        }
+      }
+    }
+  };
+
+  // one set of registers each for K and V: a step's loads go out as soon as the step before has used them up
+  auto open = [&]() {
+    hk = (int)((u - before) / sq.units);
+    c0 = (int)(u - before - (int64_t)hk * sq.units);
+    n = (int)min((int64_t)(sq.units - c0), u_end - u);
+    table = a.table + (int64_t)b * a.table_stride;
+    kh = a.c.k + hk * a.c.k_head;
+    vh = a.c.v + hk * a.c.v_head;
+    batch(0);
+    load_k(0);
+    load_v(0);
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
       const int row = m * 16 + c16;
-      const uint16_t *qr = a.q + t * a.q_tok + (hk * a.group + row) * a.q_head + g * 16;
+      const uint16_t *qr = a.q + sq.q0 * a.q_tok + (hk * a.group + row) * a.q_head + g * 16;
 #pragma unroll
       for (int s = 0; s < 2 * KL; ++s) {
         u32x4 z = {0, 0, 0, 0};
@@ -163,7 +238,9 @@ __device__ __forceinline__ void body(const PagedAttnArgs &a, float *lds) {
         qf[m][s] = __builtin_bit_cast(typename E::frag, z);
       }
     }
-
+  };
+  open();
+  for (;;) {
     f32x4 acc[MT][VB];
     float mref[MT], lsum[MT];
 #pragma unroll
@@ -173,58 +250,6 @@ __device__ __forceinline__ void body(const PagedAttnArgs &a, float *lds) {
 #pragma unroll
       for (int i = 0; i < VB; ++i) acc[m][i] = (f32x4){0, 0, 0, 0};
     }
-
-    // What lane (it % IB) * NS + s knows of subtile s of step it: where its rows lie, how many count, its scales.
-    int32_t ko_lo, ko_hi, vo_lo, vo_hi, live, vcode;
-    float kscale;
-    auto batch = [&](int it0) {
-      const int64_t key = (int64_t)(c0 + it0 + lane / NS) * UK + wave * (16 * NS) + (lane % NS) * 16;
-      const uint32_t sub = (uint32_t)(key >> 4);
-      const uint32_t blk = (uint32_t)(((uint64_t)sub * a.page_magic) >> 36);
-      int32_t page = key < len ? table[blk] : -1;
-      const bool ok = page >= 0 && page < a.c.pages;
-      page = ok ? page : 0;
-      const int64_t row = ok ? ((int64_t)sub - (int64_t)blk * (a.c.page_size >> 4)) * 16 : 0;
-      const int64_t ko = page * a.c.k_page + row * a.c.k_tok, vo = page * a.c.v_page + row * a.c.v_tok;
-      ko_lo = (int32_t)ko; ko_hi = (int32_t)(ko >> 32); vo_lo = (int32_t)vo; vo_hi = (int32_t)(vo >> 32);
-      live = ok ? (int32_t)min((int64_t)len - key, (int64_t)16) : 0;
-      kscale = pow2_code(a.c.ks[page * a.c.ks_page + hk * a.c.ks_head]) * a.qk_scale;
-      vcode = ok ? a.c.vs[page * a.c.vs_page + hk * a.c.vs_head] : 0;
-    };
-
-    u32x4 kr[NS][KL];
-    uint32_t vr[NS][4][VW];
-    auto load_k = [&](int it) {
-#pragma unroll
-      for (int s = 0; s < NS; ++s) {
-        const uint8_t *kp = kh + lane64(ko_lo, ko_hi, (it % IB) * NS + s);
-#pragma unroll
-        for (int h = 0; h < KL; ++h) kr[s][h] = *(const u32x4 *)(kp + klane + h * 64);
-      }
-    };
-    auto load_v = [&](int it) {
-#pragma unroll
-      for (int s = 0; s < NS; ++s) {
-        const uint8_t *vp = vh + lane64(vo_lo, vo_hi, (it % IB) * NS + s);
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          if constexpr (VW == 1) vr[s][r][0] = *(const uint32_t *)(vp + vlane[r]);
-          if constexpr (VW == 2) {
-            const u32x2 x = *(const u32x2 *)(vp + vlane[r]);
-            vr[s][r][0] = x[0]; vr[s][r][1] = x[1];
-          }
-          if constexpr (VW == 4) {
-            const u32x4 x = *(const u32x4 *)(vp + vlane[r]);
-            vr[s][r][0] = x[0]; vr[s][r][1] = x[1]; vr[s][r][2] = x[2]; vr[s][r][3] = x[3];
-          }
-        }
-      }
-    };
-
-    // one set of registers each for K and V: a step's loads go out as soon as the step before has used them up
-    batch(0);
-    load_k(0);
-    load_v(0);
     for (int it = 0; it < n; ++it) {
       int nv[NS], vc[NS];
       float ks[NS];
@@ -339,7 +364,23 @@ __device__ __forceinline__ void body(const PagedAttnArgs &a, float *lds) {
       if (it + 1 < n) load_v(it + 1);
     }
 
-    // ---- merge the four wavefronts ----
+    // ---- the next pair's loads, then the merge of the four wavefronts ----
+    const int32_t t = sq.q0;
+    const int my_hk = hk;
+    const bool whole = n == sq.units;
+    // (the first pair of this workgroup takes slot 0, a later one that is not whole can only be its last: slot 1)
+    const int which = u == u_first ? 0 : 1;
+    if (!whole && c0 == 0) {
+      const int64_t last = before + (int64_t)(hk + 1) * sq.units - 1; // the pair's last unit
+      if (tid == 0) *split = {t, hk, (int32_t)(((last + 1) * G + U - 1) / U - 1), which};
+      noted = true;
+    }
+    u += n;
+    const bool more = u < u_end;
+    if (more) {
+      walk.step(u, a.c.heads, &b, &before, &sq);
+      open();
+    }
     float *wo = lds, *wml = lds + 4 * 16 * MT * LD;   // sums [wave][row][LD], (reference, sum) [wave][row]
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
@@ -355,9 +396,7 @@ __device__ __forceinline__ void body(const PagedAttnArgs &a, float *lds) {
           *(f32x4 *)(wo + row * LD + (g * 4 + r) * VB + i) = (f32x4){acc[m][i][r], acc[m][i + 1][r], acc[m][i + 2][r], acc[m][i + 3][r]};
     }
     __syncthreads();
-    const bool whole = c0 == 0 && n == units;
-    // (the first segment of this workgroup takes slot 0, a later one that is not whole can only be its last: slot 1)
-    float *slot = a.part + (2 * (int64_t)blockIdx.x + (u == u_first ? 0 : 1)) * part_floats<D, MT>();
+    float *slot = a.part + (2 * (int64_t)blockIdx.x + which) * part_floats<D, MT>();
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
       const int row = m * 16 + (tid >> 4), d0 = (tid & 15) * VB;
@@ -378,7 +417,7 @@ __device__ __forceinline__ void body(const PagedAttnArgs &a, float *lds) {
       }
       if (whole) {
         if (row < a.group) {
-          const int hq = hk * a.group + row;
+          const int hq = my_hk * a.group + row;
           const bool none = l == 0.0f && mx == -kInf;
           const float inv = none ? 0.0f : kOut / l;
           uint16_t *op = a.o + t * a.o_tok + hq * a.o_head + d0;
@@ -397,86 +436,100 @@ __device__ __forceinline__ void body(const PagedAttnArgs &a, float *lds) {
         }
       }
     }
+    if (!more) break;
     __syncthreads();
-    u += n;
   }
+  if (a.part && !noted && tid == 0) split->row = -1;
 }
 
-// Joins the partial results of one (sequence, head): grid (b, heads).
-template <class E, int D, int MT> __device__ __forceinline__ void join(const PagedAttnArgs &a, int32_t *base) {
-  constexpr int NS = subtiles<D, MT>(), UK = 64 * NS, VB = D / 16;
-  const int b = blockIdx.x, hk = blockIdx.y, tid = threadIdx.x;
-  const Seq sq = seq_of<UK>(a, b);
-  if (sq.units <= 1) return; // one unit, or none, is never split
-  const int64_t U = (int64_t)scan_units<UK>(a, base, base + 256) * a.c.heads;
-  const int64_t G = min((int64_t)a.split_groups, U);
-  const int per = (a.b + 255) / 256, th = b / per;
-  int64_t first = base[th];
-  for (int x = th * per; x < b; ++x) first += seq_of<UK>(a, x).units;
-  first = first * a.c.heads + (int64_t)hk * sq.units;
-  // the workgroups that own its first and its last unit
-  auto owner = [&](int64_t u) { return ((u + 1) * G + U - 1) / U - 1; };
-  const int64_t i0 = owner(first), i1 = owner(first + sq.units - 1);
-  if (i0 == i1) return;
-  const int64_t s0 = 2 * i0 + (i0 * U / G < first ? 1 : 0);
-  auto slot = [&](int64_t i) { return a.part + (i == i0 ? s0 : 2 * i) * part_floats<D, MT>(); };
-  const int32_t t = a.cu_q[b];
+// Adds the parts of the split pair that workgroup blockIdx.x of the launch before noted, if any.  D / 4 threads a row; what
+// is left of the 256 takes several rows or several parts at once.
+template <class E, int D, int MT> __device__ __forceinline__ void join(const PagedAttnArgs &a, f32x4 *lds) {
+  constexpr int TPR = D / 4, SLOTS = 256 / TPR, PF = part_floats<D, MT>();
+  const Split sp = ((const Split *)(a.part + 2 * (int64_t)gridDim.x * PF))[blockIdx.x];
+  if (sp.row < 0) return;
+  const int tid = threadIdx.x, d4 = tid % TPR, at = tid / TPR;
+  int across = 1; // rows at once
+  while (across < SLOTS && across < a.group) across <<= 1;
+  const int deep = SLOTS / across, r0 = at % across, p0 = at / across;
+  const int parts = sp.last - (int)blockIdx.x + 1;
+  const float *first = a.part + (2 * (int64_t)blockIdx.x + sp.slot) * PF, *later = a.part + 2 * (int64_t)blockIdx.x * PF;
+  float *lm = (float *)(lds + 256), *ll = lm + 256;
+  for (int rb = 0; rb < a.group; rb += across) {
+    const int row = min(rb + r0, 16 * MT - 1);
+    float m = -kInf, l = 0.0f;
+    f32x4 o = {0, 0, 0, 0};
+    for (int p = p0; p < parts; p += 4 * deep) {
+      float pm[4], pl[4];
+      f32x4 po[4];
 #pragma unroll
-  for (int m = 0; m < MT; ++m) {
-    const int row = m * 16 + (tid >> 4), d0 = (tid & 15) * VB;
-    if (row >= a.group) continue;
-    float mx = -kInf;
-    for (int64_t i = i0; i <= i1; ++i) mx = fmaxf(mx, slot(i)[16 * MT * D + row * 2]);
-    const float mm = mx == -kInf ? 0.0f : mx;
-    float l = 0.0f, o[VB];
+      for (int i = 0; i < 4; ++i) {
+        const int j = min(p + i * deep, parts - 1);
+        const float *x = j ? later + 2 * (int64_t)j * PF : first;
+        pm[i] = x[16 * MT * D + row * 2];
+        pl[i] = x[16 * MT * D + row * 2 + 1];
+        po[i] = *(const f32x4 *)(x + row * D + d4 * 4);
+      }
 #pragma unroll
-    for (int i = 0; i < VB; ++i) o[i] = 0.0f;
-    for (int64_t i = i0; i <= i1; ++i) {
-      const float *p = slot(i);
-      const float mw = p[16 * MT * D + row * 2];
-      const float f = mw == -kInf ? 1.0f : __builtin_amdgcn_exp2f(mw - mm);
-      l += p[16 * MT * D + row * 2 + 1] * f;
-#pragma unroll
-      for (int j = 0; j < VB; j += 4) {
-        const f32x4 x = *(const f32x4 *)(p + row * D + d0 + j);
-        o[j] += x[0] * f; o[j + 1] += x[1] * f; o[j + 2] += x[2] * f; o[j + 3] += x[3] * f;
+      for (int i = 0; i < 4; ++i) {
+        if (p + i * deep >= parts) break;
+        const float mn = fmaxf(m, pm[i]), ref = mn == -kInf ? 0.0f : mn;
+        // (a row of NaN scores has reference -inf and a NaN sum: it has to stay)
+        const float f = m == -kInf ? 1.0f : __builtin_amdgcn_exp2f(m - ref), w = pm[i] == -kInf ? 1.0f : __builtin_amdgcn_exp2f(pm[i] - ref);
+        l = l * f + pl[i] * w;
+        o = o * f + po[i] * w;
+        m = mn;
       }
     }
-    const int hq = hk * a.group + row;
-    const bool none = l == 0.0f && mx == -kInf;
-    const float inv = none ? 0.0f : kOut / l;
-    uint16_t *op = a.o + t * a.o_tok + hq * a.o_head + d0;
-#pragma unroll
-    for (int i = 0; i < VB; i += 2)
-      *(uint32_t *)(op + i) = (uint32_t)E::out(o[i] * inv) |
-                              (uint32_t)E::out(o[i + 1] * inv) << 16;
-    if (a.lse && d0 == 0) a.lse[(int64_t)t * a.heads_q + hq] = none ? -kInf : mx - kLift + __builtin_log2f(l);
+    if (deep > 1) {
+      lds[tid] = o;
+      lm[tid] = m;
+      ll[tid] = l;
+      __syncthreads();
+      if (p0 == 0)
+        for (int q = 1; q < deep; ++q) {
+          const int y = tid + q * across * TPR;
+          const float mn = fmaxf(m, lm[y]), ref = mn == -kInf ? 0.0f : mn;
+          const float f = m == -kInf ? 1.0f : __builtin_amdgcn_exp2f(m - ref), w = lm[y] == -kInf ? 1.0f : __builtin_amdgcn_exp2f(lm[y] - ref);
+          l = l * f + ll[y] * w;
+          o = o * f + lds[y] * w;
+          m = mn;
+        }
+      __syncthreads();
+    }
+    if (p0 == 0 && rb + r0 < a.group) {
+      const int hq = sp.head * a.group + row;
+      const bool none = l == 0.0f && m == -kInf;
+      const float inv = none ? 0.0f : kOut / l;
+      *(u32x2 *)(a.o + sp.row * a.o_tok + hq * a.o_head + d4 * 4) =
+          (u32x2){(uint32_t)E::out(o[0] * inv) | (uint32_t)E::out(o[1] * inv) << 16, (uint32_t)E::out(o[2] * inv) | (uint32_t)E::out(o[3] * inv) << 16};
+      if (a.lse && d4 == 0) a.lse[(int64_t)sp.row * a.heads_q + hq] = none ? -kInf : m - kLift + __builtin_log2f(l);
+    }
   }
 }
 
-template <int D, int MT> constexpr int lds_floats() {
-  return 4 * 16 * MT * (D + 4) + 4 * 16 * MT * 2;
-}
+template <int D, int MT> constexpr int lds_floats() { return 4 * 16 * MT * (D + 4) + 4 * 16 * MT * 2; }
 
 } // namespace one
 
-#define PAGED_ONE(T, E, D, MT)                                                                                \
-  extern "C" __global__ __launch_bounds__(256, 2) void paged_attn_one_##T##_d##D##_r##MT(PagedAttnArgs a) {    \
+#define PAGED_ONE(T, E, D, MT, OCC)                                                                           \
+  extern "C" __global__ __launch_bounds__(256, OCC) void paged_attn_one_##T##_d##D##_r##MT(PagedAttnArgs a) {  \
     __shared__ __align__(16) float lds[one::lds_floats<D, MT>()];                                             \
     one::body<one::E, D, MT>(a, lds);                                                                         \
   }                                                                                                           \
   extern "C" __global__ __launch_bounds__(256) void paged_attn_join_##T##_d##D##_r##MT(PagedAttnArgs a) {      \
-    __shared__ int32_t base[264];                                                                             \
-    one::join<one::E, D, MT>(a, base);                                                        \
+    __shared__ one::f32x4 lds[256 + 128];                                                                     \
+    one::join<one::E, D, MT>(a, lds);                                                                         \
   }
-PAGED_ONE(bf16, Bf, 64, 1)
-PAGED_ONE(bf16, Bf, 64, 2)
-PAGED_ONE(bf16, Bf, 128, 1)
-PAGED_ONE(bf16, Bf, 128, 2)
-PAGED_ONE(bf16, Bf, 256, 1)
-PAGED_ONE(f16, Hf, 64, 1)
-PAGED_ONE(f16, Hf, 64, 2)
-PAGED_ONE(f16, Hf, 128, 1)
-PAGED_ONE(f16, Hf, 128, 2)
-PAGED_ONE(f16, Hf, 256, 1)
+// (the last number: workgroups on a CU, which the host's grid counts on too)
+PAGED_ONE(bf16, Bf, 64, 1, 3)
+PAGED_ONE(bf16, Bf, 64, 2, 3)
+PAGED_ONE(bf16, Bf, 128, 1, 3)
+PAGED_ONE(bf16, Bf, 128, 2, 2)
+PAGED_ONE(bf16, Bf, 256, 1, 2)
+PAGED_ONE(f16, Hf, 64, 1, 3)
+PAGED_ONE(f16, Hf, 64, 2, 3)
+PAGED_ONE(f16, Hf, 128, 1, 3)
+PAGED_ONE(f16, Hf, 128, 2, 2)
+PAGED_ONE(f16, Hf, 256, 1, 2)
 #undef PAGED_ONE

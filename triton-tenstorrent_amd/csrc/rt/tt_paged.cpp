@@ -63,11 +63,11 @@ Route route_of(const PagedCacheArgs &c, int32_t B, int32_t max_pages, int32_t to
   r.rows = !r.one || max_q > 1;
   if (r.one) {
     r.one_tiles = group > 16 ? 2 : 1;
-    const int64_t unit = D * r.one_tiles >= 256 ? 128 : 256;
+    const int64_t unit = D * r.one_tiles >= 128 ? 128 : 256;
     const int64_t most = std::max<int64_t>(cdiv64(keys, unit), 1);
-    r.one_groups = (uint32_t)std::min<int64_t>(most * c.heads * std::min(B, tokens), 2 * cus);
+    r.one_groups = (uint32_t)std::min<int64_t>(most * c.heads * std::min(B, tokens), (D * r.one_tiles > 128 ? 2 : 3) * cus);
     r.one_join = most > 1 && r.one_groups > 1;
-    if (r.one_join) r.one_bytes = 2 * (size_t)r.one_groups * (16 * r.one_tiles * D + 32 * r.one_tiles) * sizeof(float);
+    if (r.one_join) r.one_bytes = (size_t)r.one_groups * (2 * (16 * r.one_tiles * D + 32 * r.one_tiles) * sizeof(float) + 16);
   }
   r.workspace = r.one_bytes;
   if (r.rows) {
@@ -208,16 +208,15 @@ extern "C" int tt_paged_attn(const void *q, const int64_t q_strides[2], const tt
   if (r.fast && al) {
     const uint64_t per = (uint64_t)c.page_size / 16;
     a.page_magic = ((1ull << 36) + per - 1) / per;
-    a.split_groups = (int32_t)r.one_groups;
     a.splits = r.splits;
     a.rows_min = r.one ? 2 : 1;
     if (r.one) {
-      a.part = (float *)workspace;
+      a.part = r.one_join ? (float *)workspace : nullptr;
       snprintf(name, sizeof(name), "paged_attn_one_%s_d%d_r%d", type, c.head_dim, r.one_tiles);
       if ((rc = launch("paged", name, dim3(r.one_groups), dim3(256), 0, stream, args, 1))) return rc;
       if (r.one_join) {
         snprintf(name, sizeof(name), "paged_attn_join_%s_d%d_r%d", type, c.head_dim, r.one_tiles);
-        if ((rc = launch("paged", name, dim3((uint32_t)B, (uint32_t)c.heads), dim3(256), 0, stream, args, 1))) return rc;
+        if ((rc = launch("paged", name, dim3(r.one_groups), dim3(256), 0, stream, args, 1))) return rc;
       }
     }
     if (r.rows) {
