@@ -660,53 +660,69 @@ def _refuse(who: str, why: str):
     raise rt.InvalidLaunch(rt.RT_ERR_INVALID, f"{who}: {why}")
 
 
-def _paged_tensor(who: str, name: str, t, ndim: int, *dtypes):
-    """A tensor on the library's GPU of one of ``dtypes`` whose last dimension is contiguous."""
-    if not hasattr(t, "data_ptr") or not t.is_cuda:
+def _paged_tensor(who: str, name: str, t, ndim: int, dtype):
+    """-> (pointer, strides) of a tensor of ``dtype`` on the library's GPU whose last dimension is contiguous."""
+    try:
+        st = t.stride()
+        if t.dtype is dtype and t.get_device() == (rt._inited_device or 0) and len(st) == ndim and st[-1] == 1:
+            return t.data_ptr(), st
+    except AttributeError:
+        _refuse(who, f"{name} must be a tensor on the GPU")
+    if not t.is_cuda:
         _refuse(who, f"{name} must be a tensor on the GPU")
     if t.get_device() != (rt._inited_device or 0):
         _refuse(who, f"{name} lies on GPU {t.get_device()}, the library runs on GPU {rt._inited_device or 0}")
-    if t.dtype not in dtypes:
-        _refuse(who, f"{name} is {t.dtype}, expected {' or '.join(str(d) for d in dtypes)}")
-    if t.dim() != ndim:
-        _refuse(who, f"{name} has {t.dim()} dimensions, expected {ndim}")
-    if t.stride(-1) != 1 and t.shape[-1] != 1:
+    if t.dtype != dtype:
+        _refuse(who, f"{name} is {t.dtype}, expected {dtype}")
+    if len(st) != ndim:
+        _refuse(who, f"{name} has {len(st)} dimensions, expected {ndim}")
+    if t.shape[-1] != 1:
         _refuse(who, f"{name}'s last dimension must be contiguous")
-    return t.data_ptr()
+    return t.data_ptr(), st
 
 
 def _paged_vector(who: str, name: str, t, n: int, dtype):
-    p = _paged_tensor(who, name, t, 1, dtype)
+    ptr = _paged_tensor(who, name, t, 1, dtype)[0]
     if t.shape[0] != n:
         _refuse(who, f"{name} holds {t.shape[0]} elements, expected {n}")
-    return p
+    return ptr
 
 
-def _paged_cache(who: str, k, v, k_scale, v_scale):
+def _paged_half(who: str, name: str, t, torch):
+    """The tt_dtype of a 16-bit float tensor."""
+    if t.dtype is torch.bfloat16:
+        return rt.TT_BF16
+    if t.dtype is not torch.float16:
+        _refuse(who, f"{name} is {t.dtype}, expected torch.bfloat16 or torch.float16")
+    return rt.TT_F16
+
+
+def _paged_cache(who: str, k, v, k_scale, v_scale, torch):
     """-> (the packed tt_paged_cache, its shape [pages, heads, page size, head dim])."""
-    import torch
-    ptrs = (_paged_tensor(who, "k_cache", k, 4, torch.float8_e4m3fn), _paged_tensor(who, "v_cache", v, 4, torch.float8_e4m3fn),
-            _paged_tensor(who, "k_scale", k_scale, 2, torch.uint8), _paged_tensor(who, "v_scale", v_scale, 2, torch.uint8))
-    shape = tuple(k.shape)
-    if tuple(v.shape) != shape or tuple(k_scale.shape) != shape[:2] or tuple(v_scale.shape) != shape[:2]:
-        _refuse(who, f"cache shapes {shape}, {tuple(v.shape)}, {tuple(k_scale.shape)}, {tuple(v_scale.shape)}: K and V have one "
+    e4m3, u8 = torch.float8_e4m3fn, torch.uint8
+    pk, sk = _paged_tensor(who, "k_cache", k, 4, e4m3)
+    pv, sv = _paged_tensor(who, "v_cache", v, 4, e4m3)
+    pks, sks = _paged_tensor(who, "k_scale", k_scale, 2, u8)
+    pvs, svs = _paged_tensor(who, "v_scale", v_scale, 2, u8)
+    shape = k.shape
+    if v.shape != shape or k_scale.shape != shape[:2] or v_scale.shape != shape[:2]:
+        _refuse(who, f"cache shapes {tuple(shape)}, {tuple(v.shape)}, {tuple(k_scale.shape)}, {tuple(v_scale.shape)}: K and V have one "
                      "shape [pages, heads, page size, head dim], their scales its first two dimensions")
-    sk, sv = k.stride(), v.stride()
-    return rt.pack_paged_cache(*ptrs, *sk[:3], *sv[:3], *k_scale.stride(), *v_scale.stride(), *shape), shape
+    return rt.pack_paged_cache(pk, pv, pks, pvs, *sk[:3], *sv[:3], *sks, *svs, *shape), shape
 
 
 def _paged_plan_launch(lib, page_size: int, args, grid, stream):
     import torch
     who, i32 = "paged_plan", torch.int32
     ctx_lens, new_lens, table, free_pages, free_start, lens, cu_new, slot_map, free_end = args
-    pt = _paged_tensor(who, "block_table", table, 2, i32)
+    pt, st = _paged_tensor(who, "block_table", table, 2, i32)
     B, width = table.shape
     rc = lib.tt_paged_plan(
         _paged_vector(who, "ctx_lens", ctx_lens, B, i32), _paged_vector(who, "new_lens", new_lens, B, i32), pt,
-        table.stride(0) if B > 1 else width, B, width, _paged_tensor(who, "free_pages", free_pages, 1, i32), free_pages.shape[0],
+        st[0] if B > 1 else width, B, width, _paged_tensor(who, "free_pages", free_pages, 1, i32)[0], free_pages.shape[0],
         None if free_start is None else _paged_vector(who, "free_start", free_start, 1, i32), page_size, slot_map.shape[0],
         _paged_vector(who, "lens", lens, B, i32), _paged_vector(who, "cu_new", cu_new, B + 1, i32),
-        _paged_tensor(who, "slot_map", slot_map, 1, i32), _paged_vector(who, "free_end", free_end, 1, i32), grid, stream)
+        _paged_tensor(who, "slot_map", slot_map, 1, i32)[0], _paged_vector(who, "free_end", free_end, 1, i32), grid, stream)
     if rc:
         rt.check(rc)
     return True
@@ -714,15 +730,17 @@ def _paged_plan_launch(lib, page_size: int, args, grid, stream):
 
 def _paged_write_launch(lib, args, grid, stream):
     import torch
-    who, half = "paged_write", (torch.bfloat16, torch.float16)
+    who = "paged_write"
     k, v, slot_map, k_cache, v_cache, k_scale, v_scale = args
-    cache, (_, H, _, D) = _paged_cache(who, k_cache, v_cache, k_scale, v_scale)
-    pk, pv = _paged_tensor(who, "k", k, 3, *half), _paged_tensor(who, "v", v, 3, *half)
-    T = k.shape[0]
-    if tuple(k.shape) != (T, H, D) or k.shape != v.shape or k.dtype != v.dtype:
-        _refuse(who, f"k is {k.dtype} {tuple(k.shape)}, v is {v.dtype} {tuple(v.shape)}; the cache takes [tokens, {H}, {D}] of one type")
-    rc = lib.tt_paged_write(pk, pv, rt.pack_strides2(*k.stride()[:2]), rt.pack_strides2(*v.stride()[:2]),
-                            _paged_vector(who, "slot_map", slot_map, T, torch.int32), T, cache, _torch_dtype_code(k), grid, stream)
+    cache, (_, H, _, D) = _paged_cache(who, k_cache, v_cache, k_scale, v_scale, torch)
+    code = _paged_half(who, "k", k, torch)
+    pk, sk = _paged_tensor(who, "k", k, 3, k.dtype)
+    pv, sv = _paged_tensor(who, "v", v, 3, k.dtype)
+    T, h, d = k.shape
+    if h != H or d != D or k.shape != v.shape:
+        _refuse(who, f"k is {tuple(k.shape)}, v is {tuple(v.shape)}; the cache takes [tokens, {H}, {D}]")
+    rc = lib.tt_paged_write(pk, pv, rt.pack_strides2(sk[0], sk[1]), rt.pack_strides2(sv[0], sv[1]),
+                            _paged_vector(who, "slot_map", slot_map, T, torch.int32), T, cache, code, grid, stream)
     if rc:
         rt.check(rc)
     return True
@@ -730,25 +748,28 @@ def _paged_write_launch(lib, args, grid, stream):
 
 def _paged_attn_launch(lib, causal: bool, args, grid, stream):
     import torch
-    who, half, i32 = "paged_attn", (torch.bfloat16, torch.float16), torch.int32
+    who, i32 = "paged_attn", torch.int32
     q, k_cache, v_cache, k_scale, v_scale, table, lens, cu_q, out, lse, workspace, sm_scale, max_q = args
-    cache, (_, H, _, D) = _paged_cache(who, k_cache, v_cache, k_scale, v_scale)
-    pq, po, pt = _paged_tensor(who, "q", q, 3, *half), _paged_tensor(who, "out", out, 3, q.dtype), _paged_tensor(who, "block_table", table, 2, i32)
-    T, Hq, _ = q.shape
-    if q.shape != out.shape or q.shape[2] != D or Hq == 0 or Hq % H:
+    cache, (_, H, _, D) = _paged_cache(who, k_cache, v_cache, k_scale, v_scale, torch)
+    code = _paged_half(who, "q", q, torch)
+    pq, sq = _paged_tensor(who, "q", q, 3, q.dtype)
+    po, so = _paged_tensor(who, "out", out, 3, q.dtype)
+    pt, st = _paged_tensor(who, "block_table", table, 2, i32)
+    T, Hq, d = q.shape
+    if q.shape != out.shape or d != D or Hq == 0 or Hq % H:
         _refuse(who, f"q {tuple(q.shape)}, out {tuple(out.shape)} over a cache of {H} heads of {D}: both are [tokens, a multiple of {H}, {D}]")
     B, width = table.shape
     pl = None
     if lse is not None:
-        pl = _paged_tensor(who, "lse", lse, 2, torch.float32)
-        if tuple(lse.shape) != (T, Hq) or not lse.is_contiguous():
+        pl, sl = _paged_tensor(who, "lse", lse, 2, torch.float32)
+        if lse.shape != q.shape[:2] or (sl[0] != Hq and T != 1):
             _refuse(who, f"lse must be a contiguous [{T}, {Hq}] tensor")
     pw, nw = None, 0
     if workspace is not None:
-        pw, nw = _paged_tensor(who, "workspace", workspace, 1, torch.uint8), workspace.shape[0]
-    rc = lib.tt_paged_attn(pq, rt.pack_strides2(*q.stride()[:2]), cache, pt, table.stride(0) if B > 1 else width, B, width,
+        pw, nw = _paged_tensor(who, "workspace", workspace, 1, torch.uint8)[0], workspace.shape[0]
+    rc = lib.tt_paged_attn(pq, rt.pack_strides2(sq[0], sq[1]), cache, pt, st[0] if B > 1 else width, B, width,
                            _paged_vector(who, "lens", lens, B, i32), _paged_vector(who, "cu_q", cu_q, B + 1, i32), T, Hq,
-                           max_q, sm_scale, causal, _torch_dtype_code(q), po, rt.pack_strides2(*out.stride()[:2]), pl, pw, nw, grid, stream)
+                           max_q, sm_scale, causal, code, po, rt.pack_strides2(so[0], so[1]), pl, pw, nw, grid, stream)
     if rc:
         rt.check(rc)
     return True
@@ -768,7 +789,7 @@ def _bind_paged(launch, names: tuple, constexprs: tuple):
         cur.keep.extend(a for a in args if hasattr(a, "data_ptr"))
         fixed = functools.partial(launch, lib, *(consts[c] for c in constexprs))
         fixed(args, grid, stream)
-        cur.direct = lambda args, g, stream: fixed(args, rt.Grid3(*(g + (1, 1, 1))[:3]), stream)
+        cur.direct = lambda args, g, stream: fixed(args, rt.Grid3(*g, *(1, 1, 1)[len(g):]), stream)
         return rt.RT_OK
 
     return bind

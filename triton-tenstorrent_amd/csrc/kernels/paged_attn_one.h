@@ -14,11 +14,12 @@
 // w 2^(121 - e).  So weights can be held in fp16 (11 bits where bf16 has 8) whatever the scales' range: fp16 flushes
 // below 2^-32 of the largest contribution.
 //
-// Split: the keys of all sequences, in units of 64 * NS, are dealt evenly to the workgroups of a grid that fills the chip
-// once, whatever the lengths: workgroup i takes units [i U / G, (i+1) U / G) and meets at most two (sequence, head)
-// pairs that it does not have whole, the first and the last.  Those leave partial results (fp32 sum, reference, sum of
-// probabilities) in the workspace and paged_attn_join adds them in order, so results do not change from run to run.
-// While a pair's four wavefronts are merged, the next pair's first loads are under way.
+// Split: a group of workgroups, one for each cache head, takes an even share of the keys of all sequences, in units of
+// 64 * NS keys, whatever the lengths.  (All heads of a page are read at about the same time, by neighbouring workgroups:
+// their codes lie side by side.)  A workgroup meets at most two sequences that it
+// does not have whole, the first and the last.  Those leave partial results (fp32 sum, reference, sum of probabilities)
+// in the workspace and paged_attn_join adds them in order, so results do not change from run to run.  While a sequence's
+// four wavefronts are merged, the next one's first loads are under way.
 #pragma once
 
 namespace one {
@@ -63,6 +64,8 @@ template <int UK> struct Walk {
     per = (a.b + 63) / 64;
     int32_t n = 0;
     own = {0, 0, 0};
+    base = total = 0;
+    if (a.whole) return;
     for (int b = min(lane * per, a.b); b < min(lane * per + per, a.b); ++b) {
       own = seq_of<UK>(a, b);
       n += own.units;
@@ -80,18 +83,18 @@ template <int UK> struct Walk {
     if (per != 1) return seq_of<UK>(a, b);
     return {__builtin_amdgcn_readlane(own.q0, b), __builtin_amdgcn_readlane(own.len, b), __builtin_amdgcn_readlane(own.units, b)};
   }
-  // the sequence that holds unit u of `heads` times the total, and the units before it
-  __device__ __forceinline__ int find(int64_t u, int heads, int64_t *before, Seq *sq) const {
-    const int l = 63 - __builtin_clzll(__ballot((int64_t)base * heads <= u));
+  // the sequence that holds unit u, and the units before it
+  __device__ __forceinline__ int find(int32_t u, int32_t *before, Seq *sq) const {
+    const int l = 63 - __builtin_clzll(__ballot(base <= u));
     int b = l * per;
-    *before = (int64_t)__builtin_amdgcn_readlane(base, l) * heads;
+    *before = __builtin_amdgcn_readlane(base, l);
     *sq = at(b);
-    step(u, heads, &b, before, sq);
+    step(u, &b, before, sq);
     return b;
   }
-  __device__ __forceinline__ void step(int64_t u, int heads, int *b, int64_t *before, Seq *sq) const {
-    while (*before + (int64_t)sq->units * heads <= u) { // (u is less than all units: ends before the sequences do)
-      *before += (int64_t)sq->units * heads;
+  __device__ __forceinline__ void step(int32_t u, int *b, int32_t *before, Seq *sq) const {
+    while (*before + sq->units <= u) { // (u is less than all units: ends before the sequences do)
+      *before += sq->units;
       *sq = at(++*b);
     }
   }
@@ -122,6 +125,12 @@ struct Hf {
   static __device__ __forceinline__ uint16_t out(float f) { return out_f16(f); }
 };
 
+// Codes are read once: non-temporal loads where a row is whole 128-byte lines (782 MB of cache, head dim 128: 140 -> 126 us;
+// head dim 64, whose lines two rows share: no gain).
+template <int D, typename T> __device__ __forceinline__ T stream(const T *p) {
+  if constexpr (D >= 128) return __builtin_nontemporal_load(p);
+  return *p;
+}
 __device__ __forceinline__ int64_t uniform64(int64_t v) {
   return (int64_t)(((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32) |
                    (uint32_t)__builtin_amdgcn_readfirstlane((int)v));
@@ -133,9 +142,9 @@ __device__ __forceinline__ int64_t lane64(int32_t lo, int32_t hi, int lane) {
 // Partial result p of the workspace: rows * D sums, then rows pairs (reference, sum).
 template <int D, int MT> constexpr int part_floats() { return 16 * MT * D + 32 * MT; }
 
-// A pair that is split and whose first units are workgroup i's: the i-th entry behind the partial results.  Its parts are
-// slot 2 i + slot of workgroup i and slot 2 j of workgroups j = i + 1 .. last.
-struct Split { int32_t row, head, last, slot; }; // row: packed row of q, -1 = none
+// A sequence that is split and whose first units are workgroup i's, for that workgroup's head: the i-th entry behind the
+// partial results.  Its parts are slot 2 i + slot of workgroup i, then slot 2 j of the `more` workgroups j = i + heads, ...
+struct Split { int32_t row, more, slot, unused; }; // row: packed row of q, -1 = none
 
 template <class E, int D, int MT>
 __device__ __forceinline__ void body(const PagedAttnArgs &a, float *lds) {
@@ -144,29 +153,42 @@ __device__ __forceinline__ void body(const PagedAttnArgs &a, float *lds) {
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c16 = lane & 15, g = lane >> 4;
   const Walk<UK> walk(a);
-  const int64_t U = (int64_t)walk.total * a.c.heads;
-  const int64_t G = min((int64_t)gridDim.x, U); // fewer units than workgroups: one each
   Split *split = (Split *)(a.part + 2 * (int64_t)gridDim.x * part_floats<D, MT>()) + blockIdx.x;
-  if (blockIdx.x >= G) {
-    if (a.part && tid == 0) split->row = -1;
-    return;
-  }
-  int64_t u = blockIdx.x * U / G;
-  const int64_t u_end = (blockIdx.x + 1) * U / G, u_first = u;
-  int64_t before;
+  const int hk = blockIdx.x % a.c.heads, group = blockIdx.x / a.c.heads;
+  int32_t u, u_end, before;
+  int32_t each = 1, extra = 0; // units of a group; the first `extra` groups have one more
   Seq sq;
-  int b = walk.find(u, a.c.heads, &before, &sq);
+  int b;
+  if (a.whole) { // one sequence each
+    b = group;
+    sq = seq_of<UK>(a, b);
+    if (sq.units == 0) return;
+    before = u = 0;
+    u_end = sq.units;
+  } else {
+    const int32_t groups = min((int32_t)(gridDim.x / a.c.heads), walk.total); // fewer units than groups: one each
+    if (group >= groups) {
+      if (a.part && tid == 0) split->row = -1;
+      return;
+    }
+    each = walk.total / groups;
+    extra = walk.total - each * groups;
+    u = group * each + min(group, extra);
+    u_end = u + each + (group < extra);
+    b = walk.find(u, &before, &sq);
+  }
+  const int32_t u_first = u;
   bool noted = false;
+  const uint8_t *kh = a.c.k + hk * a.c.k_head, *vh = a.c.v + hk * a.c.v_head;
 
   const uint32_t klane = (uint32_t)(c16 * a.c.k_tok + g * 16);
   uint32_t vlane[4];
 #pragma unroll
   for (int r = 0; r < 4; ++r) vlane[r] = (uint32_t)((g * 4 + r) * a.c.v_tok + c16 * VB);
 
-  // the pair at u: units c0 .. c0 + n of its sq.units
-  int hk, c0, n;
+  // the sequence at u: units c0 .. c0 + n of its sq.units
+  int c0, n;
   const int32_t *table;
-  const uint8_t *kh, *vh;
   typename E::frag qf[MT][2 * KL];
 
   // What lane (it % IB) * NS + s knows of subtile s of step it: where its rows lie, how many count, its scales.
@@ -194,7 +216,7 @@ __device__ __forceinline__ void body(const PagedAttnArgs &a, float *lds) {
     for (int s = 0; s < NS; ++s) {
       const uint8_t *kp = kh + lane64(ko_lo, ko_hi, (it % IB) * NS + s);
 #pragma unroll
-      for (int h = 0; h < KL; ++h) kr[s][h] = *(const u32x4 *)(kp + klane + h * 64);
+      for (int h = 0; h < KL; ++h) kr[s][h] = stream<D>((const u32x4 *)(kp + klane + h * 64));
     }
   };
   auto load_v = [&](int it) {
@@ -203,13 +225,13 @@ __device__ __forceinline__ void body(const PagedAttnArgs &a, float *lds) {
       const uint8_t *vp = vh + lane64(vo_lo, vo_hi, (it % IB) * NS + s);
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        if constexpr (VW == 1) vr[s][r][0] = *(const uint32_t *)(vp + vlane[r]);
+        if constexpr (VW == 1) vr[s][r][0] = stream<D>((const uint32_t *)(vp + vlane[r]));
         if constexpr (VW == 2) {
-          const u32x2 x = *(const u32x2 *)(vp + vlane[r]);
+          const u32x2 x = stream<D>((const u32x2 *)(vp + vlane[r]));
           vr[s][r][0] = x[0]; vr[s][r][1] = x[1];
         }
         if constexpr (VW == 4) {
-          const u32x4 x = *(const u32x4 *)(vp + vlane[r]);
+          const u32x4 x = stream<D>((const u32x4 *)(vp + vlane[r]));
           vr[s][r][0] = x[0]; vr[s][r][1] = x[1]; vr[s][r][2] = x[2]; vr[s][r][3] = x[3];
         }
       }
@@ -218,12 +240,9 @@ __device__ __forceinline__ void body(const PagedAttnArgs &a, float *lds) {
 
   // one set of registers each for K and V: a step's loads go out as soon as the step before has used them up
   auto open = [&]() {
-    hk = (int)((u - before) / sq.units);
-    c0 = (int)(u - before - (int64_t)hk * sq.units);
-    n = (int)min((int64_t)(sq.units - c0), u_end - u);
+    c0 = u - before;
+    n = min(sq.units - c0, u_end - u);
     table = a.table + (int64_t)b * a.table_stride;
-    kh = a.c.k + hk * a.c.k_head;
-    vh = a.c.v + hk * a.c.v_head;
     batch(0);
     load_k(0);
     load_v(0);
@@ -364,21 +383,21 @@ __device__ __forceinline__ void body(const PagedAttnArgs &a, float *lds) {
       if (it + 1 < n) load_v(it + 1);
     }
 
-    // ---- the next pair's loads, then the merge of the four wavefronts ----
+    // ---- the next sequence's loads, then the merge of the four wavefronts ----
     const int32_t t = sq.q0;
-    const int my_hk = hk;
     const bool whole = n == sq.units;
-    // (the first pair of this workgroup takes slot 0, a later one that is not whole can only be its last: slot 1)
+    // (the first sequence of this workgroup takes slot 0, a later one that is not whole can only be its last: slot 1)
     const int which = u == u_first ? 0 : 1;
     if (!whole && c0 == 0) {
-      const int64_t last = before + (int64_t)(hk + 1) * sq.units - 1; // the pair's last unit
-      if (tid == 0) *split = {t, hk, (int32_t)(((last + 1) * G + U - 1) / U - 1), which};
+      const int32_t last = before + sq.units - 1, larger = extra * (each + 1); // its last unit, and the group that has that
+      const int32_t owner = last < larger ? last / (each + 1) : extra + (last - larger) / each;
+      if (tid == 0) *split = {t, owner - group, which, 0};
       noted = true;
     }
     u += n;
     const bool more = u < u_end;
     if (more) {
-      walk.step(u, a.c.heads, &b, &before, &sq);
+      walk.step(u, &b, &before, &sq);
       open();
     }
     float *wo = lds, *wml = lds + 4 * 16 * MT * LD;   // sums [wave][row][LD], (reference, sum) [wave][row]
@@ -417,7 +436,7 @@ __device__ __forceinline__ void body(const PagedAttnArgs &a, float *lds) {
       }
       if (whole) {
         if (row < a.group) {
-          const int hq = my_hk * a.group + row;
+          const int hq = hk * a.group + row;
           const bool none = l == 0.0f && mx == -kInf;
           const float inv = none ? 0.0f : kOut / l;
           uint16_t *op = a.o + t * a.o_tok + hq * a.o_head + d0;
@@ -442,7 +461,7 @@ __device__ __forceinline__ void body(const PagedAttnArgs &a, float *lds) {
   if (a.part && !noted && tid == 0) split->row = -1;
 }
 
-// Adds the parts of the split pair that workgroup blockIdx.x of the launch before noted, if any.  D / 4 threads a row; what
+// Adds the parts of the split sequence that workgroup blockIdx.x of the launch before noted, if any.  D / 4 threads a row; what
 // is left of the 256 takes several rows or several parts at once.
 template <class E, int D, int MT> __device__ __forceinline__ void join(const PagedAttnArgs &a, f32x4 *lds) {
   constexpr int TPR = D / 4, SLOTS = 256 / TPR, PF = part_floats<D, MT>();
@@ -452,7 +471,7 @@ template <class E, int D, int MT> __device__ __forceinline__ void join(const Pag
   int across = 1; // rows at once
   while (across < SLOTS && across < a.group) across <<= 1;
   const int deep = SLOTS / across, r0 = at % across, p0 = at / across;
-  const int parts = sp.last - (int)blockIdx.x + 1;
+  const int parts = sp.more + 1, head = blockIdx.x % a.c.heads;
   const float *first = a.part + (2 * (int64_t)blockIdx.x + sp.slot) * PF, *later = a.part + 2 * (int64_t)blockIdx.x * PF;
   float *lm = (float *)(lds + 256), *ll = lm + 256;
   for (int rb = 0; rb < a.group; rb += across) {
@@ -465,7 +484,7 @@ template <class E, int D, int MT> __device__ __forceinline__ void join(const Pag
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int j = min(p + i * deep, parts - 1);
-        const float *x = j ? later + 2 * (int64_t)j * PF : first;
+        const float *x = j ? later + 2 * (int64_t)j * a.c.heads * PF : first;
         pm[i] = x[16 * MT * D + row * 2];
         pl[i] = x[16 * MT * D + row * 2 + 1];
         po[i] = *(const f32x4 *)(x + row * D + d4 * 4);
@@ -498,7 +517,7 @@ template <class E, int D, int MT> __device__ __forceinline__ void join(const Pag
       __syncthreads();
     }
     if (p0 == 0 && rb + r0 < a.group) {
-      const int hq = sp.head * a.group + row;
+      const int hq = head * a.group + row;
       const bool none = l == 0.0f && m == -kInf;
       const float inv = none ? 0.0f : kOut / l;
       *(u32x2 *)(a.o + sp.row * a.o_tok + hq * a.o_head + d4 * 4) =

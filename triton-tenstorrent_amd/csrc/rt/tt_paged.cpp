@@ -42,7 +42,7 @@ struct Route {
   bool fast = false;
   // single tokens: paged_attn_one_*, its 16-row tiles of query heads, its workgroups, and whether sequences may be
   // split (partial results, joined by a second launch)
-  bool one = false, one_join = false;
+  bool one = false, one_whole = false, one_join = false;
   int one_tiles = 1;
   uint32_t one_groups = 0;
   // several queries: paged_attn_rows_*, its bound of 128-row tiles and the parts of a tile's keys
@@ -65,8 +65,18 @@ Route route_of(const PagedCacheArgs &c, int32_t B, int32_t max_pages, int32_t to
     r.one_tiles = group > 16 ? 2 : 1;
     const int64_t unit = D * r.one_tiles >= 128 ? 128 : 256;
     const int64_t most = std::max<int64_t>(cdiv64(keys, unit), 1);
-    r.one_groups = (uint32_t)std::min<int64_t>(most * c.heads * std::min(B, tokens), (D * r.one_tiles > 128 ? 2 : 3) * cus);
-    r.one_join = most > 1 && r.one_groups > 1;
+    // a workgroup for each head of a group; the groups fill the chip once (two or three workgroups a CU) or have a unit each
+    const int64_t slots = std::max((D * r.one_tiles > 128 ? 2 : 3) * cus / c.heads, 1);
+    r.one_groups = (uint32_t)(std::min<int64_t>(most * std::min(B, tokens), slots) * c.heads);
+    // A workgroup for each (sequence, head) instead, without parts to join, where the table allows no long sequence: up to
+    // 8 units take less than the second launch costs (8 heads of 512 keys: 7.4 us against 11.5; 2048 keys: 20), up to 16
+    // where there are pairs enough to keep the chip busy (512 pairs of 2048 keys: 44.6 us against 56).
+    const int64_t pairs = (int64_t)B * c.heads;
+    if (most <= (pairs >= slots * c.heads / 2 ? 16 : 8) && pairs <= INT32_MAX) {
+      r.one_whole = true;
+      r.one_groups = (uint32_t)pairs;
+    }
+    r.one_join = !r.one_whole && most > 1 && r.one_groups > (uint32_t)c.heads;
     if (r.one_join) r.one_bytes = (size_t)r.one_groups * (2 * (16 * r.one_tiles * D + 32 * r.one_tiles) * sizeof(float) + 16);
   }
   r.workspace = r.one_bytes;
@@ -211,6 +221,7 @@ extern "C" int tt_paged_attn(const void *q, const int64_t q_strides[2], const tt
     a.splits = r.splits;
     a.rows_min = r.one ? 2 : 1;
     if (r.one) {
+      a.whole = r.one_whole;
       a.part = r.one_join ? (float *)workspace : nullptr;
       snprintf(name, sizeof(name), "paged_attn_one_%s_d%d_r%d", type, c.head_dim, r.one_tiles);
       if ((rc = launch("paged", name, dim3(r.one_groups), dim3(256), 0, stream, args, 1))) return rc;

@@ -406,8 +406,8 @@ def paged_plan(ctx_lens: torch.Tensor, new_lens: torch.Tensor, block_table: torc
     ``new_lens``; with a larger one the surplus slots are -1, so that a captured step serves batches of several sizes.
     ``free_end`` is where the next step's ``free_start`` begins; past ``len(free_pages)`` it says that pages ran out."""
     B = block_table.shape[0]
-    i32 = dict(dtype=torch.int32, device=block_table.device)
-    plan = PagedPlan(torch.empty(B, **i32), torch.empty(B + 1, **i32), torch.empty(max_tokens, **i32), torch.empty(1, **i32))
+    made = torch.empty(2 * B + 2 + max_tokens, dtype=torch.int32, device=block_table.device)
+    plan = PagedPlan(*made.split_with_sizes((B, B + 1, max_tokens, 1)))     # one allocation
     paged_plan_kernel[(B, )](ctx_lens, new_lens, block_table, free_pages, free_start, *plan, PAGE_SIZE=page_size)
     return plan
 
@@ -442,13 +442,13 @@ def paged_attention(q: torch.Tensor, cache: PagedCache, block_table: torch.Tenso
     number of rows); 1 for a decode step takes the kernel for single tokens.  A query without a key gives 0 (lse -inf);
     rows outside every sequence are left as they are in ``out``.  Returns ``out``, or (``out``, lse [tokens, heads_q] in
     base 2) with ``return_lse``."""
-    out = torch.empty(q.shape, dtype=q.dtype, device=q.device) if out is None else out
-    tokens, heads_q = q.shape[0], q.shape[1]
+    out = torch.empty_like(q) if out is None else out
+    tokens, heads_q = q.shape[:2]
     lse = torch.empty((tokens, heads_q), dtype=torch.float32, device=q.device) if return_lse else None
     B, max_pages = block_table.shape
     if tokens and B:
         max_q = tokens if max_q is None else max_q
-        need = _paged_attn_workspace(q.get_device(), B, max_pages, tokens, heads_q, max_q, tuple(cache.k.shape)) if q.is_cuda else 0
+        need = _paged_attn_workspace(q.get_device(), B, max_pages, tokens, heads_q, max_q, cache.k.shape) if q.is_cuda else 0
         workspace = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
         paged_attn_kernel[(tokens, heads_q)](q, *cache, block_table, lens, cu_q, out, lse, workspace, float(sm_scale), max_q,
                                              CAUSAL=bool(causal))
