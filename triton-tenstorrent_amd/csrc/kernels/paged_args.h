@@ -42,7 +42,6 @@ struct PagedAttnArgs {
   uint64_t page_magic;  // ceil(2^36 / (page_size / 16)): n / (page_size / 16) = (n * page_magic) >> 36 for n < 2^27,
                         // page_size <= 8192
   float *part;          // partial results of split sequences
-  int32_t whole;        // single-token launch: a workgroup for each (sequence, head) instead of an even share of the keys
-  int32_t splits;       // parts of a row tile's keys (launch for several queries)
-  int32_t rows_min;     // sequences of fewer queries are not that launch's: 1, or 2 beside a single-token launch
+  int32_t whole;        // a workgroup for each (sequence or row tile, head) instead of an even share of the keys
+  int32_t rows_min;     // launch for several queries: sequences of fewer are not its; 1, or 2 beside a single-token launch
 };

@@ -11,7 +11,9 @@
 // holds two tiles; one barrier a tile.
 // Bound: MFMA and the exponentials (32 v_exp_f32 a lane and tile against 32 MFMAs of 32 cycles), LDS reads behind them.
 //
-// Where the rows are too few to fill the chip the keys are split `splits` ways and paged_attn_rows_join adds the parts.
+// Split: with row tiles enough to fill the chip twice, a workgroup takes one, late rows (which attend most keys) first.
+// With fewer, a group of workgroups, one for each cache head, takes an even share of the steps of all row tiles, and
+// paged_attn_rows_join adds the parts of those that were cut, as in paged_attn_one.h.
 #pragma once
 
 namespace rows {
@@ -37,49 +39,11 @@ struct Hf : one::Hf {
 
 constexpr int kRows = 128;
 
-struct Seq { int32_t q0, n, len, units; }; // first packed row, queries, keys, tiles of 128 rows
+struct Seq { int32_t q0, n, len, tiles; }; // first packed row, queries, keys, tiles of 128 rows
 __device__ __forceinline__ Seq seq_of(const PagedAttnArgs &a, int b) {
   const int32_t q0 = clampi(a.cu_q[b], 0, a.tokens), q1 = clampi(a.cu_q[b + 1], q0, a.tokens);
   const int32_t n = q1 - q0 >= a.rows_min ? q1 - q0 : 0;
   return {q0, n, clampi(a.lens[b], 0, a.max_pages * a.c.page_size), (int32_t)(((int64_t)n * a.group + kRows - 1) / kRows)};
-}
-
-__device__ __forceinline__ int scan_units(const PagedAttnArgs &a, int32_t *base, int32_t *part) {
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, per = (a.b + 255) / 256;
-  int32_t n = 0;
-  for (int b = min(tid * per, a.b); b < min(tid * per + per, a.b); ++b) n += seq_of(a, b).units;
-  int32_t v = n;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const int32_t o = __shfl_up(v, d);
-    if (lane >= d) v += o;
-  }
-  if (lane == 63) part[wave] = v;
-  __syncthreads();
-  for (int w = 0; w < wave; ++w) v += part[w];
-  base[tid] = v - n;
-  const int total = part[0] + part[1] + part[2] + part[3];
-  __syncthreads();
-  return total;
-}
-
-// The sequence that holds row tile u, and the tile's number in it.
-struct Item { int b, tile; Seq sq; };
-__device__ __forceinline__ Item item_of(const PagedAttnArgs &a, const int32_t *base, int u) {
-  const int per = (a.b + 255) / 256;
-  int lo = 0, hi = 255;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (base[mid] <= u) lo = mid; else hi = mid - 1;
-  }
-  int b = __builtin_amdgcn_readfirstlane(min(lo * per, a.b - 1));
-  int before = __builtin_amdgcn_readfirstlane(base[lo]);
-  Seq sq = seq_of(a, b);
-  while (before + sq.units <= u) {
-    before += sq.units;
-    sq = seq_of(a, ++b);
-  }
-  return {b, u - before, sq};
 }
 
 // Last key that query i of the sequence attends (-1: none).
@@ -87,11 +51,91 @@ __device__ __forceinline__ int32_t last_key(const PagedAttnArgs &a, const Seq &s
   return a.causal ? max(sq.len - sq.n + i, -1) : sq.len - 1;
 }
 
-// A tile's steps of 64 keys, and split s of them.
+// A tile's steps of 64 keys: one at least, so that rows without a key are written too.
 __device__ __forceinline__ int steps_of(const PagedAttnArgs &a, const Seq &sq, int tile) {
   const int32_t r1 = (int32_t)min((int64_t)(tile + 1) * kRows, (int64_t)sq.n * a.group) - 1;
-  return (last_key(a, sq, r1 / a.group) + 64) / 64;
+  return max((last_key(a, sq, r1 / a.group) + 64) / 64, 1);
 }
+
+__device__ __forceinline__ int32_t scan64(int32_t v) { // inclusive, over the wavefront
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int32_t o = __shfl_up(v, d);
+    if (lane >= d) v += o;
+  }
+  return v;
+}
+
+// Where the units of all sequences lie: tiles (whole tiles a workgroup) or steps.  Every wavefront scans by itself, lane i
+// the sequences i * per and up.
+struct Walk {
+  const PagedAttnArgs &a;
+  int per;
+  int32_t base, total;
+  __device__ __forceinline__ int32_t units_of(const Seq &sq) const {
+    if (a.whole) return sq.tiles;
+    int32_t n = 0;
+    for (int i = 0; i < sq.tiles; ++i) n += steps_of(a, sq, i);
+    return n;
+  }
+  __device__ __forceinline__ Walk(const PagedAttnArgs &args) : a(args) {
+    const int lane = threadIdx.x & 63;
+    per = (a.b + 63) / 64;
+    int32_t n = 0;
+    bool large = false; // a sequence of many tiles, which all lanes count together
+    for (int b = min(lane * per, a.b); b < min(lane * per + per, a.b); ++b) {
+      const Seq sq = seq_of(a, b);
+      large = per == 1 && !a.whole && sq.tiles > 8;
+      if (!large) n += units_of(sq);
+    }
+    for (uint64_t todo = __ballot(large); todo; todo &= todo - 1) {
+      const int b = __builtin_ctzll(todo);
+      const Seq sq = seq_of(a, b);
+      int32_t m = 0;
+      for (int i = lane; i < sq.tiles; i += 64) m += steps_of(a, sq, i);
+#pragma unroll
+      for (int d = 32; d; d >>= 1) m += __shfl_xor(m, d);
+      if (lane == b) n = m;
+    }
+    const int32_t v = scan64(n);
+    base = v - n;
+    total = __builtin_amdgcn_readlane(v, 63);
+  }
+  // the sequence that holds unit u, with the units before it
+  __device__ __forceinline__ int find(int32_t u, int32_t *before, Seq *sq) const {
+    const int l = 63 - __builtin_clzll(__ballot(base <= u));
+    int b = l * per;
+    *before = __builtin_amdgcn_readlane(base, l);
+    *sq = seq_of(a, b);
+    while (per > 1) {
+      const int32_t n = units_of(*sq);
+      if (*before + n > u) break;
+      *before += n;
+      *sq = seq_of(a, ++b);
+    }
+    return b;
+  }
+  // the tile of sequence sq that holds its step `at`, and the steps before that tile
+  __device__ __forceinline__ int tile_of(const Seq &sq, int32_t at, int32_t *before) const {
+    const int lane = threadIdx.x & 63;
+    *before = 0;
+    for (int i0 = 0;; i0 += 64) {
+      const int32_t n = i0 + lane < sq.tiles ? steps_of(a, sq, i0 + lane) : 0, v = scan64(n);
+      const uint64_t past = __ballot(*before + v > at);
+      if (past) {
+        const int l = __builtin_ctzll(past);
+        *before += __builtin_amdgcn_readlane(v - n, l);
+        return i0 + l;
+      }
+      *before += __builtin_amdgcn_readlane(v, 63);
+    }
+  }
+};
+
+// A tile that is split and whose first steps are workgroup i's: the i-th entry behind the partial results, as in
+// paged_attn_one.h.
+struct Split { int32_t b, more, slot, tile; }; // b: sequence, -1 = none
 
 // Floats of one part: 128 rows of D sums, then (reference, sum) of each row.
 template <int D> constexpr int part_floats() { return kRows * D + 2 * kRows; }
@@ -107,20 +151,42 @@ __device__ __forceinline__ void body(const PagedAttnArgs &a, uint8_t *lds) {
   constexpr int KMASK = D == 64 ? 7 : 15, KSH = D == 64 ? 1 : 0; // chunk swizzle of K rows
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c32 = lane & 31, hi = lane >> 5;
-  int32_t *base = (int32_t *)lds, *part = base + 256;
-  const int total = scan_units(a, base, part);
+  const Walk walk(a);
+  const int heads = a.c.heads, hk = blockIdx.x % heads, group = blockIdx.x / heads;
+  Split *split = (Split *)(a.part + 2 * (int64_t)gridDim.x * part_floats<D>()) + blockIdx.x;
+  int32_t u, u_end, before;
+  int32_t each = 1, extra = 0; // steps of a group; the first `extra` groups have one more
+  if (a.whole) {
+    u = walk.total - 1 - group; // late rows, which attend most keys, first
+    if (u < 0) return;
+    u_end = u + 1;
+  } else {
+    const int32_t groups = min((int32_t)(gridDim.x / heads), walk.total);
+    if (group >= groups) {
+      if (tid == 0) split->b = -1;
+      return;
+    }
+    each = walk.total / groups;
+    extra = walk.total - each * groups;
+    u = group * each + min(group, extra);
+    u_end = u + each + (group < extra);
+  }
+  Seq sq;
+  int b = walk.find(u, &before, &sq), tile;
+  if (a.whole) {
+    tile = u - before;
+  } else {
+    int32_t inside;
+    tile = walk.tile_of(sq, u - before, &inside);
+    before += inside; // from here on: the units before the tile
+  }
+  const int32_t u_first = u;
+  bool noted = false;
 
-  const int heads = a.c.heads, splits = a.splits;
-  const int hk = blockIdx.x % heads, rest = blockIdx.x / heads, split = rest % splits;
-  const int u = total - 1 - rest / splits; // late rows, which attend most keys, first
-  if (u < 0) return;
-  const Item item = item_of(a, base, u);
-  __syncthreads(); // `base` shares its LDS with the tiles
-  const Seq sq = item.sq;
-  const int R = sq.n * a.group, row0 = item.tile * kRows;
-  const int nsteps = steps_of(a, sq, item.tile);
-  const int k_lo = (int)((int64_t)split * nsteps / splits), k_hi = (int)((int64_t)(split + 1) * nsteps / splits);
-  if (splits > 1 && k_lo >= k_hi && !(nsteps == 0 && split == 0)) return; // (an item without a key writes its zeros once)
+  for (;;) {
+  const int R = sq.n * a.group, row0 = tile * kRows;
+  const int nsteps = steps_of(a, sq, tile);
+  const int k_lo = a.whole ? 0 : u - before, k_hi = a.whole ? nsteps : min(nsteps, k_lo + (u_end - u));
 
   const int row = row0 + wave * 32 + c32;
   const int qi = min(row, R - 1) / a.group, qg = min(row, R - 1) % a.group;
@@ -143,7 +209,7 @@ __device__ __forceinline__ void body(const PagedAttnArgs &a, uint8_t *lds) {
   for (int i = 0; i < DT; ++i) acc[i] = (f32x16){0};
   float mref = -kInf, lsum = 0.0f;
 
-  const int32_t *table = a.table + (int64_t)item.b * a.table_stride;
+  const int32_t *table = a.table + (int64_t)b * a.table_stride;
   const uint8_t *kh = a.c.k + hk * a.c.k_head, *vh = a.c.v + hk * a.c.v_head;
   // staging: K row tid / 4 of the tile, KB codes from column (tid % 4) * KB; V keys 4 (tid / 16) .. + 3, VB codes from
   // column (tid % 16) * VB.  Both lie in the wavefront's 16 keys.
@@ -365,76 +431,102 @@ __device__ __forceinline__ void body(const PagedAttnArgs &a, uint8_t *lds) {
   }
 
   lsum += __shfl_xor(lsum, 32);
-  if (!alive || row >= R) return;
-  if (splits == 1) {
-    const bool none = lsum == 0.0f && mref == -kInf;
-    const float inv = none ? 0.0f : kOut / lsum;
-    uint16_t *op = a.o + t * a.o_tok + hq * a.o_head + hi * 4;
+  const bool cut = k_lo > 0 || k_hi < nsteps;
+  // (the first tile of this workgroup takes slot 0, a later one that is cut can only be its last: slot 1)
+  const int which = u == u_first ? 0 : 1;
+  if (alive && row < R) {
+    if (!cut) {
+      const bool none = lsum == 0.0f && mref == -kInf;
+      const float inv = none ? 0.0f : kOut / lsum;
+      uint16_t *op = a.o + t * a.o_tok + hq * a.o_head + hi * 4;
 #pragma unroll
-    for (int i = 0; i < DT; ++i)
+      for (int i = 0; i < DT; ++i)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        uint16_t x[4];
+        for (int r = 0; r < 4; ++r) {
+          uint16_t x[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) x[j] = E::out(acc[i][r * 4 + j] * inv);
-        *(u32x2 *)(op + i * 32 + r * 8) = (u32x2){(uint32_t)x[0] | (uint32_t)x[1] << 16, (uint32_t)x[2] | (uint32_t)x[3] << 16};
-      }
-    if (a.lse && hi == 0) a.lse[t * a.heads_q + hq] = none ? -kInf : mref - kLift + __builtin_log2f(lsum);
-  } else {
-    float *p = a.part + (((int64_t)u * heads + hk) * splits + split) * part_floats<D>();
-    const int lr = wave * 32 + c32;
+          for (int j = 0; j < 4; ++j) x[j] = E::out(acc[i][r * 4 + j] * inv);
+          *(u32x2 *)(op + i * 32 + r * 8) = (u32x2){(uint32_t)x[0] | (uint32_t)x[1] << 16, (uint32_t)x[2] | (uint32_t)x[3] << 16};
+        }
+      if (a.lse && hi == 0) a.lse[t * a.heads_q + hq] = none ? -kInf : mref - kLift + __builtin_log2f(lsum);
+    } else {
+      float *p = a.part + (2 * (int64_t)blockIdx.x + which) * part_floats<D>();
+      const int lr = wave * 32 + c32;
 #pragma unroll
-    for (int i = 0; i < DT; ++i)
+      for (int i = 0; i < DT; ++i)
 #pragma unroll
-      for (int r = 0; r < 4; ++r)
-        *(f32x4 *)(p + lr * D + i * 32 + r * 8 + hi * 4) = (f32x4){acc[i][r * 4], acc[i][r * 4 + 1], acc[i][r * 4 + 2], acc[i][r * 4 + 3]};
-    if (hi == 0) { p[kRows * D + lr * 2] = mref; p[kRows * D + lr * 2 + 1] = lsum; }
+        for (int r = 0; r < 4; ++r)
+          *(f32x4 *)(p + lr * D + i * 32 + r * 8 + hi * 4) = (f32x4){acc[i][r * 4], acc[i][r * 4 + 1], acc[i][r * 4 + 2], acc[i][r * 4 + 3]};
+      if (hi == 0) { p[kRows * D + lr * 2] = mref; p[kRows * D + lr * 2 + 1] = lsum; }
+    }
   }
+  if (a.whole) return;
+  if (cut && k_lo == 0) {
+    const int32_t last = before + nsteps - 1, larger = extra * (each + 1); // the tile's last step, and the group that has it
+    const int32_t owner = last < larger ? last / (each + 1) : extra + (last - larger) / each;
+    if (tid == 0) *split = {b, owner - group, which, tile};
+    noted = true;
+  }
+  u += k_hi - k_lo;
+  if (u >= u_end) break;
+  before += nsteps;
+  if (++tile == sq.tiles) {
+    tile = 0;
+    do sq = seq_of(a, ++b);
+    while (sq.tiles == 0); // (u is less than all units)
+  }
+  }
+  if (!noted && tid == 0) split->b = -1;
 }
 
-// Adds the parts of one row tile: grid (row tiles, heads).
-template <class E, int D> __device__ __forceinline__ void join(const PagedAttnArgs &a, int32_t *base) {
-  constexpr int VB = D / 16;
-  const int total = scan_units(a, base, base + 256), u = blockIdx.x, hk = blockIdx.y, tid = threadIdx.x, splits = a.splits;
-  if (u >= total) return;
-  const Item item = item_of(a, base, u);
-  const Seq sq = item.sq;
-  const int R = sq.n * a.group, row0 = item.tile * kRows, nsteps = steps_of(a, sq, item.tile);
-  auto has = [&](int s) { return (int64_t)(s + 1) * nsteps / splits > (int64_t)s * nsteps / splits || (nsteps == 0 && s == 0); };
-  const float *p0 = a.part + ((int64_t)u * a.c.heads + hk) * splits * part_floats<D>();
-  for (int lr = tid >> 4; lr < min(R - row0, kRows); lr += 16) {
-    const int d0 = (tid & 15) * VB;
-    float mx = -kInf;
-    for (int s = 0; s < splits; ++s) {
-      if (has(s)) mx = fmaxf(mx, p0[(int64_t)s * part_floats<D>() + kRows * D + lr * 2]);
+// Adds the parts of the split tile that workgroup blockIdx.x of the launch before noted, if any: grid (workgroups, 8),
+// 16 rows each.
+template <class E, int D> __device__ __forceinline__ void join(const PagedAttnArgs &a) {
+  constexpr int PF = part_floats<D>(), VB = D / 16;
+  const Split sp = ((const Split *)(a.part + 2 * (int64_t)gridDim.x * PF))[blockIdx.x];
+  if (sp.b < 0) return;
+  const Seq sq = seq_of(a, sp.b);
+  const int row0 = sp.tile * kRows, lr = blockIdx.y * 16 + (threadIdx.x >> 4), d0 = (threadIdx.x & 15) * VB;
+  if (row0 + lr >= sq.n * a.group) return;
+  const int heads = a.c.heads, parts = sp.more + 1;
+  const float *first = a.part + (2 * (int64_t)blockIdx.x + sp.slot) * PF, *later = a.part + 2 * (int64_t)blockIdx.x * PF;
+  float m = -kInf, l = 0.0f;
+  f32x4 o[VB / 4];
+#pragma unroll
+  for (int i = 0; i < VB / 4; ++i) o[i] = (f32x4){0, 0, 0, 0};
+  for (int p = 0; p < parts; p += 4) {
+    float pm[4], pl[4];
+    f32x4 po[4][VB / 4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int j = min(p + i, parts - 1);
+      const float *x = j ? later + 2 * (int64_t)j * heads * PF : first;
+      pm[i] = x[kRows * D + lr * 2];
+      pl[i] = x[kRows * D + lr * 2 + 1];
+#pragma unroll
+      for (int v = 0; v < VB / 4; ++v) po[i][v] = *(const f32x4 *)(x + lr * D + d0 + v * 4);
     }
-    const float mm = mx == -kInf ? 0.0f : mx;
-    float l = 0.0f, o[VB];
 #pragma unroll
-    for (int i = 0; i < VB; ++i) o[i] = 0.0f;
-    for (int s = 0; s < splits; ++s) {
-      if (!has(s)) continue;
-      const float *p = p0 + (int64_t)s * part_floats<D>();
-      const float m = p[kRows * D + lr * 2];
-      const float f = m == -kInf ? 1.0f : __builtin_amdgcn_exp2f(m - mm); // (a row of NaN scores has reference -inf)
-      l += p[kRows * D + lr * 2 + 1] * f;
+    for (int i = 0; i < 4; ++i) {
+      if (p + i >= parts) break;
+      const float mn = fmaxf(m, pm[i]), ref = mn == -kInf ? 0.0f : mn;
+      // (a row of NaN scores has reference -inf and a NaN sum: it has to stay)
+      const float f = m == -kInf ? 1.0f : __builtin_amdgcn_exp2f(m - ref), w = pm[i] == -kInf ? 1.0f : __builtin_amdgcn_exp2f(pm[i] - ref);
+      l = l * f + pl[i] * w;
 #pragma unroll
-      for (int j = 0; j < VB; j += 4) {
-        const f32x4 y = *(const f32x4 *)(p + lr * D + d0 + j);
-        o[j] += y[0] * f; o[j + 1] += y[1] * f; o[j + 2] += y[2] * f; o[j + 3] += y[3] * f;
-      }
+      for (int v = 0; v < VB / 4; ++v) o[v] = o[v] * f + po[i][v] * w;
+      m = mn;
     }
-    const int qi = (row0 + lr) / a.group, hq = hk * a.group + (row0 + lr) % a.group;
-    const int64_t t = sq.q0 + qi;
-    const bool none = l == 0.0f && mx == -kInf;
-    const float inv = none ? 0.0f : kOut / l;
-    uint16_t *op = a.o + t * a.o_tok + hq * a.o_head + d0;
-#pragma unroll
-    for (int i = 0; i < VB; i += 2)
-      *(uint32_t *)(op + i) = (uint32_t)E::out(o[i] * inv) |
-                              (uint32_t)E::out(o[i + 1] * inv) << 16;
-    if (a.lse && d0 == 0) a.lse[t * a.heads_q + hq] = none ? -kInf : mx - kLift + __builtin_log2f(l);
   }
+  const int qi = (row0 + lr) / a.group, hq = blockIdx.x % heads * a.group + (row0 + lr) % a.group;
+  const int64_t t = sq.q0 + qi;
+  const bool none = l == 0.0f && m == -kInf;
+  const float inv = none ? 0.0f : kOut / l;
+#pragma unroll
+  for (int v = 0; v < VB / 4; ++v)
+    *(u32x2 *)(a.o + t * a.o_tok + hq * a.o_head + d0 + v * 4) =
+        (u32x2){(uint32_t)E::out(o[v][0] * inv) | (uint32_t)E::out(o[v][1] * inv) << 16, (uint32_t)E::out(o[v][2] * inv) | (uint32_t)E::out(o[v][3] * inv) << 16};
+  if (a.lse && d0 == 0) a.lse[t * a.heads_q + hq] = none ? -kInf : m - kLift + __builtin_log2f(l);
 }
 
 } // namespace rows
@@ -445,8 +537,7 @@ template <class E, int D> __device__ __forceinline__ void join(const PagedAttnAr
     rows::body<rows::E, D>(a, lds);                                                                           \
   }                                                                                                           \
   extern "C" __global__ __launch_bounds__(256) void paged_attn_rows_join_##T##_d##D(PagedAttnArgs a) {         \
-    __shared__ int32_t base[264];                                                                             \
-    rows::join<rows::E, D>(a, base);                                                                          \
+    rows::join<rows::E, D>(a);                                                                                \
   }
 PAGED_ROWS(bf16, Bf, 64, 2)
 PAGED_ROWS(bf16, Bf, 128, 2)

@@ -45,9 +45,9 @@ struct Route {
   bool one = false, one_whole = false, one_join = false;
   int one_tiles = 1;
   uint32_t one_groups = 0;
-  // several queries: paged_attn_rows_*, its bound of 128-row tiles and the parts of a tile's keys
-  bool rows = false;
-  int32_t row_tiles = 0, splits = 1;
+  // several queries: paged_attn_rows_*, its workgroups, and whether each has a 128-row tile of its own
+  bool rows = false, rows_whole = false;
+  int64_t rows_groups = 0;
   size_t one_bytes = 0, workspace = 0;
 };
 Route route_of(const PagedCacheArgs &c, int32_t B, int32_t max_pages, int32_t tokens, int32_t heads_q, int32_t max_q) {
@@ -81,11 +81,10 @@ Route route_of(const PagedCacheArgs &c, int32_t B, int32_t max_pages, int32_t to
   }
   r.workspace = r.one_bytes;
   if (r.rows) {
-    r.row_tiles = (int32_t)((int64_t)tokens * group / 128 + std::min(B, tokens));
-    // two workgroups a CU (one at head dim 256); a part has 256 keys at least
-    const int64_t items = (int64_t)r.row_tiles * c.heads, want = cdiv64((D == 256 ? 1 : 2) * cus, items);
-    r.splits = (int32_t)std::max<int64_t>(std::min(want, cdiv64(keys, 256)), 1);
-    if (r.splits > 1) r.workspace += (size_t)items * r.splits * (128 * D + 256) * sizeof(float);
+    const int64_t items = ((int64_t)tokens * group / 128 + std::min(B, tokens)) * c.heads, slots = (D == 256 ? 1 : 2) * cus;
+    r.rows_whole = items >= 2 * slots || keys <= 64;
+    r.rows_groups = r.rows_whole ? items : std::max<int64_t>(slots / c.heads, 1) * c.heads;
+    if (!r.rows_whole) r.workspace += (size_t)r.rows_groups * (2 * (128 * D + 256) * sizeof(float) + 16);
   }
   return r;
 }
@@ -218,7 +217,6 @@ extern "C" int tt_paged_attn(const void *q, const int64_t q_strides[2], const tt
   if (r.fast && al) {
     const uint64_t per = (uint64_t)c.page_size / 16;
     a.page_magic = ((1ull << 36) + per - 1) / per;
-    a.splits = r.splits;
     a.rows_min = r.one ? 2 : 1;
     if (r.one) {
       a.whole = r.one_whole;
@@ -233,12 +231,12 @@ extern "C" int tt_paged_attn(const void *q, const int64_t q_strides[2], const tt
     if (r.rows) {
       a.part = (float *)((char *)workspace + r.one_bytes);
       snprintf(name, sizeof(name), "paged_attn_rows_%s_d%d", type, c.head_dim);
-      const int64_t wgs = (int64_t)r.row_tiles * c.heads * r.splits;
-      if (wgs > INT32_MAX) return fail(RT_ERR_UNSUPPORTED, "%s: tokens * heads exceeds the grid", who);
-      if ((rc = launch("paged", name, dim3((uint32_t)wgs), dim3(256), 0, stream, args, 1))) return rc;
-      if (r.splits > 1) {
+      if (r.rows_groups > INT32_MAX) return fail(RT_ERR_UNSUPPORTED, "%s: tokens * heads exceeds the grid", who);
+      a.whole = r.rows_whole;
+      if ((rc = launch("paged", name, dim3((uint32_t)r.rows_groups), dim3(256), 0, stream, args, 1))) return rc;
+      if (!r.rows_whole) {
         snprintf(name, sizeof(name), "paged_attn_rows_join_%s_d%d", type, c.head_dim);
-        if ((rc = launch("paged", name, dim3((uint32_t)r.row_tiles, (uint32_t)c.heads), dim3(256), 0, stream, args, 1))) return rc;
+        if ((rc = launch("paged", name, dim3((uint32_t)r.rows_groups, 8), dim3(256), 0, stream, args, 1))) return rc;
       }
     }
     return RT_OK;
