@@ -140,8 +140,11 @@ struct Split { int32_t b, more, slot, tile; }; // b: sequence, -1 = none
 // Floats of one part: 128 rows of D sums, then (reference, sum) of each row.
 template <int D> constexpr int part_floats() { return kRows * D + 2 * kRows; }
 
-// K tile, V^T tile, flags (32 bytes), and where V holds NaN: a bit for each code, 16 bits for each (key, staging thread)
-template <int D> constexpr int stage_bytes() { return (64 * D * 2 * 2 + 32 + 64 * 16 * 2 + 511) / 512 * 512; }
+// K tile, V^T tile; of each 16-key subtile the score factor, the score offset and what brings weights back to probabilities
+// (4 floats each), whether a key of it counts, whether its V holds NaN (4 words each); and where V holds NaN, a bit for
+// each code, 16 bits for each (key, staging thread)
+constexpr int kMeta = 80;
+template <int D> constexpr int stage_bytes() { return (64 * D * 2 * 2 + kMeta + 64 * 16 * 2 + 511) / 512 * 512; }
 template <int D> constexpr int lds_bytes() { return 2 * stage_bytes<D>(); }
 
 template <class E, int D>
@@ -202,7 +205,8 @@ __device__ __forceinline__ void body(const PagedAttnArgs &a, uint8_t *lds) {
   {
     const uint16_t *qr = a.q + t * a.q_tok + hq * a.q_head + hi * 8;
 #pragma unroll
-    for (int s = 0; s < DK; ++s) qf[s] = __builtin_bit_cast(typename E::frag, *(const u32x4 *)(qr + s * 16));
+    for (int s = 0; s < DK; ++s) // (a negative scale's sign goes into q: factors of scores are positive below)
+      qf[s] = __builtin_bit_cast(typename E::frag, *(const u32x4 *)(qr + s * 16) ^ (a.qk_scale < 0.0f ? 0x80008000u : 0u));
   }
   f32x16 acc[DT];
 #pragma unroll
@@ -232,22 +236,17 @@ __device__ __forceinline__ void body(const PagedAttnArgs &a, uint8_t *lds) {
     const int64_t ko = page * a.c.k_page + prow * a.c.k_tok, vo = page * a.c.v_page + prow * a.c.v_tok;
     ko_lo = (int32_t)ko; ko_hi = (int32_t)(ko >> 32); vo_lo = (int32_t)vo; vo_hi = (int32_t)(vo >> 32);
     live = ok ? (int32_t)min((int64_t)sq.len - key, (int64_t)16) : 0;
-    kscale = pow2_code(a.c.ks[page * a.c.ks_page + hk * a.c.ks_head]) * a.qk_scale;
+    kscale = pow2_code(a.c.ks[page * a.c.ks_page + hk * a.c.ks_head]) * fabsf(a.qk_scale);
     vcode = ok ? a.c.vs[page * a.c.vs_page + hk * a.c.vs_head] : 0;
   };
   u32x4 kr[KW];
   uint32_t vr[4][VW];
-  struct Meta { float ks[4]; int nv[4], vc[4]; };
-  Meta staged; // of the codes in kr and vr
+  int staged_at, staged_nv; // of the codes in kr and vr: the lane that knows the tile's first subtile, the wavefront's live keys
   auto load = [&](int k, int k_first) {
     const int at = ((k - k_first) & 15) * 4;
     if (((k - k_first) & 15) == 0) batch(k);
-#pragma unroll
-    for (int s = 0; s < 4; ++s) {
-      staged.ks[s] = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, kscale), at + s));
-      staged.nv[s] = __builtin_amdgcn_readlane(live, at + s);
-      staged.vc[s] = __builtin_amdgcn_readlane(vcode, at + s);
-    }
+    staged_at = at;
+    staged_nv = __builtin_amdgcn_readlane(live, at + wave);
     const uint8_t *kp = kh + one::lane64(ko_lo, ko_hi, at + wave), *vp = vh + one::lane64(vo_lo, vo_hi, at + wave);
 #pragma unroll
     for (int i = 0; i < KW; ++i) kr[i] = *(const u32x4 *)(kp + kvo + i * 16);
@@ -275,13 +274,21 @@ __device__ __forceinline__ void body(const PagedAttnArgs &a, uint8_t *lds) {
   // codes in registers -> tile in LDS.  `edge`: some row does not attend some of these keys, so a NaN in V must be told
   // from the others' results (found here, handled by the readers).
   auto store = [&](uint32_t buf, bool edge) {
+    // (the batch still is the one these codes came from: load() of a later tile comes after)
+    if (wave == 0 && (uint32_t)(lane - staged_at) < 4) {
+      float *m = (float *)(lds + buf + FOFF) + (lane - staged_at);
+      m[0] = fmaxf(kscale, 1e-37f); // (not 0: a masked score times it has to stay -inf)
+      m[4] = (float)(vcode - kBase);
+      m[8] = unweight(vcode);
+      ((int32_t *)m)[12] = live;
+    }
     const uint32_t kw = buf + k_wr, vw = buf + v_wr;
 #pragma unroll
     for (int i = 0; i < KW; ++i)
 #pragma unroll
       for (int h = 0; h < 2; ++h)
         *(u32x4 *)(lds + (kw ^ ((i * 2 + h) << 4))) = __builtin_bit_cast(u32x4, E::codes(kr[i][2 * h], kr[i][2 * h + 1]));
-    const int nv = wave == 0 ? staged.nv[0] : wave == 1 ? staged.nv[1] : wave == 2 ? staged.nv[2] : staged.nv[3];
+    const int nv = staged_nv;
     const int mm = (tid >> 4) & 3; // 4-key group of the 16
     if (nv < 16) {
 #pragma unroll
@@ -299,7 +306,7 @@ __device__ __forceinline__ void body(const PagedAttnArgs &a, uint8_t *lds) {
           any |= nan[r][w];
         }
       const bool found = __any(any != 0);
-      if (lane == 0) *(int32_t *)(lds + buf + FOFF + wave * 4) = found;
+      if (lane == 0) *(int32_t *)(lds + buf + FOFF + 64 + wave * 4) = found;
       if (found) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
@@ -310,7 +317,7 @@ __device__ __forceinline__ void body(const PagedAttnArgs &a, uint8_t *lds) {
             bits |= (((nan[r][w] >> 7) * 0x00204081u) >> 21 & 15u) << (w * 4);
             vr[r][w] &= ~((nan[r][w] >> 7) * 0xffu);
           }
-          ((uint16_t *)(lds + buf + FOFF + 32))[(wave * 16 + mm * 4 + r) * 16 + (tid & 15)] = (uint16_t)bits;
+          ((uint16_t *)(lds + buf + FOFF + kMeta))[(wave * 16 + mm * 4 + r) * 16 + (tid & 15)] = (uint16_t)bits;
         }
       }
     }
@@ -336,12 +343,10 @@ __device__ __forceinline__ void body(const PagedAttnArgs &a, uint8_t *lds) {
     load(k_lo, k_lo);
     store(0, edge_of(k_lo));
   }
-  Meta now = staged; // of the tile in LDS that is computed
   if (k_lo + 1 < k_hi) load(k_lo + 1, k_lo);
   __syncthreads();
   for (int k = k_lo; k < k_hi; ++k) {
     const uint32_t buf = ((k - k_lo) & 1) * stage_bytes<D>(), next = stage_bytes<D>() - buf;
-    Meta after = staged;
     if (k + 1 < k_hi) {
       store(next, edge_of(k + 1));
       if (k + 2 < k_hi) load(k + 2, k_lo);
@@ -350,23 +355,32 @@ __device__ __forceinline__ void body(const PagedAttnArgs &a, uint8_t *lds) {
     if (alive && k * 64 <= wave_last) {
       const uint32_t kb = buf + k_rd, vb = buf + v_rd;
       f32x16 st[2] = {(f32x16){0}, (f32x16){0}};
+      // The order is pinned: left alone, the scheduler reads each fragment right before its product and waits for it.
+      // Four reads are on their way at any time.
+      u32x4 x[4];
+      auto k_frag = [&](int i) { return *(const u32x4 *)(lds + (kb ^ ((i >> 1) << 5)) + (i & 1) * 32 * KROW); };
 #pragma unroll
-      for (int s = 0; s < DK; ++s)
+      for (int i = 0; i < 4; ++i) x[i] = k_frag(i);
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const u32x4 x = *(const u32x4 *)(lds + (kb ^ (s << 5)) + j * 32 * KROW);
-          st[j] = E::mfma32(__builtin_bit_cast(typename E::frag, x), qf[s], st[j]);
-        }
+      for (int i = 0; i < 2 * DK; ++i) {
+        __builtin_amdgcn_sched_barrier(0);
+        st[i & 1] = E::mfma32(__builtin_bit_cast(typename E::frag, x[i & 3]), qf[i >> 1], st[i & 1]);
+        if (i + 4 < 2 * DK) x[i & 3] = k_frag(i + 4);
+      }
       __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-      for (int j = 0; j < 2; ++j)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) st[j][r] = fmaf(st[j][r], now.ks[j * 2 + (r >> 3)], (float)(now.vc[j * 2 + (r >> 3)] - kBase));
+      const f32x4 factor = *(const f32x4 *)(lds + buf + FOFF), offset = *(const f32x4 *)(lds + buf + FOFF + 16);
+      const f32x4 back = *(const f32x4 *)(lds + buf + FOFF + 32);
       const bool edge = edge_of(k);
-      if (edge || !(now.nv[0] && now.nv[1] && now.nv[2] && now.nv[3])) {
+      bool whole_tile = !edge;
+      if (!edge) { // (also where every row attends every key a page may be missing)
+        const u32x4 nv = *(const u32x4 *)(lds + buf + FOFF + 48);
+        whole_tile = __builtin_amdgcn_readfirstlane(nv[0] & nv[1] & nv[2] & nv[3]) == 16;
+      }
+      if (!whole_tile) {
+        const u32x4 nv = *(const u32x4 *)(lds + buf + FOFF + 48);
 #pragma unroll
         for (int s = 0; s < 4; ++s) {
-          const int32_t rel = now.nv[s] ? limit - k * 64 - s * 16 - hi * 4 : -1; // (keys past the end are past the limit)
+          const int32_t rel = nv[s] ? limit - k * 64 - s * 16 - hi * 4 : -1; // (keys past the end are past the limit)
 #pragma unroll
           for (int r = 0; r < 8; ++r) {
             const float x = st[s >> 1][(s & 1) * 8 + r];
@@ -374,11 +388,15 @@ __device__ __forceinline__ void body(const PagedAttnArgs &a, uint8_t *lds) {
           }
         }
       }
+      // x = score * factor + offset, whose maximum is that of the scores
       float top = -kInf;
 #pragma unroll
-      for (int j = 0; j < 2; ++j)
+      for (int s = 0; s < 4; ++s) {
+        float m = st[s >> 1][(s & 1) * 8];
 #pragma unroll
-        for (int r = 0; r < 16; ++r) top = fmaxf(top, st[j][r]);
+        for (int r = 1; r < 8; ++r) m = fmaxf(m, st[s >> 1][(s & 1) * 8 + r]);
+        top = fmaxf(top, fmaf(m, factor[s], offset[s]));
+      }
       if (__any(top > mref + kLazy)) {
         const float mn = fmaxf(mref, fmaxf(top, __shfl_xor(top, 32)));
         const float al = mn == -kInf ? 1.0f : __builtin_amdgcn_exp2f(mref - mn);
@@ -390,31 +408,38 @@ __device__ __forceinline__ void body(const PagedAttnArgs &a, uint8_t *lds) {
           for (int r = 0; r < 16; ++r) acc[i][r] *= al;
       }
       const float ref = (mref == -kInf ? 0.0f : mref) - kLift;
+      // weights of a subtile between the products of the one before, V fragments four reads ahead
       f16x8 pf[4];
+      float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+      auto weights = [&](int s, int r0, int n) {
+        const float c = offset[s] - ref;
 #pragma unroll
-      for (int s = 0; s < 4; ++s) {
-        float sum = 0.0f;
-#pragma unroll
-        for (int r = 0; r < 8; ++r) {
-          const float w = __builtin_amdgcn_exp2f(st[s >> 1][(s & 1) * 8 + r] - ref);
-          sum += w;
+        for (int r = r0; r < r0 + n; ++r) {
+          const float w = __builtin_amdgcn_exp2f(fmaf(st[s >> 1][(s & 1) * 8 + r], factor[s], c));
+          sum[s] += w; // (the sum of probabilities has to be fp32's: the log-sum-exp is a result)
           pf[s][r] = (_Float16)w;
         }
-        lsum = fmaf(sum, unweight(now.vc[s]), lsum);
+      };
+      auto v_frag = [&](int i) { return *(const u32x4 *)(lds + (vb ^ (((i / DT) ^ (i % DT & 3)) << 5)) + i % DT * 32 * 128); };
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[i] = v_frag(i);
+      weights(0, 0, 8);
+#pragma unroll
+      for (int i = 0; i < 4 * DT; ++i) {
+        __builtin_amdgcn_sched_barrier(0);
+        acc[i % DT] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, x[i & 3]), pf[i / DT], acc[i % DT], 0, 0, 0);
+        if (i + 4 < 4 * DT) x[i & 3] = v_frag(i + 4);
+        if (i < 3 * DT) weights(i / DT + 1, i % DT * (8 / DT), 8 / DT);
       }
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int s = 0; s < 4; ++s)
-#pragma unroll
-        for (int i = 0; i < DT; ++i) {
-          const u32x4 x = *(const u32x4 *)(lds + (vb ^ ((s ^ (i & 3)) << 5)) + i * 32 * 128);
-          acc[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, x), pf[s], acc[i], 0, 0, 0);
-        }
+      for (int s = 0; s < 4; ++s) lsum = fmaf(sum[s], back[s], lsum);
       if (edge) { // NaN in V, taken out of the tile: it reaches the rows that attend its key
         for (int s = 0; s < 4; ++s) {
-          if (!__builtin_amdgcn_readfirstlane(*(const int32_t *)(lds + buf + FOFF + s * 4))) continue;
+          if (!__builtin_amdgcn_readfirstlane(*(const int32_t *)(lds + buf + FOFF + 64 + s * 4))) continue;
           for (int j = 0; j < 16; ++j) {
             if (k * 64 + s * 16 + j > limit) continue;
-            const uint16_t *bits = (const uint16_t *)(lds + buf + FOFF + 32) + (s * 16 + j) * 16;
+            const uint16_t *bits = (const uint16_t *)(lds + buf + FOFF + kMeta) + (s * 16 + j) * 16;
 #pragma unroll
             for (int i = 0; i < DT; ++i)
 #pragma unroll
@@ -426,7 +451,6 @@ __device__ __forceinline__ void body(const PagedAttnArgs &a, uint8_t *lds) {
         }
       }
     }
-    now = after;
     __syncthreads();
   }
 
