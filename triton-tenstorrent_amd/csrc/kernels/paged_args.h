@@ -43,5 +43,5 @@ struct PagedAttnArgs {
                         // page_size <= 8192
   float *part;          // partial results of split sequences
   int32_t whole;        // a workgroup for each (sequence or row tile, head) instead of an even share of the keys
-  int32_t rows_min;     // launch for several queries: sequences of fewer are not its; 1, or 2 beside a single-token launch
+  int32_t few_rows;     // launch for many rows: sequences of at most so many (queries times group) are not its
 };

@@ -1,10 +1,11 @@
-// Attention over the paged cache, one query of each sequence (decode).
+// Attention over the paged cache, few queries of a sequence: one (a decode step), or some (verification) as long as
+// they and their heads fit 16 MT rows.
 //
-// What bounds it: one pass over the cached codes, HBM.  A wavefront owns all query heads of one cache head (rows of an
-// MFMA tile; a group of fewer than 16 leaves rows empty, which costs nothing here) and streams keys from global memory
+// What bounds it: one pass over the cached codes, HBM.  A wavefront owns all queries and query heads of one cache head
+// (row r is query r / group, head r % group; empty rows of the MFMA tile cost nothing here) and streams keys from global memory
 // into registers, with no LDS between: every code is used once, by one wavefront.
-//   S^T[key, q] = K . Q^T       v_mfma_f32_16x16x32, A = 16 rows of K, B = Q; lane l ends with query l%16, keys (l/16)*4+r
-//   O^T[d, q]  += V^T . P^T     B = P^T is what the lane already holds; A = V^T, whose lane needs 8 keys of one d: it loads
+//   S^T[key, r] = K . Q^T       v_mfma_f32_16x16x32, A = 16 rows of K, B = Q; lane l ends with row l%16, keys (l/16)*4+r
+//   O^T[d, r]  += V^T . P^T     B = P^T is what the lane already holds; A = V^T, whose lane needs 8 keys of one d: it loads
 //                               D/16 consecutive codes of each of its keys and pairs neighbouring keys' bytes with
 //                               v_perm_b32, one for two conversions.  MFMA number i takes the lanes' i-th code, so its
 //                               row l%16 stands for d = (l%16) * D/16 + i.
@@ -43,18 +44,18 @@ constexpr float kInf = __builtin_inff();
 // and make finer units than four (513 keys, 8 heads: 7.2 us against 9.3); at head dim 64 two would be too few bytes in flight.
 template <int D, int MT> constexpr int subtiles() { return D * MT >= 128 ? 2 : 4; }
 
-// Sequence b as this kernel sees it: no units where it is not this kernel's (no query, or several).
-struct Seq { int32_t q0, len, units; };
-template <int UK> __device__ __forceinline__ Seq seq_of(const PagedAttnArgs &a, int b) {
-  const int32_t q0 = a.cu_q[b], q1 = a.cu_q[b + 1];
-  const int32_t len = clampi(a.lens[b], 0, a.max_pages * a.c.page_size);
-  const bool mine = q1 - q0 == 1 && q0 >= 0 && q0 < a.tokens;
-  return {q0, len, mine ? max((len + UK - 1) / UK, 1) : 0};
+// Sequence b as this kernel sees it: no units where it is not this kernel's (no query, or too many).
+struct Seq { int32_t q0, n, len, units; };
+template <int UK, int ROWS, bool FEW> __device__ __forceinline__ Seq seq_of(const PagedAttnArgs &a, int b) {
+  const int32_t q0 = clampi(a.cu_q[b], 0, a.tokens), q1 = clampi(a.cu_q[b + 1], q0, a.tokens);
+  const int32_t len = clampi(a.lens[b], 0, a.max_pages * a.c.page_size), n = q1 - q0;
+  const bool mine = FEW ? n > 0 && (int64_t)n * a.group <= ROWS : n == 1;
+  return {q0, n, len, mine ? max((len + UK - 1) / UK, 1) : 0};
 }
 
 // Where the units of all sequences lie: every wavefront scans the lengths by itself, lane i the sequences i * per and
 // up.  Up to 64 sequences stay in registers.
-template <int UK> struct Walk {
+template <int UK, int ROWS, bool FEW> struct Walk {
   const PagedAttnArgs &a;
   int per;
   int32_t base, total;
@@ -63,11 +64,11 @@ template <int UK> struct Walk {
     const int lane = threadIdx.x & 63;
     per = (a.b + 63) / 64;
     int32_t n = 0;
-    own = {0, 0, 0};
+    own = {0, 0, 0, 0};
     base = total = 0;
     if (a.whole) return;
     for (int b = min(lane * per, a.b); b < min(lane * per + per, a.b); ++b) {
-      own = seq_of<UK>(a, b);
+      own = seq_of<UK, ROWS, FEW>(a, b);
       n += own.units;
     }
     int32_t v = n;
@@ -80,8 +81,9 @@ template <int UK> struct Walk {
     total = __builtin_amdgcn_readlane(v, 63);
   }
   __device__ __forceinline__ Seq at(int b) const {
-    if (per != 1) return seq_of<UK>(a, b);
-    return {__builtin_amdgcn_readlane(own.q0, b), __builtin_amdgcn_readlane(own.len, b), __builtin_amdgcn_readlane(own.units, b)};
+    if (per != 1) return seq_of<UK, ROWS, FEW>(a, b);
+    return {__builtin_amdgcn_readlane(own.q0, b), __builtin_amdgcn_readlane(own.n, b), __builtin_amdgcn_readlane(own.len, b),
+            __builtin_amdgcn_readlane(own.units, b)};
   }
   // the sequence that holds unit u, and the units before it
   __device__ __forceinline__ int find(int32_t u, int32_t *before, Seq *sq) const {
@@ -144,15 +146,16 @@ template <int D, int MT> constexpr int part_floats() { return 16 * MT * D + 32 *
 
 // A sequence that is split and whose first units are workgroup i's, for that workgroup's head: the i-th entry behind the
 // partial results.  Its parts are slot 2 i + slot of workgroup i, then slot 2 j of the `more` workgroups j = i + heads, ...
-struct Split { int32_t row, more, slot, unused; }; // row: packed row of q, -1 = none
+struct Split { int32_t q0, more, slot, rows; }; // q0: first packed row of its queries, -1 = none; rows: queries times group
 
-template <class E, int D, int MT>
+// FEW: sequences may have several queries; without it exactly one, and nothing below looks at a row's own limit.
+template <class E, int D, int MT, bool FEW>
 __device__ __forceinline__ void body(const PagedAttnArgs &a, float *lds) {
   constexpr int NS = subtiles<D, MT>(), UK = 64 * NS, KL = D / 64, VW = D / 64; // 16-byte loads of K, dwords of V per row
   constexpr int VB = D / 16, IB = 64 / NS, LD = D + 4;                      // LD: padded LDS row of the merge
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c16 = lane & 15, g = lane >> 4;
-  const Walk<UK> walk(a);
+  const Walk<UK, 16 * MT, FEW> walk(a);
   Split *split = (Split *)(a.part + 2 * (int64_t)gridDim.x * part_floats<D, MT>()) + blockIdx.x;
   const int hk = blockIdx.x % a.c.heads, group = blockIdx.x / a.c.heads;
   int32_t u, u_end, before;
@@ -161,14 +164,14 @@ __device__ __forceinline__ void body(const PagedAttnArgs &a, float *lds) {
   int b;
   if (a.whole) { // one sequence each
     b = group;
-    sq = seq_of<UK>(a, b);
+    sq = seq_of<UK, 16 * MT, FEW>(a, b);
     if (sq.units == 0) return;
     before = u = 0;
     u_end = sq.units;
   } else {
     const int32_t groups = min((int32_t)(gridDim.x / a.c.heads), walk.total); // fewer units than groups: one each
     if (group >= groups) {
-      if (a.part && tid == 0) split->row = -1;
+      if (a.part && tid == 0) split->q0 = -1;
       return;
     }
     each = walk.total / groups;
@@ -188,6 +191,7 @@ __device__ __forceinline__ void body(const PagedAttnArgs &a, float *lds) {
 
   // the sequence at u: units c0 .. c0 + n of its sq.units
   int c0, n;
+  int32_t limit[MT]; // last key that the lane's row attends
   const int32_t *table;
   typename E::frag qf[MT][2 * KL];
 
@@ -248,12 +252,13 @@ __device__ __forceinline__ void body(const PagedAttnArgs &a, float *lds) {
     load_v(0);
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
-      const int row = m * 16 + c16;
-      const uint16_t *qr = a.q + sq.q0 * a.q_tok + (hk * a.group + row) * a.q_head + g * 16;
+      const int row = m * 16 + c16, i = FEW ? min(row / a.group, sq.n - 1) : 0;
+      limit[m] = a.causal ? sq.len - sq.n + i : sq.len - 1;
+      const uint16_t *qr = a.q + (sq.q0 + i) * a.q_tok + (hk * a.group + (FEW ? row % a.group : row)) * a.q_head + g * 16;
 #pragma unroll
       for (int s = 0; s < 2 * KL; ++s) {
         u32x4 z = {0, 0, 0, 0};
-        if (row < a.group) z = *(const u32x4 *)(qr + (s >> 1) * 64 + (s & 1) * 8);
+        if (row < (FEW ? sq.n * a.group : a.group)) z = *(const u32x4 *)(qr + (s >> 1) * 64 + (s & 1) * 8);
         qf[m][s] = __builtin_bit_cast(typename E::frag, z);
       }
     }
@@ -304,17 +309,27 @@ __device__ __forceinline__ void body(const PagedAttnArgs &a, float *lds) {
         if ((it + 1) % IB == 0) batch(it + 1);
         load_k(it + 1);
       }
-      if (nmin < 16) { // rows behind the end or on no page: their scores count for nothing, their V must not be NaN
+      // keys behind the end or on no page, and those that some row does not attend
+      const int32_t key0 = (c0 + it) * UK + wave * (16 * NS);
+      const bool edge = FEW && a.causal && key0 + 16 * NS - 1 > sq.len - sq.n;
+      bool nan = false;
+      if (nmin < 16 || edge) {
+        uint32_t any = 0;
 #pragma unroll
         for (int s = 0; s < NS; ++s)
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
             const bool in = g * 4 + r < nv[s];
 #pragma unroll
-            for (int m = 0; m < MT; ++m) st[m][s][r] = in ? st[m][s][r] : -kInf;
+            for (int m = 0; m < MT; ++m) st[m][s][r] = in && (!FEW || key0 + s * 16 + g * 4 + r <= limit[m]) ? st[m][s][r] : -kInf;
 #pragma unroll
-            for (int w = 0; w < VW; ++w) vr[s][r][w] = in ? vr[s][r][w] : 0;
+            for (int w = 0; w < VW; ++w) { // (what lies in dead rows may be NaN)
+              vr[s][r][w] = in ? vr[s][r][w] : 0;
+              if (FEW) any |= (vr[s][r][w] & 0x7f7f7f7fu) + 0x01010101u;
+            }
           }
+        // a NaN in V of a key that some row does not attend must not reach that row
+        nan = edge && sq.n > 1 && __any((any & 0x80808080u) != 0);
       }
       // the reference
       float top[MT];
@@ -374,24 +389,42 @@ __device__ __forceinline__ void body(const PagedAttnArgs &a, float *lds) {
           }
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const u32x4 x = {f[i][0], f[i][1], f[i][2], f[i][3]};
+            f16x8 x = __builtin_bit_cast(f16x8, (u32x4){f[i][0], f[i][1], f[i][2], f[i][3]});
+            if (FEW && __builtin_expect(nan, 0)) { // the sum runs without NaN, another product counts those that a row attends
+              f16x8 y;
+#pragma unroll
+              for (int j = 0; j < 8; ++j) {
+                y[j] = x[j] != x[j] ? (_Float16)1.0f : (_Float16)0.0f;
+                x[j] = x[j] != x[j] ? (_Float16)0.0f : x[j];
+              }
+#pragma unroll
+              for (int m = 0; m < MT; ++m) {
+                f16x8 sees;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) sees[j] = key0 + (2 * p + (j >> 2)) * 16 + g * 4 + (j & 3) <= limit[m] ? (_Float16)1.0f : (_Float16)0.0f;
+                const f32x4 bad = __builtin_amdgcn_mfma_f32_16x16x32_f16(y, sees, (f32x4){0, 0, 0, 0}, 0, 0, 0);
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                  if (bad[r] > 0.0f) acc[m][w * 4 + i][r] = __builtin_nanf("");
+              }
+            }
 #pragma unroll
             for (int m = 0; m < MT; ++m)
-              acc[m][w * 4 + i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, x), pf[m][p], acc[m][w * 4 + i], 0, 0, 0);
+              acc[m][w * 4 + i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, pf[m][p], acc[m][w * 4 + i], 0, 0, 0);
           }
         }
       if (it + 1 < n) load_v(it + 1);
     }
 
     // ---- the next sequence's loads, then the merge of the four wavefronts ----
-    const int32_t t = sq.q0;
+    const int32_t q0 = sq.q0, rows = FEW ? sq.n * a.group : a.group;
     const bool whole = n == sq.units;
     // (the first sequence of this workgroup takes slot 0, a later one that is not whole can only be its last: slot 1)
     const int which = u == u_first ? 0 : 1;
     if (!whole && c0 == 0) {
       const int32_t last = before + sq.units - 1, larger = extra * (each + 1); // its last unit, and the group that has that
       const int32_t owner = last < larger ? last / (each + 1) : extra + (last - larger) / each;
-      if (tid == 0) *split = {t, owner - group, which, 0};
+      if (tid == 0) *split = {q0, owner - group, which, rows};
       noted = true;
     }
     u += n;
@@ -435,8 +468,9 @@ __device__ __forceinline__ void body(const PagedAttnArgs &a, float *lds) {
         for (int i = 0; i < VB; ++i) o[i] += wo[(w * 16 * MT + row) * LD + d0 + i] * f;
       }
       if (whole) {
-        if (row < a.group) {
-          const int hq = hk * a.group + row;
+        if (row < rows) {
+          const int64_t t = q0 + (FEW ? row / a.group : 0);
+          const int hq = hk * a.group + (FEW ? row % a.group : row);
           const bool none = l == 0.0f && mx == -kInf;
           const float inv = none ? 0.0f : kOut / l;
           uint16_t *op = a.o + t * a.o_tok + hq * a.o_head + d0;
@@ -444,7 +478,7 @@ __device__ __forceinline__ void body(const PagedAttnArgs &a, float *lds) {
           for (int i = 0; i < VB; i += 2)
             *(uint32_t *)(op + i) = (uint32_t)E::out(o[i] * inv) |
                                     (uint32_t)E::out(o[i + 1] * inv) << 16;
-          if (a.lse && d0 == 0) a.lse[(int64_t)t * a.heads_q + hq] = none ? -kInf : mx - kLift + __builtin_log2f(l);
+          if (a.lse && d0 == 0) a.lse[t * a.heads_q + hq] = none ? -kInf : mx - kLift + __builtin_log2f(l);
         }
       } else {
 #pragma unroll
@@ -458,7 +492,7 @@ __device__ __forceinline__ void body(const PagedAttnArgs &a, float *lds) {
     if (!more) break;
     __syncthreads();
   }
-  if (a.part && !noted && tid == 0) split->row = -1;
+  if (a.part && !noted && tid == 0) split->q0 = -1;
 }
 
 // Adds the parts of the split sequence that workgroup blockIdx.x of the launch before noted, if any.  D / 4 threads a row; what
@@ -466,15 +500,15 @@ __device__ __forceinline__ void body(const PagedAttnArgs &a, float *lds) {
 template <class E, int D, int MT> __device__ __forceinline__ void join(const PagedAttnArgs &a, f32x4 *lds) {
   constexpr int TPR = D / 4, SLOTS = 256 / TPR, PF = part_floats<D, MT>();
   const Split sp = ((const Split *)(a.part + 2 * (int64_t)gridDim.x * PF))[blockIdx.x];
-  if (sp.row < 0) return;
+  if (sp.q0 < 0) return;
   const int tid = threadIdx.x, d4 = tid % TPR, at = tid / TPR;
   int across = 1; // rows at once
-  while (across < SLOTS && across < a.group) across <<= 1;
+  while (across < SLOTS && across < sp.rows) across <<= 1;
   const int deep = SLOTS / across, r0 = at % across, p0 = at / across;
   const int parts = sp.more + 1, head = blockIdx.x % a.c.heads;
   const float *first = a.part + (2 * (int64_t)blockIdx.x + sp.slot) * PF, *later = a.part + 2 * (int64_t)blockIdx.x * PF;
   float *lm = (float *)(lds + 256), *ll = lm + 256;
-  for (int rb = 0; rb < a.group; rb += across) {
+  for (int rb = 0; rb < sp.rows; rb += across) {
     const int row = min(rb + r0, 16 * MT - 1);
     float m = -kInf, l = 0.0f;
     f32x4 o = {0, 0, 0, 0};
@@ -516,13 +550,14 @@ template <class E, int D, int MT> __device__ __forceinline__ void join(const Pag
         }
       __syncthreads();
     }
-    if (p0 == 0 && rb + r0 < a.group) {
-      const int hq = head * a.group + row;
+    if (p0 == 0 && rb + r0 < sp.rows) {
+      const int64_t t = sp.q0 + row / a.group;
+      const int hq = head * a.group + row % a.group;
       const bool none = l == 0.0f && m == -kInf;
       const float inv = none ? 0.0f : kOut / l;
-      *(u32x2 *)(a.o + sp.row * a.o_tok + hq * a.o_head + d4 * 4) =
+      *(u32x2 *)(a.o + t * a.o_tok + hq * a.o_head + d4 * 4) =
           (u32x2){(uint32_t)E::out(o[0] * inv) | (uint32_t)E::out(o[1] * inv) << 16, (uint32_t)E::out(o[2] * inv) | (uint32_t)E::out(o[3] * inv) << 16};
-      if (a.lse && d4 == 0) a.lse[(int64_t)sp.row * a.heads_q + hq] = none ? -kInf : m - kLift + __builtin_log2f(l);
+      if (a.lse && d4 == 0) a.lse[t * a.heads_q + hq] = none ? -kInf : m - kLift + __builtin_log2f(l);
     }
   }
 }
@@ -534,13 +569,17 @@ template <int D, int MT> constexpr int lds_floats() { return 4 * 16 * MT * (D + 
 #define PAGED_ONE(T, E, D, MT, OCC)                                                                           \
   extern "C" __global__ __launch_bounds__(256, OCC) void paged_attn_one_##T##_d##D##_r##MT(PagedAttnArgs a) {  \
     __shared__ __align__(16) float lds[one::lds_floats<D, MT>()];                                             \
-    one::body<one::E, D, MT>(a, lds);                                                                         \
+    one::body<one::E, D, MT, false>(a, lds);                                                                  \
+  }                                                                                                           \
+  extern "C" __global__ __launch_bounds__(256, 2) void paged_attn_few_##T##_d##D##_r##MT(PagedAttnArgs a) {    \
+    __shared__ __align__(16) float lds[one::lds_floats<D, MT>()];                                             \
+    one::body<one::E, D, MT, true>(a, lds);                                                                   \
   }                                                                                                           \
   extern "C" __global__ __launch_bounds__(256) void paged_attn_join_##T##_d##D##_r##MT(PagedAttnArgs a) {      \
     __shared__ one::f32x4 lds[256 + 128];                                                                     \
     one::join<one::E, D, MT>(a, lds);                                                                         \
   }
-// (the last number: workgroups on a CU, which the host's grid counts on too)
+// (the last number: workgroups of paged_attn_one on a CU, which the host's grid counts on too; paged_attn_few has two)
 PAGED_ONE(bf16, Bf, 64, 1, 3)
 PAGED_ONE(bf16, Bf, 64, 2, 3)
 PAGED_ONE(bf16, Bf, 128, 1, 3)

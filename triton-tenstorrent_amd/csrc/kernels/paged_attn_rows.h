@@ -42,7 +42,7 @@ constexpr int kRows = 128;
 struct Seq { int32_t q0, n, len, tiles; }; // first packed row, queries, keys, tiles of 128 rows
 __device__ __forceinline__ Seq seq_of(const PagedAttnArgs &a, int b) {
   const int32_t q0 = clampi(a.cu_q[b], 0, a.tokens), q1 = clampi(a.cu_q[b + 1], q0, a.tokens);
-  const int32_t n = q1 - q0 >= a.rows_min ? q1 - q0 : 0;
+  const int32_t n = (int64_t)(q1 - q0) * a.group > a.few_rows ? q1 - q0 : 0; // fewer are the other kernel's
   return {q0, n, clampi(a.lens[b], 0, a.max_pages * a.c.page_size), (int32_t)(((int64_t)n * a.group + kRows - 1) / kRows)};
 }
 

@@ -40,12 +40,12 @@ int check_grid(const char *who, const uint32_t grid[3], int32_t x, int32_t y) {
 // How tt_paged_attn runs a call of these sizes.
 struct Route {
   bool fast = false;
-  // single tokens: paged_attn_one_*, its 16-row tiles of query heads, its workgroups, and whether sequences may be
+  // few queries of a sequence: paged_attn_one_* (exactly one) or paged_attn_few_*, its 16-row tiles of query heads, its workgroups, and whether sequences may be
   // split (partial results, joined by a second launch)
   bool one = false, one_whole = false, one_join = false;
   int one_tiles = 1;
   uint32_t one_groups = 0;
-  // several queries: paged_attn_rows_*, its workgroups, and whether each has a 128-row tile of its own
+  // many: paged_attn_rows_*, its workgroups, and whether each has a 128-row tile of its own
   bool rows = false, rows_whole = false;
   int64_t rows_groups = 0;
   size_t one_bytes = 0, workspace = 0;
@@ -57,16 +57,18 @@ Route route_of(const PagedCacheArgs &c, int32_t B, int32_t max_pages, int32_t to
   if ((int64_t)tokens * group > INT32_MAX - 256) return r;
   r.fast = true;
   const int64_t keys = (int64_t)max_pages * c.page_size;
-  // sequences of one query go to their own kernel where a head group's rows fit it, unless the call has one sequence
-  // of several
-  r.one = group <= (D == 256 ? 16 : 32) && (max_q == 1 || B > 1);
-  r.rows = !r.one || max_q > 1;
+  // Sequences of few queries go to their own kernel: queries times group up to 32 rows (16 at head dim 256), or 16 where
+  // none can have more.  It is left out where one sequence is all there is and may have more.
+  const int64_t rows = (int64_t)max_q * group;
+  const int few = D == 256 || rows <= 16 ? 16 : 32;
+  r.one = group <= few && (rows <= few || B > 1);
+  r.rows = !r.one || rows > few;
   if (r.one) {
-    r.one_tiles = group > 16 ? 2 : 1;
+    r.one_tiles = few / 16;
     const int64_t unit = D * r.one_tiles >= 128 ? 128 : 256;
     const int64_t most = std::max<int64_t>(cdiv64(keys, unit), 1);
     // a workgroup for each head of a group; the groups fill the chip once (two or three workgroups a CU) or have a unit each
-    const int64_t slots = std::max((D * r.one_tiles > 128 ? 2 : 3) * cus / c.heads, 1);
+    const int64_t slots = std::max((D * r.one_tiles > 128 || max_q > 1 ? 2 : 3) * cus / c.heads, 1);
     r.one_groups = (uint32_t)(std::min<int64_t>(most * std::min(B, tokens), slots) * c.heads);
     // A workgroup for each (sequence, head) instead, without parts to join, where the table allows no long sequence: up to
     // 8 units take less than the second launch costs (8 heads of 512 keys: 7.4 us against 11.5; 2048 keys: 20), up to 16
@@ -217,11 +219,11 @@ extern "C" int tt_paged_attn(const void *q, const int64_t q_strides[2], const tt
   if (r.fast && al) {
     const uint64_t per = (uint64_t)c.page_size / 16;
     a.page_magic = ((1ull << 36) + per - 1) / per;
-    a.rows_min = r.one ? 2 : 1;
+    a.few_rows = r.one ? 16 * r.one_tiles : 0;
     if (r.one) {
       a.whole = r.one_whole;
       a.part = r.one_join ? (float *)workspace : nullptr;
-      snprintf(name, sizeof(name), "paged_attn_one_%s_d%d_r%d", type, c.head_dim, r.one_tiles);
+      snprintf(name, sizeof(name), "paged_attn_%s_%s_d%d_r%d", max_q > 1 ? "few" : "one", type, c.head_dim, r.one_tiles);
       if ((rc = launch("paged", name, dim3(r.one_groups), dim3(256), 0, stream, args, 1))) return rc;
       if (r.one_join) {
         snprintf(name, sizeof(name), "paged_attn_join_%s_d%d_r%d", type, c.head_dim, r.one_tiles);
