@@ -430,6 +430,54 @@ def test_offsets_past_32_bits():
         compare(o, lse, want, 500, D, torch.bfloat16)
 
 
+# ---- refusals, which the library makes before anything is launched ----------
+def test_attention_refusals():
+    q, codes, scales, table, lens, cu = make([300, 150], [1, 1], 4, 2, 16, 64, torch.bfloat16)
+    c, tb, ln, cq, q = device_cache(codes, scales), i32(table), i32(lens), i32(cu), q.cuda()
+    out = torch.empty_like(q)
+    run = lambda grid=(2, 4), qq=q, cc=c, t=tb, ws=None, sm=0.1, mq=1, o=out: K.paged_attn_kernel[grid](
+        qq, *cc, t, ln, cq, o, None, ws, sm, mq, CAUSAL=True)
+    for bad in (dict(grid=(2, 3)), dict(grid=(3, 4)), dict(grid=(2, 4, 2)), dict(sm=float("inf")), dict(sm=float("nan")), dict(mq=0),
+                dict(mq=-1), dict(o=out[:1].expand(2, 4, 64))):
+        with pytest.raises(ValueError):
+            run(**bad)
+    wide = K.paged_cache(4, 1, 320, 16)
+    with pytest.raises(NotImplementedError):
+        K.paged_attention(torch.zeros(2, 1, 320, dtype=torch.bfloat16, device="cuda"), wide, tb, ln, cq, 0.1)
+    # a table that allows long sequences: parts need room
+    t2 = torch.cat([tb, torch.full((2, 400), -1, **I32)], 1)
+    for ws in (None, torch.empty(16, dtype=torch.uint8, device="cuda")):
+        with pytest.raises(ValueError, match="workspace"):
+            run(t=t2, ws=ws)
+    assert rt.load() is not None and torch.isfinite(K.paged_attention(q, c, t2, ln, cq, 0.1, max_q=1).float()).all()
+
+
+def test_plan_and_write_refusals():
+    t, one = i32(np.full((2, 3), -1)), i32([1, 1])
+    with pytest.raises(ValueError):
+        K.paged_plan(one, one, t, i32([0, 1]), 0, 4)
+    with pytest.raises(NotImplementedError):
+        K.paged_plan(one, one, t, i32([0, 1]), 2**30, 4)
+    x = torch.zeros(2, 1, 64, dtype=torch.bfloat16, device="cuda")
+    cache = K.paged_cache(2, 1, 64, 16)
+    with pytest.raises(ValueError):
+        K.paged_write_kernel[(3, )](x, x, one, *cache)
+    with pytest.raises(ValueError):     # pages on top of one another
+        K.paged_write(x, x, one, K.PagedCache(cache.k[:1].expand(2, 1, 16, 64), *cache[1:]))
+
+
+def test_which_kernel_runs():
+    for lens, n, Hq, H, D, max_q, want in (
+            ([90], [1], 4, 2, 128, 1, "paged_attn_one_bf16_d128_r1"), ([5000], [1], 4, 2, 128, 1, "paged_attn_join_bf16_d128_r1"),
+            ([90], [1], 20, 1, 64, 1, "paged_attn_one_bf16_d64_r2"), ([90, 40], [5, 2], 8, 2, 128, 5, "paged_attn_few_bf16_d128_r2"),
+            ([90, 40], [5, 2], 6, 2, 256, 5, "paged_attn_few_bf16_d256_r1"), ([90, 40], [60, 1], 4, 2, 128, 60, "paged_attn_rows_join_bf16_d128_r1"),
+            ([60, 40], [60, 1], 4, 2, 64, 60, "paged_attn_rows_bf16_d64_r2"), ([90], [1], 4, 2, 80, 1, "paged_attn_any_bf16")):
+        q, codes, scales, table, ln, cu = make(lens, n, Hq, H, 16, D, torch.bfloat16)
+        table = np.ascontiguousarray(table[:, :-1])
+        K.paged_attention(q.cuda(), device_cache(codes, scales), i32(table), i32(ln), i32(cu), 0.1, max_q=max_q)
+        assert rt.last_kernel_name() == want
+
+
 # ---- together ---------------------------------------------------------------
 def serve(steps, H, Hq, D, P, pages, B, seed, capture=False):
     """Plan, write and attend step by step (each step: new tokens of each sequence); every step against the 64-bit form."""
@@ -526,3 +574,74 @@ def test_two_streams_at_once():
         torch.cuda.synchronize()
         for (o, lse), (wo, wl) in zip(got, alone):
             assert torch.equal(o, wo) and torch.equal(lse, wl)
+
+
+def test_two_captured_graphs_replayed_side_by_side():
+    # a prompt's piece and a decode step over long sequences, both with parts to join, each with its own workspace
+    made = [make([2500, 4000], [n, n], 8, 2, 64, 128, torch.bfloat16, seed=30 + n) for n in (1, 24)]
+    graphs, eager, out = [], [], []
+    for n, (q, codes, scales, table, lens, cu) in zip((1, 24), made):
+        args = (q.cuda(), device_cache(codes, scales), i32(table), i32(lens), i32(cu), 0.09)
+        eager.append(K.paged_attention(*args, max_q=n, return_lse=True))
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out.append(K.paged_attention(*args, max_q=n, return_lse=True))
+        graphs.append((g, args))
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(6):
+        for o in out:
+            o[0].zero_()
+        torch.cuda.synchronize()
+        for s, (g, _) in zip(streams, graphs):
+            with torch.cuda.stream(s):
+                g.replay()
+        torch.cuda.synchronize()
+        for (o, lse), (wo, wl) in zip(out, eager):
+            assert torch.equal(o, wo) and torch.equal(lse, wl)
+
+
+def test_many_sequences_and_a_long_prompt_together():
+    # over 64 sequences (each lane scans several), prompts beside single tokens and empty ones
+    rng = np.random.default_rng(5)
+    lens = rng.integers(0, 200, 150)
+    n = np.minimum(rng.integers(0, 2, 150), lens)
+    n[[3, 70, 149]] = np.minimum([150, 37, 20], lens[[3, 70, 149]])
+    for Hq, H, D in ((4, 2, 64), (2, 1, 128)):
+        check_attention(list(lens), list(n), Hq, H, 32, D, max_q=int(max(n)), seed=1)
+        check_attention(list(lens), list(np.minimum(n, 1)), Hq, H, 32, D, max_q=1, seed=2)
+        check_attention(list(lens), list(np.minimum(n, 4)), Hq, H, 32, D, max_q=4, seed=3)
+
+
+def dense_on_gpu(q, codes, scales, table, lens, cu, sm_scale, causal):
+    """The 64-bit form with a whole (sequence, head) at a time, for sizes that the row-by-row one is too slow for."""
+    T, Hq, D = q.shape
+    H, P = codes.shape[2], codes.shape[3]
+    values = torch.from_numpy(orc.E4M3).cuda()
+    two = torch.from_numpy(np.ldexp(1.0, np.arange(-127, 129))).cuda()
+    c, s, qd = torch.from_numpy(codes).cuda(), torch.from_numpy(scales).cuda(), q.cuda().double()
+    o, lse = torch.zeros(T, Hq, D, dtype=torch.float64, device="cuda"), torch.zeros(T, Hq, dtype=torch.float64, device="cuda")
+    spread, reach = torch.zeros_like(o), torch.zeros_like(lse)
+    for b in range(len(lens)):
+        n, L = int(cu[b + 1] - cu[b]), int(lens[b])
+        at = torch.from_numpy(table[b, :-(-L // P)]).cuda()
+        hide = torch.arange(L, device="cuda") > torch.arange(L - n, L, device="cuda")[:, None] if causal else torch.zeros(n, L, dtype=torch.bool, device="cuda")
+        for h in range(Hq):
+            k, v = ((values[c[j][at, h * H // Hq].long()] * two[s[j][at, h * H // Hq]][:, None, None]).reshape(-1, D)[:L] for j in range(2))
+            rows = slice(int(cu[b]), int(cu[b + 1]))
+            x = (qd[rows, h] @ k.T * sm_scale).masked_fill(hide, -torch.inf)
+            z = torch.logsumexp(x, 1)
+            p = torch.exp(x - z[:, None])
+            o[rows, h], spread[rows, h], lse[rows, h] = p @ v, p @ v.abs(), z / np.log(2.0)
+            reach[rows, h] = (qd[rows, h].abs() @ k.abs().T).amax(1) * abs(sm_scale) / np.log(2.0)
+    return tuple(x.cpu().numpy() for x in (o, lse, spread, reach))
+
+
+@pytest.mark.parametrize("n,lens,Hq,H,D,causal", [
+    ([1400, 700], [1400, 1500], 64, 64, 64, True), ([1100, 1], [1111, 300], 32, 16, 256, True),     # a workgroup for each row tile
+    ([1900, 150], [1900, 4000], 32, 4, 128, True), ([900, 20], [2000, 3000], 8, 8, 128, False)])    # an even share of the steps
+def test_prompts_of_many_row_tiles(n, lens, Hq, H, D, causal):
+    q, codes, scales, table, lens, cu = make(lens, n, Hq, H, 64, D, torch.bfloat16, seed=D)
+    o, lse = K.paged_attention(q.cuda(), device_cache(codes, scales), i32(table), i32(lens), i32(cu), D ** -0.5, max_q=max(n),
+                               causal=causal, return_lse=True)
+    compare(o, lse, dense_on_gpu(q, codes, scales, table, lens, cu, D ** -0.5, causal), max(lens), D, torch.bfloat16)

@@ -41,7 +41,8 @@ struct PagedAttnArgs {
   float qk_scale;    // sm_scale * log2(e)
   uint64_t page_magic;  // ceil(2^36 / (page_size / 16)): n / (page_size / 16) = (n * page_magic) >> 36 for n < 2^27,
                         // page_size <= 8192
-  float *part;          // partial results of split sequences
-  int32_t whole;        // a workgroup for each (sequence or row tile, head) instead of an even share of the keys
+  float *part, *rows_part; // partial results of split sequences and of split row tiles
+  int32_t whole, rows_whole; // a workgroup for each (sequence, head), (row tile, head) instead of an even share of the keys
+  int32_t rows_groups;  // workgroups for many rows, in front of those for few
   int32_t few_rows;     // launch for many rows: sequences of at most so many (queries times group) are not its
 };

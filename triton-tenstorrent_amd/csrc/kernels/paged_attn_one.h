@@ -150,14 +150,14 @@ struct Split { int32_t q0, more, slot, rows; }; // q0: first packed row of its q
 
 // FEW: sequences may have several queries; without it exactly one, and nothing below looks at a row's own limit.
 template <class E, int D, int MT, bool FEW>
-__device__ __forceinline__ void body(const PagedAttnArgs &a, float *lds) {
+__device__ __forceinline__ void body(const PagedAttnArgs &a, float *lds, int wg, int wgs) {
   constexpr int NS = subtiles<D, MT>(), UK = 64 * NS, KL = D / 64, VW = D / 64; // 16-byte loads of K, dwords of V per row
   constexpr int VB = D / 16, IB = 64 / NS, LD = D + 4;                      // LD: padded LDS row of the merge
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c16 = lane & 15, g = lane >> 4;
   const Walk<UK, 16 * MT, FEW> walk(a);
-  Split *split = (Split *)(a.part + 2 * (int64_t)gridDim.x * part_floats<D, MT>()) + blockIdx.x;
-  const int hk = blockIdx.x % a.c.heads, group = blockIdx.x / a.c.heads;
+  Split *split = (Split *)(a.part + 2 * (int64_t)wgs * part_floats<D, MT>()) + wg;
+  const int hk = wg % a.c.heads, group = wg / a.c.heads;
   int32_t u, u_end, before;
   int32_t each = 1, extra = 0; // units of a group; the first `extra` groups have one more
   Seq sq;
@@ -169,7 +169,7 @@ __device__ __forceinline__ void body(const PagedAttnArgs &a, float *lds) {
     before = u = 0;
     u_end = sq.units;
   } else {
-    const int32_t groups = min((int32_t)(gridDim.x / a.c.heads), walk.total); // fewer units than groups: one each
+    const int32_t groups = min(wgs / a.c.heads, walk.total); // fewer units than groups: one each
     if (group >= groups) {
       if (a.part && tid == 0) split->q0 = -1;
       return;
@@ -448,7 +448,7 @@ __device__ __forceinline__ void body(const PagedAttnArgs &a, float *lds) {
           *(f32x4 *)(wo + row * LD + (g * 4 + r) * VB + i) = (f32x4){acc[m][i][r], acc[m][i + 1][r], acc[m][i + 2][r], acc[m][i + 3][r]};
     }
     __syncthreads();
-    float *slot = a.part + (2 * (int64_t)blockIdx.x + which) * part_floats<D, MT>();
+    float *slot = a.part + (2 * (int64_t)wg + which) * part_floats<D, MT>();
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
       const int row = m * 16 + (tid >> 4), d0 = (tid & 15) * VB;
@@ -495,18 +495,18 @@ __device__ __forceinline__ void body(const PagedAttnArgs &a, float *lds) {
   if (a.part && !noted && tid == 0) split->q0 = -1;
 }
 
-// Adds the parts of the split sequence that workgroup blockIdx.x of the launch before noted, if any.  D / 4 threads a row; what
+// Adds the parts of the split sequence that workgroup wg of the launch before noted, if any.  D / 4 threads a row; what
 // is left of the 256 takes several rows or several parts at once.
-template <class E, int D, int MT> __device__ __forceinline__ void join(const PagedAttnArgs &a, f32x4 *lds) {
+template <class E, int D, int MT> __device__ __forceinline__ void join(const PagedAttnArgs &a, f32x4 *lds, int wg, int wgs) {
   constexpr int TPR = D / 4, SLOTS = 256 / TPR, PF = part_floats<D, MT>();
-  const Split sp = ((const Split *)(a.part + 2 * (int64_t)gridDim.x * PF))[blockIdx.x];
+  const Split sp = ((const Split *)(a.part + 2 * (int64_t)wgs * PF))[wg];
   if (sp.q0 < 0) return;
   const int tid = threadIdx.x, d4 = tid % TPR, at = tid / TPR;
   int across = 1; // rows at once
   while (across < SLOTS && across < sp.rows) across <<= 1;
   const int deep = SLOTS / across, r0 = at % across, p0 = at / across;
-  const int parts = sp.more + 1, head = blockIdx.x % a.c.heads;
-  const float *first = a.part + (2 * (int64_t)blockIdx.x + sp.slot) * PF, *later = a.part + 2 * (int64_t)blockIdx.x * PF;
+  const int parts = sp.more + 1, head = wg % a.c.heads;
+  const float *first = a.part + (2 * (int64_t)wg + sp.slot) * PF, *later = a.part + 2 * (int64_t)wg * PF;
   float *lm = (float *)(lds + 256), *ll = lm + 256;
   for (int rb = 0; rb < sp.rows; rb += across) {
     const int row = min(rb + r0, 16 * MT - 1);
@@ -569,15 +569,15 @@ template <int D, int MT> constexpr int lds_floats() { return 4 * 16 * MT * (D + 
 #define PAGED_ONE(T, E, D, MT, OCC)                                                                           \
   extern "C" __global__ __launch_bounds__(256, OCC) void paged_attn_one_##T##_d##D##_r##MT(PagedAttnArgs a) {  \
     __shared__ __align__(16) float lds[one::lds_floats<D, MT>()];                                             \
-    one::body<one::E, D, MT, false>(a, lds);                                                                  \
+    one::body<one::E, D, MT, false>(a, lds, blockIdx.x, gridDim.x);                                                                  \
   }                                                                                                           \
   extern "C" __global__ __launch_bounds__(256, 2) void paged_attn_few_##T##_d##D##_r##MT(PagedAttnArgs a) {    \
     __shared__ __align__(16) float lds[one::lds_floats<D, MT>()];                                             \
-    one::body<one::E, D, MT, true>(a, lds);                                                                   \
+    one::body<one::E, D, MT, true>(a, lds, blockIdx.x, gridDim.x);                                                                   \
   }                                                                                                           \
   extern "C" __global__ __launch_bounds__(256) void paged_attn_join_##T##_d##D##_r##MT(PagedAttnArgs a) {      \
     __shared__ one::f32x4 lds[256 + 128];                                                                     \
-    one::join<one::E, D, MT>(a, lds);                                                                         \
+    one::join<one::E, D, MT>(a, lds, blockIdx.x, gridDim.x);                                                                         \
   }
 // (the last number: workgroups of paged_attn_one on a CU, which the host's grid counts on too; paged_attn_few has two)
 PAGED_ONE(bf16, Bf, 64, 1, 3)

@@ -74,7 +74,7 @@ struct Walk {
   int per;
   int32_t base, total;
   __device__ __forceinline__ int32_t units_of(const Seq &sq) const {
-    if (a.whole) return sq.tiles;
+    if (a.rows_whole) return sq.tiles;
     int32_t n = 0;
     for (int i = 0; i < sq.tiles; ++i) n += steps_of(a, sq, i);
     return n;
@@ -86,7 +86,7 @@ struct Walk {
     bool large = false; // a sequence of many tiles, which all lanes count together
     for (int b = min(lane * per, a.b); b < min(lane * per + per, a.b); ++b) {
       const Seq sq = seq_of(a, b);
-      large = per == 1 && !a.whole && sq.tiles > 8;
+      large = per == 1 && !a.rows_whole && sq.tiles > 8;
       if (!large) n += units_of(sq);
     }
     for (uint64_t todo = __ballot(large); todo; todo &= todo - 1) {
@@ -148,23 +148,23 @@ template <int D> constexpr int stage_bytes() { return (64 * D * 2 * 2 + kMeta + 
 template <int D> constexpr int lds_bytes() { return 2 * stage_bytes<D>(); }
 
 template <class E, int D>
-__device__ __forceinline__ void body(const PagedAttnArgs &a, uint8_t *lds) {
+__device__ __forceinline__ void body(const PagedAttnArgs &a, uint8_t *lds, int wg, int wgs) {
   constexpr int DK = D / 16, DT = D / 32, KB = D / 4, VB = D / 16, KW = KB / 16, VW = VB / 4;
   constexpr int KROW = D * 2, VOFF = 64 * KROW, FOFF = 2 * VOFF;
   constexpr int KMASK = D == 64 ? 7 : 15, KSH = D == 64 ? 1 : 0; // chunk swizzle of K rows
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c32 = lane & 31, hi = lane >> 5;
   const Walk walk(a);
-  const int heads = a.c.heads, hk = blockIdx.x % heads, group = blockIdx.x / heads;
-  Split *split = (Split *)(a.part + 2 * (int64_t)gridDim.x * part_floats<D>()) + blockIdx.x;
+  const int heads = a.c.heads, hk = wg % heads, group = wg / heads;
+  Split *split = (Split *)(a.rows_part + 2 * (int64_t)wgs * part_floats<D>()) + wg;
   int32_t u, u_end, before;
   int32_t each = 1, extra = 0; // steps of a group; the first `extra` groups have one more
-  if (a.whole) {
+  if (a.rows_whole) {
     u = walk.total - 1 - group; // late rows, which attend most keys, first
     if (u < 0) return;
     u_end = u + 1;
   } else {
-    const int32_t groups = min((int32_t)(gridDim.x / heads), walk.total);
+    const int32_t groups = min(wgs / heads, walk.total);
     if (group >= groups) {
       if (tid == 0) split->b = -1;
       return;
@@ -176,7 +176,7 @@ __device__ __forceinline__ void body(const PagedAttnArgs &a, uint8_t *lds) {
   }
   Seq sq;
   int b = walk.find(u, &before, &sq), tile;
-  if (a.whole) {
+  if (a.rows_whole) {
     tile = u - before;
   } else {
     int32_t inside;
@@ -189,7 +189,7 @@ __device__ __forceinline__ void body(const PagedAttnArgs &a, uint8_t *lds) {
   for (;;) {
   const int R = sq.n * a.group, row0 = tile * kRows;
   const int nsteps = steps_of(a, sq, tile);
-  const int k_lo = a.whole ? 0 : u - before, k_hi = a.whole ? nsteps : min(nsteps, k_lo + (u_end - u));
+  const int k_lo = a.rows_whole ? 0 : u - before, k_hi = a.rows_whole ? nsteps : min(nsteps, k_lo + (u_end - u));
 
   const int row = row0 + wave * 32 + c32;
   const int qi = min(row, R - 1) / a.group, qg = min(row, R - 1) % a.group;
@@ -474,7 +474,7 @@ __device__ __forceinline__ void body(const PagedAttnArgs &a, uint8_t *lds) {
         }
       if (a.lse && hi == 0) a.lse[t * a.heads_q + hq] = none ? -kInf : mref - kLift + __builtin_log2f(lsum);
     } else {
-      float *p = a.part + (2 * (int64_t)blockIdx.x + which) * part_floats<D>();
+      float *p = a.rows_part + (2 * (int64_t)wg + which) * part_floats<D>();
       const int lr = wave * 32 + c32;
 #pragma unroll
       for (int i = 0; i < DT; ++i)
@@ -484,7 +484,7 @@ __device__ __forceinline__ void body(const PagedAttnArgs &a, uint8_t *lds) {
       if (hi == 0) { p[kRows * D + lr * 2] = mref; p[kRows * D + lr * 2 + 1] = lsum; }
     }
   }
-  if (a.whole) return;
+  if (a.rows_whole) return;
   if (cut && k_lo == 0) {
     const int32_t last = before + nsteps - 1, larger = extra * (each + 1); // the tile's last step, and the group that has it
     const int32_t owner = last < larger ? last / (each + 1) : extra + (last - larger) / each;
@@ -503,17 +503,16 @@ __device__ __forceinline__ void body(const PagedAttnArgs &a, uint8_t *lds) {
   if (!noted && tid == 0) split->b = -1;
 }
 
-// Adds the parts of the split tile that workgroup blockIdx.x of the launch before noted, if any: grid (workgroups, 8),
-// 16 rows each.
-template <class E, int D> __device__ __forceinline__ void join(const PagedAttnArgs &a) {
+// Adds the parts of the split tile that workgroup wg of the launch before noted, if any: rows 16 part .. + 15.
+template <class E, int D> __device__ __forceinline__ void join(const PagedAttnArgs &a, int wg, int part, int wgs) {
   constexpr int PF = part_floats<D>(), VB = D / 16;
-  const Split sp = ((const Split *)(a.part + 2 * (int64_t)gridDim.x * PF))[blockIdx.x];
+  const Split sp = ((const Split *)(a.rows_part + 2 * (int64_t)wgs * PF))[wg];
   if (sp.b < 0) return;
   const Seq sq = seq_of(a, sp.b);
-  const int row0 = sp.tile * kRows, lr = blockIdx.y * 16 + (threadIdx.x >> 4), d0 = (threadIdx.x & 15) * VB;
+  const int row0 = sp.tile * kRows, lr = part * 16 + (threadIdx.x >> 4), d0 = (threadIdx.x & 15) * VB;
   if (row0 + lr >= sq.n * a.group) return;
   const int heads = a.c.heads, parts = sp.more + 1;
-  const float *first = a.part + (2 * (int64_t)blockIdx.x + sp.slot) * PF, *later = a.part + 2 * (int64_t)blockIdx.x * PF;
+  const float *first = a.rows_part + (2 * (int64_t)wg + sp.slot) * PF, *later = a.rows_part + 2 * (int64_t)wg * PF;
   float m = -kInf, l = 0.0f;
   f32x4 o[VB / 4];
 #pragma unroll
@@ -542,7 +541,7 @@ template <class E, int D> __device__ __forceinline__ void join(const PagedAttnAr
       m = mn;
     }
   }
-  const int qi = (row0 + lr) / a.group, hq = blockIdx.x % heads * a.group + (row0 + lr) % a.group;
+  const int qi = (row0 + lr) / a.group, hq = wg % heads * a.group + (row0 + lr) % a.group;
   const int64_t t = sq.q0 + qi;
   const bool none = l == 0.0f && m == -kInf;
   const float inv = none ? 0.0f : kOut / l;
@@ -555,18 +554,30 @@ template <class E, int D> __device__ __forceinline__ void join(const PagedAttnAr
 
 } // namespace rows
 
-#define PAGED_ROWS(T, E, D, OCC)                                                                              \
-  extern "C" __global__ __launch_bounds__(256, OCC) void paged_attn_rows_##T##_d##D(PagedAttnArgs a) {         \
-    __shared__ __align__(512) uint8_t lds[rows::lds_bytes<D>()];                                               \
-    rows::body<rows::E, D>(a, lds);                                                                           \
+// Many rows, and beside them, in the workgroups behind, the sequences of few.
+#define PAGED_MIXED(T, E, D, MT, OCC)                                                                         \
+  extern "C" __global__ __launch_bounds__(256, OCC) void paged_attn_rows_##T##_d##D##_r##MT(PagedAttnArgs a) { \
+    constexpr int bytes = rows::lds_bytes<D>() > one::lds_floats<D, MT>() * 4 ? rows::lds_bytes<D>() : one::lds_floats<D, MT>() * 4; \
+    __shared__ __align__(512) uint8_t lds[bytes];                                                             \
+    if ((int)blockIdx.x < a.rows_groups)                                                                      \
+      rows::body<rows::E, D>(a, lds, blockIdx.x, a.rows_groups);                                              \
+    else                                                                                                      \
+      one::body<one::E, D, MT, true>(a, (float *)lds, blockIdx.x - a.rows_groups, gridDim.x - a.rows_groups); \
   }                                                                                                           \
-  extern "C" __global__ __launch_bounds__(256) void paged_attn_rows_join_##T##_d##D(PagedAttnArgs a) {         \
-    rows::join<rows::E, D>(a);                                                                                \
+  /* 8 workgroups for each that may have split a row tile, then one for each that may have split a sequence */ \
+  extern "C" __global__ __launch_bounds__(256) void paged_attn_rows_join_##T##_d##D##_r##MT(PagedAttnArgs a) { \
+    __shared__ one::f32x4 lds[256 + 128];                                                                     \
+    if ((int)blockIdx.x < 8 * a.rows_groups)                                                                  \
+      rows::join<rows::E, D>(a, blockIdx.x / 8, blockIdx.x % 8, a.rows_groups);                               \
+    else                                                                                                      \
+      one::join<one::E, D, MT>(a, lds, blockIdx.x - 8 * a.rows_groups, gridDim.x - 8 * a.rows_groups);        \
   }
-PAGED_ROWS(bf16, Bf, 64, 2)
-PAGED_ROWS(bf16, Bf, 128, 2)
-PAGED_ROWS(bf16, Bf, 256, 1)
-PAGED_ROWS(f16, Hf, 64, 2)
-PAGED_ROWS(f16, Hf, 128, 2)
-PAGED_ROWS(f16, Hf, 256, 1)
-#undef PAGED_ROWS
+PAGED_MIXED(bf16, Bf, 64, 1, 2)
+PAGED_MIXED(bf16, Bf, 64, 2, 2)
+PAGED_MIXED(bf16, Bf, 128, 1, 2)
+PAGED_MIXED(bf16, Bf, 256, 1, 1)
+PAGED_MIXED(f16, Hf, 64, 1, 2)
+PAGED_MIXED(f16, Hf, 64, 2, 2)
+PAGED_MIXED(f16, Hf, 128, 1, 2)
+PAGED_MIXED(f16, Hf, 256, 1, 1)
+#undef PAGED_MIXED

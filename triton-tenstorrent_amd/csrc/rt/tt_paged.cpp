@@ -40,8 +40,8 @@ int check_grid(const char *who, const uint32_t grid[3], int32_t x, int32_t y) {
 // How tt_paged_attn runs a call of these sizes.
 struct Route {
   bool fast = false;
-  // few queries of a sequence: paged_attn_one_* (exactly one) or paged_attn_few_*, its 16-row tiles of query heads, its workgroups, and whether sequences may be
-  // split (partial results, joined by a second launch)
+  // few queries of a sequence: paged_attn_one_* (exactly one), paged_attn_few_*, or a part of paged_attn_rows_*; its
+  // 16-row tiles, its workgroups, and whether sequences may be split (partial results, joined by a second launch)
   bool one = false, one_whole = false, one_join = false;
   int one_tiles = 1;
   uint32_t one_groups = 0;
@@ -57,10 +57,12 @@ Route route_of(const PagedCacheArgs &c, int32_t B, int32_t max_pages, int32_t to
   if ((int64_t)tokens * group > INT32_MAX - 256) return r;
   r.fast = true;
   const int64_t keys = (int64_t)max_pages * c.page_size;
-  // Sequences of few queries go to their own kernel: queries times group up to 32 rows (16 at head dim 256), or 16 where
-  // none can have more.  It is left out where one sequence is all there is and may have more.
+  // Sequences of few queries go to their own kernel: queries times group up to 32 rows, or 16 where none can have more,
+  // where the head dim is 256, or where it is 128 and the registers are shared with the kernel for many rows (pieces of
+  // prompts and single tokens: 95 us against 98 with 32).  It is left out where one sequence is all there is and may
+  // have more.
   const int64_t rows = (int64_t)max_q * group;
-  const int few = D == 256 || rows <= 16 ? 16 : 32;
+  const int few = D == 256 || rows <= 16 || (D == 128 && rows > 32) ? 16 : 32;
   r.one = group <= few && (rows <= few || B > 1);
   r.rows = !r.one || rows > few;
   if (r.one) {
@@ -134,6 +136,11 @@ extern "C" int tt_paged_write(const void *k, const void *v, const int64_t k_stri
   if (!k || !v || !k_strides || !v_strides || !slot_map) return fail(RT_ERR_INVALID, "%s: null pointer", who);
   for (int i = 0; i < 2; ++i)
     if (k_strides[i] < 0 || v_strides[i] < 0) return fail(RT_ERR_INVALID, "%s: negative stride", who);
+  // the cache is written: no two of its elements may lie in one place because a stride is 0
+  const PagedCacheArgs &w = a.c;
+  if ((w.pages > 1 && (!w.k_page || !w.v_page || !w.ks_page || !w.vs_page)) || (w.heads > 1 && (!w.k_head || !w.v_head || !w.ks_head || !w.vs_head)) ||
+      (w.page_size > 1 && (!w.k_tok || !w.v_tok)))
+    return fail(RT_ERR_INVALID, "%s: a cache stride is 0", who);
   if (!aligned(k, 2) || !aligned(v, 2) || !aligned(slot_map, 4)) return fail(RT_ERR_INVALID, "%s: misaligned pointer", who);
   if ((rc = check_grid(who, grid, tokens, 1))) return rc;
   a.k = (const uint16_t *)k; a.v = (const uint16_t *)v; a.slots = slot_map;
@@ -195,6 +202,7 @@ extern "C" int tt_paged_attn(const void *q, const int64_t q_strides[2], const tt
   if ((int64_t)max_pages * a.c.page_size > INT32_MAX) return fail(RT_ERR_UNSUPPORTED, "%s: max_pages * page_size exceeds int32", who);
   for (int i = 0; i < 2; ++i)
     if (q_strides[i] < 0 || o_strides[i] < 0) return fail(RT_ERR_INVALID, "%s: negative stride", who);
+  if ((tokens > 1 && !o_strides[0]) || (heads_q > 1 && !o_strides[1])) return fail(RT_ERR_INVALID, "%s: a stride of o is 0", who);
   if (!aligned(q, 2) || !aligned(o, 2) || !aligned(block_table, 4) || !aligned(lens, 4) || !aligned(cu_q, 4) || !aligned(lse, 4))
     return fail(RT_ERR_INVALID, "%s: misaligned pointer", who);
   if (!std::isfinite(sm_scale)) return fail(RT_ERR_INVALID, "%s: sm_scale is not finite", who);
@@ -220,28 +228,23 @@ extern "C" int tt_paged_attn(const void *q, const int64_t q_strides[2], const tt
     const uint64_t per = (uint64_t)c.page_size / 16;
     a.page_magic = ((1ull << 36) + per - 1) / per;
     a.few_rows = r.one ? 16 * r.one_tiles : 0;
-    if (r.one) {
-      a.whole = r.one_whole;
-      a.part = r.one_join ? (float *)workspace : nullptr;
-      snprintf(name, sizeof(name), "paged_attn_%s_%s_d%d_r%d", max_q > 1 ? "few" : "one", type, c.head_dim, r.one_tiles);
-      if ((rc = launch("paged", name, dim3(r.one_groups), dim3(256), 0, stream, args, 1))) return rc;
-      if (r.one_join) {
-        snprintf(name, sizeof(name), "paged_attn_join_%s_d%d_r%d", type, c.head_dim, r.one_tiles);
-        if ((rc = launch("paged", name, dim3(r.one_groups), dim3(256), 0, stream, args, 1))) return rc;
-      }
-    }
+    a.whole = r.one_whole;
+    a.part = r.one_join ? (float *)workspace : nullptr;
+    const bool few = r.rows || max_q > 1;
+    const char *kernel = r.rows ? "rows" : few ? "few" : "one";
+    snprintf(name, sizeof(name), "paged_attn_%s_%s_d%d_r%d", kernel, type, c.head_dim, r.one_tiles);
     if (r.rows) {
-      a.part = (float *)((char *)workspace + r.one_bytes);
-      snprintf(name, sizeof(name), "paged_attn_rows_%s_d%d", type, c.head_dim);
-      if (r.rows_groups > INT32_MAX) return fail(RT_ERR_UNSUPPORTED, "%s: tokens * heads exceeds the grid", who);
-      a.whole = r.rows_whole;
-      if ((rc = launch("paged", name, dim3((uint32_t)r.rows_groups), dim3(256), 0, stream, args, 1))) return rc;
-      if (!r.rows_whole) {
-        snprintf(name, sizeof(name), "paged_attn_rows_join_%s_d%d", type, c.head_dim);
-        if ((rc = launch("paged", name, dim3((uint32_t)r.rows_groups, 8), dim3(256), 0, stream, args, 1))) return rc;
-      }
+      a.rows_whole = r.rows_whole;
+      a.rows_part = (float *)((char *)workspace + r.one_bytes);
+      a.rows_groups = (int32_t)r.rows_groups;
     }
-    return RT_OK;
+    if (r.rows_groups + r.one_groups > INT32_MAX / 8) return fail(RT_ERR_UNSUPPORTED, "%s: tokens * heads exceeds the grid", who);
+    if ((rc = launch("paged", name, dim3((uint32_t)(r.rows_groups + r.one_groups)), dim3(256), 0, stream, args, 1))) return rc;
+    if (r.rows_whole) a.rows_groups = 0; // nothing to join there
+    const uint32_t joins = 8 * (uint32_t)a.rows_groups + (r.one_join ? r.one_groups : 0);
+    if (!joins) return RT_OK;
+    snprintf(name, sizeof(name), "paged_attn_%s_%s_d%d_r%d", r.rows ? "rows_join" : "join", type, c.head_dim, r.one_tiles);
+    return launch("paged", name, dim3(joins), dim3(256), 0, stream, args, 1);
   }
   return launch("paged", dtype == TT_BF16 ? "paged_attn_any_bf16" : "paged_attn_any_f16",
                 dim3((uint32_t)tokens, (uint32_t)heads_q), dim3(64), 0, stream, args, 1);
