@@ -43,6 +43,7 @@ struct PagedAttnArgs {
                         // page_size <= 8192
   float *part, *rows_part; // partial results of split sequences and of split row tiles
   int32_t whole, rows_whole; // a workgroup for each (sequence, head), (row tile, head) instead of an even share of the keys
+  int32_t join_pieces;  // workgroups that join a split sequence of few rows
   int32_t rows_groups;  // workgroups for many rows, in front of those for few
   int32_t few_rows;     // launch for many rows: sequences of at most so many (queries times group) are not its
 };

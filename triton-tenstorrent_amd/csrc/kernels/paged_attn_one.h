@@ -495,20 +495,22 @@ __device__ __forceinline__ void body(const PagedAttnArgs &a, float *lds, int wg,
   if (a.part && !noted && tid == 0) split->q0 = -1;
 }
 
-// Adds the parts of the split sequence that workgroup wg of the launch before noted, if any.  D / 4 threads a row; what
+// Adds the parts of the split sequence that workgroup wg of the launch before noted, if any: one of
+// `join_pieces` pieces of its rows.  D / 4 threads a row; what
 // is left of the 256 takes several rows or several parts at once.
-template <class E, int D, int MT> __device__ __forceinline__ void join(const PagedAttnArgs &a, f32x4 *lds, int wg, int wgs) {
+template <class E, int D, int MT> __device__ __forceinline__ void join(const PagedAttnArgs &a, f32x4 *lds, int wg, int piece, int wgs) {
   constexpr int TPR = D / 4, SLOTS = 256 / TPR, PF = part_floats<D, MT>();
   const Split sp = ((const Split *)(a.part + 2 * (int64_t)wgs * PF))[wg];
   if (sp.q0 < 0) return;
   const int tid = threadIdx.x, d4 = tid % TPR, at = tid / TPR;
+  const int share = (sp.rows + a.join_pieces - 1) / a.join_pieces, row_end = min((piece + 1) * share, sp.rows); // this piece's rows
   int across = 1; // rows at once
-  while (across < SLOTS && across < sp.rows) across <<= 1;
+  while (across < SLOTS && across < share) across <<= 1;
   const int deep = SLOTS / across, r0 = at % across, p0 = at / across;
   const int parts = sp.more + 1, head = wg % a.c.heads;
   const float *first = a.part + (2 * (int64_t)wg + sp.slot) * PF, *later = a.part + 2 * (int64_t)wg * PF;
   float *lm = (float *)(lds + 256), *ll = lm + 256;
-  for (int rb = 0; rb < sp.rows; rb += across) {
+  for (int rb = piece * share; rb < row_end; rb += across) {
     const int row = min(rb + r0, 16 * MT - 1);
     float m = -kInf, l = 0.0f;
     f32x4 o = {0, 0, 0, 0};
@@ -550,7 +552,7 @@ template <class E, int D, int MT> __device__ __forceinline__ void join(const Pag
         }
       __syncthreads();
     }
-    if (p0 == 0 && rb + r0 < sp.rows) {
+    if (p0 == 0 && rb + r0 < row_end) {
       const int64_t t = sp.q0 + row / a.group;
       const int hq = head * a.group + row % a.group;
       const bool none = l == 0.0f && m == -kInf;
@@ -577,7 +579,7 @@ template <int D, int MT> constexpr int lds_floats() { return 4 * 16 * MT * (D + 
   }                                                                                                           \
   extern "C" __global__ __launch_bounds__(256) void paged_attn_join_##T##_d##D##_r##MT(PagedAttnArgs a) {      \
     __shared__ one::f32x4 lds[256 + 128];                                                                     \
-    one::join<one::E, D, MT>(a, lds, blockIdx.x, gridDim.x);                                                                         \
+    one::join<one::E, D, MT>(a, lds, blockIdx.x / a.join_pieces, blockIdx.x % a.join_pieces, gridDim.x / a.join_pieces);                                                                         \
   }
 // (the last number: workgroups of paged_attn_one on a CU, which the host's grid counts on too; paged_attn_few has two)
 PAGED_ONE(bf16, Bf, 64, 1, 3)

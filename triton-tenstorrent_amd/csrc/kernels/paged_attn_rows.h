@@ -564,13 +564,14 @@ template <class E, int D> __device__ __forceinline__ void join(const PagedAttnAr
     else                                                                                                      \
       one::body<one::E, D, MT, true>(a, (float *)lds, blockIdx.x - a.rows_groups, gridDim.x - a.rows_groups); \
   }                                                                                                           \
-  /* 8 workgroups for each that may have split a row tile, then one for each that may have split a sequence */ \
+  /* 8 workgroups for each that may have split a row tile, then join_pieces for each that may have split a sequence */ \
   extern "C" __global__ __launch_bounds__(256) void paged_attn_rows_join_##T##_d##D##_r##MT(PagedAttnArgs a) { \
     __shared__ one::f32x4 lds[256 + 128];                                                                     \
     if ((int)blockIdx.x < 8 * a.rows_groups)                                                                  \
       rows::join<rows::E, D>(a, blockIdx.x / 8, blockIdx.x % 8, a.rows_groups);                               \
     else                                                                                                      \
-      one::join<one::E, D, MT>(a, lds, blockIdx.x - 8 * a.rows_groups, gridDim.x - 8 * a.rows_groups);        \
+      one::join<one::E, D, MT>(a, lds, (blockIdx.x - 8 * a.rows_groups) / a.join_pieces,                      \
+                               (blockIdx.x - 8 * a.rows_groups) % a.join_pieces, (gridDim.x - 8 * a.rows_groups) / a.join_pieces); \
   }
 PAGED_MIXED(bf16, Bf, 64, 1, 2)
 PAGED_MIXED(bf16, Bf, 64, 2, 2)

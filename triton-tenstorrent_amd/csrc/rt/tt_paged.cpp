@@ -43,7 +43,7 @@ struct Route {
   // few queries of a sequence: paged_attn_one_* (exactly one), paged_attn_few_*, or a part of paged_attn_rows_*; its
   // 16-row tiles, its workgroups, and whether sequences may be split (partial results, joined by a second launch)
   bool one = false, one_whole = false, one_join = false;
-  int one_tiles = 1;
+  int one_tiles = 1, join_pieces = 1;
   uint32_t one_groups = 0;
   // many: paged_attn_rows_*, its workgroups, and whether each has a 128-row tile of its own
   bool rows = false, rows_whole = false;
@@ -81,6 +81,9 @@ Route route_of(const PagedCacheArgs &c, int32_t B, int32_t max_pages, int32_t to
       r.one_groups = (uint32_t)pairs;
     }
     r.one_join = !r.one_whole && most > 1 && r.one_groups > (uint32_t)c.heads;
+    // sequences of many parts: their rows are joined by several workgroups (6 sequences of 16 parts: 9 us -> 5; with 2 to 3
+    // parts the more workgroups cost 2 us)
+    if (r.one_groups / c.heads >= 4 * (uint32_t)B) r.join_pieces = 4;
     if (r.one_join) r.one_bytes = (size_t)r.one_groups * (2 * (16 * r.one_tiles * D + 32 * r.one_tiles) * sizeof(float) + 16);
   }
   r.workspace = r.one_bytes;
@@ -230,6 +233,7 @@ extern "C" int tt_paged_attn(const void *q, const int64_t q_strides[2], const tt
     a.few_rows = r.one ? 16 * r.one_tiles : 0;
     a.whole = r.one_whole;
     a.part = r.one_join ? (float *)workspace : nullptr;
+    a.join_pieces = r.join_pieces;
     const bool few = r.rows || max_q > 1;
     const char *kernel = r.rows ? "rows" : few ? "few" : "one";
     snprintf(name, sizeof(name), "paged_attn_%s_%s_d%d_r%d", kernel, type, c.head_dim, r.one_tiles);
@@ -241,7 +245,7 @@ extern "C" int tt_paged_attn(const void *q, const int64_t q_strides[2], const tt
     if (r.rows_groups + r.one_groups > INT32_MAX / 8) return fail(RT_ERR_UNSUPPORTED, "%s: tokens * heads exceeds the grid", who);
     if ((rc = launch("paged", name, dim3((uint32_t)(r.rows_groups + r.one_groups)), dim3(256), 0, stream, args, 1))) return rc;
     if (r.rows_whole) a.rows_groups = 0; // nothing to join there
-    const uint32_t joins = 8 * (uint32_t)a.rows_groups + (r.one_join ? r.one_groups : 0);
+    const uint32_t joins = 8 * (uint32_t)a.rows_groups + (r.one_join ? r.one_groups * r.join_pieces : 0);
     if (!joins) return RT_OK;
     snprintf(name, sizeof(name), "paged_attn_%s_%s_d%d_r%d", r.rows ? "rows_join" : "join", type, c.head_dim, r.one_tiles);
     return launch("paged", name, dim3(joins), dim3(256), 0, stream, args, 1);
