@@ -645,3 +645,24 @@ def test_prompts_of_many_row_tiles(n, lens, Hq, H, D, causal):
     o, lse = K.paged_attention(q.cuda(), device_cache(codes, scales), i32(table), i32(lens), i32(cu), D ** -0.5, max_q=max(n),
                                causal=causal, return_lse=True)
     compare(o, lse, dense_on_gpu(q, codes, scales, table, lens, cu, D ** -0.5, causal), max(lens), D, torch.bfloat16)
+
+
+@pytest.mark.parametrize("a,b", [("ctx_lens", "lens"), ("new_lens", "lens"), ("free_start", "free_end"), ("block_table", "lens"),
+                                 ("free_pages", "slot_map"), ("cu_new", "slot_map"), ("lens", "cu_new")])
+def test_plan_refuses_outputs_over_other_arguments(a, b):
+    make = lambda: dict(ctx_lens=i32([3, 0]), new_lens=i32([1, 1]), block_table=i32([[4, -1], [-1, -1]]), free_pages=i32([1, 2, 3]),
+                        free_start=i32([0]), lens=i32([0, 0]), cu_new=i32([0, 0, 0]), slot_map=i32([0, 0, 0]), free_end=i32([0]))
+    v = make()
+    n = v[b].numel()
+    whole = i32([0] * 8)
+    v[a] = whole[:v[a].numel()].view(v[a].shape)
+    v[b] = whole[v[a].numel() - 1:][:n]        # the last element of the one is the first of the other
+    with pytest.raises(ValueError, match="overlap"):
+        K.paged_plan_kernel[(2, )](*v.values(), PAGE_SIZE=4)
+    v[b] = whole[v[a].numel():][:n].view(v[b].shape) if v[a].numel() + n <= 8 else i32([0] * n)
+    K.paged_plan_kernel[(2, )](*v.values(), PAGE_SIZE=4)       # side by side
+
+
+def test_plan_of_no_sequence_is_refused():
+    with pytest.raises(ValueError):
+        K.paged_plan(i32([]), i32([]), torch.empty(0, 3, **I32), i32([1]), 4, 2)

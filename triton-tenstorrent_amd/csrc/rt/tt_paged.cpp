@@ -116,6 +116,16 @@ extern "C" int tt_paged_plan(const int32_t *ctx_lens, const int32_t *new_lens, i
                         (const void *)free_start, (const void *)lens, (const void *)cu_new, (const void *)slot_map,
                         (const void *)free_end})
     if (!aligned(p, 4)) return fail(RT_ERR_INVALID, "%s: pointer not aligned to 4 bytes", who);
+  // One workgroup may write its results while another still reads: no output may share memory with anything else.
+  const struct { const char *name; const void *p; int64_t n; bool out; } v[] = {
+      {"ctx_lens", ctx_lens, B, false}, {"new_lens", new_lens, B, false}, {"free_pages", free_pages, num_free, false},
+      {"free_start", free_start, free_start ? 1 : 0, false}, {"block_table", block_table, (B - 1) * table_stride + max_pages, true},
+      {"lens", lens, B, true}, {"cu_new", cu_new, (int64_t)B + 1, true}, {"slot_map", slot_map, max_tokens, true},
+      {"free_end", free_end, 1, true}};
+  for (const auto &x : v)
+    for (const auto &y : v)
+      if (&x < &y && y.out && x.n && y.n && (uintptr_t)x.p < (uintptr_t)y.p + 4 * y.n && (uintptr_t)y.p < (uintptr_t)x.p + 4 * x.n)
+        return fail(RT_ERR_INVALID, "%s: %s and %s overlap", who, x.name, y.name);
   int rc;
   if ((rc = check_grid(who, grid, B, 1))) return rc;
   PagedPlanArgs a{ctx_lens, new_lens, block_table, free_pages, free_start, lens, cu_new, slot_map, free_end,
