@@ -666,3 +666,20 @@ def test_plan_refuses_outputs_over_other_arguments(a, b):
 def test_plan_of_no_sequence_is_refused():
     with pytest.raises(ValueError):
         K.paged_plan(i32([]), i32([]), torch.empty(0, 3, **I32), i32([1]), 4, 2)
+
+
+@pytest.mark.parametrize("P,width,B,n,kernel", [
+    (16, 2**27 - 1, 1, 1, "any"),            # positions up to 2^31 - 16
+    (16, 2**27 - 1, 1, 9, "any"),
+    (8192, 2**18 - 1, 130, 1, "one"),        # 130 sequences of up to 2^24 units of 128 keys: each is one workgroup's
+    (8192, 2**18 - 1, 66, 10, "rows"),       # the same for row tiles
+])
+def test_tables_of_nearly_31_bits(P, width, B, n, kernel):
+    q, codes, scales, narrow, lens, cu = make([7 * b % 40 + n for b in range(B)], [n] * B, 4, 1, P, 128, torch.bfloat16)
+    table = torch.full((B, width), -1, **I32)
+    table[:, :narrow.shape[1]] = i32(narrow)
+    cache = device_cache(codes, scales)
+    o, lse = K.paged_attention(q.cuda(), cache, table, i32(lens), i32(cu), 0.09, max_q=n, return_lse=True)
+    assert f"_{kernel}_" in rt.last_kernel_name()
+    want = orc.attention(q.double().numpy(), codes[0], codes[1], scales[0], scales[1], narrow, lens, cu, 0.09, True)
+    compare(o, lse, want, max(lens), 128, torch.bfloat16)

@@ -54,9 +54,10 @@ Route route_of(const PagedCacheArgs &c, int32_t B, int32_t max_pages, int32_t to
   Route r;
   const int D = c.head_dim, group = heads_q / c.heads, cus = props()->multiprocessor_count;
   if ((D != 64 && D != 128 && D != 256) || c.page_size % 16 || c.page_size > 8192) return r;
-  if ((int64_t)tokens * group > INT32_MAX - 256) return r;
-  r.fast = true;
   const int64_t keys = (int64_t)max_pages * c.page_size;
+  // positions and rows, rounded up to a unit or a tile, are 32-bit there
+  if ((int64_t)tokens * group > INT32_MAX - 1024 || keys > INT32_MAX - 1024) return r;
+  r.fast = true;
   // Sequences of few queries go to their own kernel: queries times group up to 32 rows, or 16 where none can have more,
   // where the head dim is 256, or where it is 128 and the registers are shared with the kernel for many rows (pieces of
   // prompts and single tokens: 95 us against 98 with 32).  It is left out where one sequence is all there is and may
@@ -75,8 +76,10 @@ Route route_of(const PagedCacheArgs &c, int32_t B, int32_t max_pages, int32_t to
     // A workgroup for each (sequence, head) instead, without parts to join, where the table allows no long sequence: up to
     // 8 units take less than the second launch costs (8 heads of 512 keys: 7.4 us against 11.5; 2048 keys: 20), up to 16
     // where there are pairs enough to keep the chip busy (512 pairs of 2048 keys: 44.6 us against 56).
+    // Also where the table allows more units than 32 bits count.
     const int64_t pairs = (int64_t)B * c.heads;
-    if (most <= (pairs >= slots * c.heads / 2 ? 16 : 8) && pairs <= INT32_MAX) {
+    if (most <= (pairs >= slots * c.heads / 2 ? 16 : 8) || most * std::min(B, tokens) > INT32_MAX) {
+      if (pairs > INT32_MAX / 16) return Route();
       r.one_whole = true;
       r.one_groups = (uint32_t)pairs;
     }
@@ -89,7 +92,8 @@ Route route_of(const PagedCacheArgs &c, int32_t B, int32_t max_pages, int32_t to
   r.workspace = r.one_bytes;
   if (r.rows) {
     const int64_t items = ((int64_t)tokens * group / 128 + std::min(B, tokens)) * c.heads, slots = (D == 256 ? 1 : 2) * cus;
-    r.rows_whole = items >= 2 * slots || keys <= 64;
+    // (the last condition: more steps than 32 bits count)
+    r.rows_whole = items >= 2 * slots || keys <= 64 || items / c.heads * cdiv64(keys, 64) > INT32_MAX;
     r.rows_groups = r.rows_whole ? items : std::max<int64_t>(slots / c.heads, 1) * c.heads;
     if (!r.rows_whole) r.workspace += (size_t)r.rows_groups * (2 * (128 * D + 256) * sizeof(float) + 16);
   }
