@@ -144,6 +144,15 @@ def test_another_current_device_is_refused(lib, monkeypatch):
         K.paged_attn_kernel[(6, 8)](*attn_args(), CAUSAL=True)
 
 
+def test_another_current_device_is_refused_in_a_repeated_launch(lib, monkeypatch):
+    for _ in range(3):
+        K.paged_attn_kernel[(6, 8)](*attn_args(), CAUSAL=True)
+    monkeypatch.setattr(drv.TTDriver, "get_current_device", lambda self: 1)
+    with pytest.raises(rt.InvalidLaunch, match="current device"):
+        K.paged_attn_kernel[(6, 8)](*attn_args(), CAUSAL=True)
+    assert len(lib.calls) == 3
+
+
 def test_tensors_on_the_cpu_are_refused_by_the_wrappers():
     q = torch.zeros(2, 4, 64, dtype=BF16)
     c = K.paged_cache(4, 2, 64, 16, device="cpu")
