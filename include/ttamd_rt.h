@@ -357,11 +357,11 @@ TTAMD_API int tt_attn_fwd(float sm_scale, float *M, int32_t Z, int32_t H, const 
 /* ----------------------------------------------------------------------- */
 
 /* The cache of one layer: for K and for V, e4m3 codes [num_pages, heads, page_size, head_dim] and one scale for each
- * (page, head), held as its exponent: code s (a byte, 0..254) stands for 2^(s - 127), and a cached value is its code
- * times its page's scale.  Strides are in elements, of dimensions page, head and token (codes; the last dimension is
+ * (page, head), held as its exponent: code s (a byte, 1..247; tt_paged_write makes 27..247) stands for 2^(s - 127), and a
+ * cached value is its code times its page's scale.  Strides are in elements, of dimensions page, head and token (codes; the last dimension is
  * contiguous) and page and head (scales).  A sequence's tokens lie in the pages its row of the block table names:
  * position p in page table[p / page_size], row p % page_size.
- * All strides must be >= 0; num_pages, heads, page_size, head_dim >= 1, num_pages * page_size < 2^31. */
+ * All strides must be >= 0; num_pages, heads, page_size, head_dim >= 1, num_pages * page_size < 2^31, page_size * head_dim < 2^31. */
 typedef struct tt_paged_cache {
   void *k, *v;
   void *k_scale, *v_scale;

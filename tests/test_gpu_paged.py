@@ -5,6 +5,8 @@ most (D + 4) u reach, a probability by the relative ln 2 times that, one exp2 (2
 numerator and denominator; the weights and the output are rounded to 11 or 8 bits at half a step each.  A V scale of code
 e enters as score + (e - 121), one more rounding of a sum of magnitude reach + |e - 121|, and leaves the same way in the
 log-sum-exp (codes here are within 54 of 121)."""
+import ctypes
+
 import numpy as np
 import pytest
 import torch
@@ -683,3 +685,11 @@ def test_tables_of_nearly_31_bits(P, width, B, n, kernel):
     assert f"_{kernel}_" in rt.last_kernel_name()
     want = orc.attention(q.double().numpy(), codes[0], codes[1], scales[0], scales[1], narrow, lens, cu, 0.09, True)
     compare(o, lse, want, max(lens), 128, torch.bfloat16)
+
+
+def test_a_page_of_more_elements_than_31_bits_is_refused():
+    n = ctypes.c_size_t()
+    c = rt.pack_paged_cache(1, 1, 1, 1, *([0] * 10), 1, 1, 2**25, 64)
+    assert rt.load().tt_paged_attn_workspace(1, 1, 1, 1, 1, c, ctypes.byref(n)) == rt.RT_ERR_UNSUPPORTED
+    c = rt.pack_paged_cache(1, 1, 1, 1, *([0] * 10), 1, 1, 2**25 - 1, 64)
+    assert rt.load().tt_paged_attn_workspace(1, 1, 1, 1, 1, c, ctypes.byref(n)) == rt.RT_OK

@@ -19,6 +19,8 @@ int check_cache(const char *who, const tt_paged_cache *c, PagedCacheArgs *out) {
                 c->page_size, c->head_dim);
   if ((int64_t)c->num_pages * c->page_size > INT32_MAX)
     return fail(RT_ERR_UNSUPPORTED, "%s: num_pages * page_size exceeds int32", who);
+  if ((int64_t)c->page_size * c->head_dim > INT32_MAX)
+    return fail(RT_ERR_UNSUPPORTED, "%s: page_size * head_dim exceeds int32", who);
   if (c->head_dim > 256) return fail(RT_ERR_UNSUPPORTED, "%s: head dim %d (at most 256)", who, c->head_dim);
   for (int i = 0; i < 3; ++i)
     if (c->k_strides[i] < 0 || c->v_strides[i] < 0) return fail(RT_ERR_INVALID, "%s: negative cache stride", who);
