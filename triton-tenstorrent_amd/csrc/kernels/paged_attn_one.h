@@ -17,9 +17,8 @@
 //
 // Split: a group of workgroups, one for each cache head, takes an even share of the keys of all sequences, in units of
 // 64 * NS keys, whatever the lengths.  (All heads of a page are read at about the same time, by neighbouring workgroups:
-// their codes lie side by side.)  A workgroup meets at most two sequences that it
-// does not have whole, the first and the last.  Those leave partial results (fp32 sum, reference, sum of probabilities)
-// in the workspace and paged_attn_join adds them in order, so results do not change from run to run.  While a sequence's
+// their codes lie side by side.)  A workgroup meets at most two sequences that it does not have whole, the first and the
+// last.  Those leave partial results (fp32 sum, reference, sum of probabilities) in the workspace and paged_attn_join adds them in order, so results do not change from run to run.  While a sequence's
 // four wavefronts are merged, the next one's first loads are under way.
 #pragma once
 
@@ -132,10 +131,6 @@ struct Hf {
 template <int D, typename T> __device__ __forceinline__ T stream(const T *p) {
   if constexpr (D >= 128) return __builtin_nontemporal_load(p);
   return *p;
-}
-__device__ __forceinline__ int64_t uniform64(int64_t v) {
-  return (int64_t)(((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32) |
-                   (uint32_t)__builtin_amdgcn_readfirstlane((int)v));
 }
 __device__ __forceinline__ int64_t lane64(int32_t lo, int32_t hi, int lane) {
   return (int64_t)(((uint64_t)(uint32_t)__builtin_amdgcn_readlane(hi, lane) << 32) | (uint32_t)__builtin_amdgcn_readlane(lo, lane));
@@ -495,9 +490,8 @@ __device__ __forceinline__ void body(const PagedAttnArgs &a, float *lds, int wg,
   if (a.part && !noted && tid == 0) split->q0 = -1;
 }
 
-// Adds the parts of the split sequence that workgroup wg of the launch before noted, if any: one of
-// `join_pieces` pieces of its rows.  D / 4 threads a row; what
-// is left of the 256 takes several rows or several parts at once.
+// Adds the parts of the split sequence that workgroup wg of the launch before noted, if any: one of `join_pieces` pieces
+// of its rows.  D / 4 threads a row; what is left of the 256 takes several rows or several parts at once.
 template <class E, int D, int MT> __device__ __forceinline__ void join(const PagedAttnArgs &a, f32x4 *lds, int wg, int piece, int wgs) {
   constexpr int TPR = D / 4, SLOTS = 256 / TPR, PF = part_floats<D, MT>();
   const Split sp = ((const Split *)(a.part + 2 * (int64_t)wgs * PF))[wg];
@@ -571,15 +565,15 @@ template <int D, int MT> constexpr int lds_floats() { return 4 * 16 * MT * (D + 
 #define PAGED_ONE(T, E, D, MT, OCC)                                                                           \
   extern "C" __global__ __launch_bounds__(256, OCC) void paged_attn_one_##T##_d##D##_r##MT(PagedAttnArgs a) {  \
     __shared__ __align__(16) float lds[one::lds_floats<D, MT>()];                                             \
-    one::body<one::E, D, MT, false>(a, lds, blockIdx.x, gridDim.x);                                                                  \
+    one::body<one::E, D, MT, false>(a, lds, blockIdx.x, gridDim.x);                                           \
   }                                                                                                           \
   extern "C" __global__ __launch_bounds__(256, 2) void paged_attn_few_##T##_d##D##_r##MT(PagedAttnArgs a) {    \
     __shared__ __align__(16) float lds[one::lds_floats<D, MT>()];                                             \
-    one::body<one::E, D, MT, true>(a, lds, blockIdx.x, gridDim.x);                                                                   \
+    one::body<one::E, D, MT, true>(a, lds, blockIdx.x, gridDim.x);                                            \
   }                                                                                                           \
   extern "C" __global__ __launch_bounds__(256) void paged_attn_join_##T##_d##D##_r##MT(PagedAttnArgs a) {      \
     __shared__ one::f32x4 lds[256 + 128];                                                                     \
-    one::join<one::E, D, MT>(a, lds, blockIdx.x / a.join_pieces, blockIdx.x % a.join_pieces, gridDim.x / a.join_pieces);                                                                         \
+    one::join<one::E, D, MT>(a, lds, blockIdx.x / a.join_pieces, blockIdx.x % a.join_pieces, gridDim.x / a.join_pieces); \
   }
 // (the last number: workgroups of paged_attn_one on a CU, which the host's grid counts on too; paged_attn_few has two)
 PAGED_ONE(bf16, Bf, 64, 1, 3)

@@ -187,318 +187,318 @@ __device__ __forceinline__ void body(const PagedAttnArgs &a, uint8_t *lds, int w
   bool noted = false;
 
   for (;;) {
-  const int R = sq.n * a.group, row0 = tile * kRows;
-  const int nsteps = steps_of(a, sq, tile);
-  const int k_lo = a.rows_whole ? 0 : u - before, k_hi = a.rows_whole ? nsteps : min(nsteps, k_lo + (u_end - u));
+    const int R = sq.n * a.group, row0 = tile * kRows;
+    const int nsteps = steps_of(a, sq, tile);
+    const int k_lo = a.rows_whole ? 0 : u - before, k_hi = a.rows_whole ? nsteps : min(nsteps, k_lo + (u_end - u));
 
-  const int row = row0 + wave * 32 + c32;
-  const int qi = min(row, R - 1) / a.group, qg = min(row, R - 1) % a.group;
-  const int64_t t = sq.q0 + qi;
-  const int hq = hk * a.group + qg;
-  const int32_t limit = last_key(a, sq, qi);
-  const bool alive = row0 + wave * 32 < R;  // the wavefront has rows
-  // keys that all rows of the workgroup attend end here; the wavefront's own rows see nothing from `wave_end` on
-  const int32_t all_to = last_key(a, sq, row0 / a.group);
-  const int32_t wave_last = __builtin_amdgcn_readfirstlane(last_key(a, sq, min(row0 + wave * 32 + 31, R - 1) / a.group));
+    const int row = row0 + wave * 32 + c32;
+    const int qi = min(row, R - 1) / a.group, qg = min(row, R - 1) % a.group;
+    const int64_t t = sq.q0 + qi;
+    const int hq = hk * a.group + qg;
+    const int32_t limit = last_key(a, sq, qi);
+    const bool alive = row0 + wave * 32 < R;  // the wavefront has rows
+    // keys that all rows of the workgroup attend end here; the wavefront's own rows see nothing from `wave_end` on
+    const int32_t all_to = last_key(a, sq, row0 / a.group);
+    const int32_t wave_last = __builtin_amdgcn_readfirstlane(last_key(a, sq, min(row0 + wave * 32 + 31, R - 1) / a.group));
 
-  typename E::frag qf[DK];
-  {
-    const uint16_t *qr = a.q + t * a.q_tok + hq * a.q_head + hi * 8;
-#pragma unroll
-    for (int s = 0; s < DK; ++s) // (a negative scale's sign goes into q: factors of scores are positive below)
-      qf[s] = __builtin_bit_cast(typename E::frag, *(const u32x4 *)(qr + s * 16) ^ (a.qk_scale < 0.0f ? 0x80008000u : 0u));
-  }
-  f32x16 acc[DT];
-#pragma unroll
-  for (int i = 0; i < DT; ++i) acc[i] = (f32x16){0};
-  float mref = -kInf, lsum = 0.0f;
-
-  const int32_t *table = a.table + (int64_t)b * a.table_stride;
-  const uint8_t *kh = a.c.k + hk * a.c.k_head, *vh = a.c.v + hk * a.c.v_head;
-  // staging: K row tid / 4 of the tile, KB codes from column (tid % 4) * KB; V keys 4 (tid / 16) .. + 3, VB codes from
-  // column (tid % 16) * VB.  Both lie in the wavefront's 16 keys.
-  const uint32_t kvo = (uint32_t)(((tid >> 2) & 15) * a.c.k_tok + (tid & 3) * KB);
-  uint32_t vvo[4];
-#pragma unroll
-  for (int r = 0; r < 4; ++r) vvo[r] = (uint32_t)(((((tid >> 4) & 3) * 4 + r)) * a.c.v_tok + (tid & 15) * VB);
-
-  // What lane (k % 16) * 4 + s knows of subtile s of step k (16 steps at a time).
-  int32_t ko_lo, ko_hi, vo_lo, vo_hi, live, vcode;
-  float kscale;
-  auto batch = [&](int k0) {
-    const int64_t key = (int64_t)(k0 + (lane >> 2)) * 64 + (lane & 3) * 16;
-    const uint32_t sub = (uint32_t)(key >> 4);
-    const uint32_t blk = (uint32_t)(((uint64_t)sub * a.page_magic) >> 36);
-    int32_t page = key < sq.len ? table[blk] : -1;
-    const bool ok = page >= 0 && page < a.c.pages;
-    page = ok ? page : 0;
-    const int64_t prow = ok ? ((int64_t)sub - (int64_t)blk * (a.c.page_size >> 4)) * 16 : 0;
-    const int64_t ko = page * a.c.k_page + prow * a.c.k_tok, vo = page * a.c.v_page + prow * a.c.v_tok;
-    ko_lo = (int32_t)ko; ko_hi = (int32_t)(ko >> 32); vo_lo = (int32_t)vo; vo_hi = (int32_t)(vo >> 32);
-    live = ok ? (int32_t)min((int64_t)sq.len - key, (int64_t)16) : 0;
-    kscale = pow2_code(a.c.ks[page * a.c.ks_page + hk * a.c.ks_head]) * fabsf(a.qk_scale);
-    vcode = ok ? a.c.vs[page * a.c.vs_page + hk * a.c.vs_head] : 0;
-  };
-  u32x4 kr[KW];
-  uint32_t vr[4][VW];
-  int staged_at, staged_nv; // of the codes in kr and vr: the lane that knows the tile's first subtile, the wavefront's live keys
-  auto load = [&](int k, int k_first) {
-    const int at = ((k - k_first) & 15) * 4;
-    if (((k - k_first) & 15) == 0) batch(k);
-    staged_at = at;
-    staged_nv = __builtin_amdgcn_readlane(live, at + wave);
-    const uint8_t *kp = kh + one::lane64(ko_lo, ko_hi, at + wave), *vp = vh + one::lane64(vo_lo, vo_hi, at + wave);
-#pragma unroll
-    for (int i = 0; i < KW; ++i) kr[i] = *(const u32x4 *)(kp + kvo + i * 16);
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      if constexpr (VW == 1) vr[r][0] = *(const uint32_t *)(vp + vvo[r]);
-      if constexpr (VW == 2) {
-        const u32x2 x = *(const u32x2 *)(vp + vvo[r]);
-        vr[r][0] = x[0]; vr[r][1] = x[1];
-      }
-      if constexpr (VW == 4) {
-        const u32x4 x = *(const u32x4 *)(vp + vvo[r]);
-        vr[r][0] = x[0]; vr[r][1] = x[1]; vr[r][2] = x[2]; vr[r][3] = x[3];
-      }
+    typename E::frag qf[DK];
+    {
+      const uint16_t *qr = a.q + t * a.q_tok + hq * a.q_head + hi * 8;
+  #pragma unroll
+      for (int s = 0; s < DK; ++s) // (a negative scale's sign goes into q: factors of scores are positive below)
+        qf[s] = __builtin_bit_cast(typename E::frag, *(const u32x4 *)(qr + s * 16) ^ (a.qk_scale < 0.0f ? 0x80008000u : 0u));
     }
-  };
-  // LDS addresses.  16-byte chunk c of K row r lies at c ^ (r / (256 / KROW) & KMASK), chunk c of V^T row d at
-  // c ^ swz(d), which spreads what one instruction touches over the banks; a tile begins on 512 bytes, so that every
-  // address below is one of four lane constants ^ a compile-time constant + another.
-  auto swz = [](int d) { return ((d >> 1) ^ (d >> 4)) & 7; };
-  const uint32_t k_rd = c32 * KROW + ((hi ^ ((c32 >> KSH) & KMASK)) << 4);
-  const uint32_t v_rd = VOFF + c32 * 128 + ((hi ^ swz(c32)) << 4);
-  const uint32_t k_wr = (tid >> 2) * KROW + ((((tid & 3) * (KB / 8)) ^ (((tid >> 2) >> KSH) & KMASK)) << 4);
-  const uint32_t v_wr = VOFF + (tid & 15) * VB * 128 + (((wave * 2 + ((tid >> 4) & 1)) ^ swz((tid & 15) * VB)) << 4) + ((tid >> 5) & 1) * 8;
-  // codes in registers -> tile in LDS.  `edge`: some row does not attend some of these keys, so a NaN in V must be told
-  // from the others' results (found here, handled by the readers).
-  auto store = [&](uint32_t buf, bool edge) {
-    // (the batch still is the one these codes came from: load() of a later tile comes after)
-    if (wave == 0 && (uint32_t)(lane - staged_at) < 4) {
-      float *m = (float *)(lds + buf + FOFF) + (lane - staged_at);
-      m[0] = fmaxf(kscale, 1e-37f); // (not 0: a masked score times it has to stay -inf)
-      m[4] = (float)(vcode - kBase);
-      m[8] = unweight(vcode);
-      ((int32_t *)m)[12] = live;
-    }
-    const uint32_t kw = buf + k_wr, vw = buf + v_wr;
-#pragma unroll
-    for (int i = 0; i < KW; ++i)
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-        *(u32x4 *)(lds + (kw ^ ((i * 2 + h) << 4))) = __builtin_bit_cast(u32x4, E::codes(kr[i][2 * h], kr[i][2 * h + 1]));
-    const int nv = staged_nv;
-    const int mm = (tid >> 4) & 3; // 4-key group of the 16
-    if (nv < 16) {
-#pragma unroll
-      for (int r = 0; r < 4; ++r)
-#pragma unroll
-        for (int w = 0; w < VW; ++w) vr[r][w] = mm * 4 + r < nv ? vr[r][w] : 0;
-    }
-    if (edge) {
-      uint32_t nan[4][VW], any = 0;
-#pragma unroll
-      for (int r = 0; r < 4; ++r)
-#pragma unroll
-        for (int w = 0; w < VW; ++w) {
-          nan[r][w] = ((vr[r][w] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
-          any |= nan[r][w];
+    f32x16 acc[DT];
+  #pragma unroll
+    for (int i = 0; i < DT; ++i) acc[i] = (f32x16){0};
+    float mref = -kInf, lsum = 0.0f;
+
+    const int32_t *table = a.table + (int64_t)b * a.table_stride;
+    const uint8_t *kh = a.c.k + hk * a.c.k_head, *vh = a.c.v + hk * a.c.v_head;
+    // staging: K row tid / 4 of the tile, KB codes from column (tid % 4) * KB; V keys 4 (tid / 16) .. + 3, VB codes from
+    // column (tid % 16) * VB.  Both lie in the wavefront's 16 keys.
+    const uint32_t kvo = (uint32_t)(((tid >> 2) & 15) * a.c.k_tok + (tid & 3) * KB);
+    uint32_t vvo[4];
+  #pragma unroll
+    for (int r = 0; r < 4; ++r) vvo[r] = (uint32_t)(((((tid >> 4) & 3) * 4 + r)) * a.c.v_tok + (tid & 15) * VB);
+
+    // What lane (k % 16) * 4 + s knows of subtile s of step k (16 steps at a time).
+    int32_t ko_lo, ko_hi, vo_lo, vo_hi, live, vcode;
+    float kscale;
+    auto batch = [&](int k0) {
+      const int64_t key = (int64_t)(k0 + (lane >> 2)) * 64 + (lane & 3) * 16;
+      const uint32_t sub = (uint32_t)(key >> 4);
+      const uint32_t blk = (uint32_t)(((uint64_t)sub * a.page_magic) >> 36);
+      int32_t page = key < sq.len ? table[blk] : -1;
+      const bool ok = page >= 0 && page < a.c.pages;
+      page = ok ? page : 0;
+      const int64_t prow = ok ? ((int64_t)sub - (int64_t)blk * (a.c.page_size >> 4)) * 16 : 0;
+      const int64_t ko = page * a.c.k_page + prow * a.c.k_tok, vo = page * a.c.v_page + prow * a.c.v_tok;
+      ko_lo = (int32_t)ko; ko_hi = (int32_t)(ko >> 32); vo_lo = (int32_t)vo; vo_hi = (int32_t)(vo >> 32);
+      live = ok ? (int32_t)min((int64_t)sq.len - key, (int64_t)16) : 0;
+      kscale = pow2_code(a.c.ks[page * a.c.ks_page + hk * a.c.ks_head]) * fabsf(a.qk_scale);
+      vcode = ok ? a.c.vs[page * a.c.vs_page + hk * a.c.vs_head] : 0;
+    };
+    u32x4 kr[KW];
+    uint32_t vr[4][VW];
+    int staged_at, staged_nv; // of the codes in kr and vr: the lane that knows the tile's first subtile, the wavefront's live keys
+    auto load = [&](int k, int k_first) {
+      const int at = ((k - k_first) & 15) * 4;
+      if (((k - k_first) & 15) == 0) batch(k);
+      staged_at = at;
+      staged_nv = __builtin_amdgcn_readlane(live, at + wave);
+      const uint8_t *kp = kh + one::lane64(ko_lo, ko_hi, at + wave), *vp = vh + one::lane64(vo_lo, vo_hi, at + wave);
+  #pragma unroll
+      for (int i = 0; i < KW; ++i) kr[i] = *(const u32x4 *)(kp + kvo + i * 16);
+  #pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        if constexpr (VW == 1) vr[r][0] = *(const uint32_t *)(vp + vvo[r]);
+        if constexpr (VW == 2) {
+          const u32x2 x = *(const u32x2 *)(vp + vvo[r]);
+          vr[r][0] = x[0]; vr[r][1] = x[1];
         }
-      const bool found = __any(any != 0);
-      if (lane == 0) *(int32_t *)(lds + buf + FOFF + 64 + wave * 4) = found;
-      if (found) {
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          uint32_t bits = 0;
-#pragma unroll
-          for (int w = 0; w < VW; ++w) {
-            // bits 7, 15, 23, 31 -> 0 .. 3
-            bits |= (((nan[r][w] >> 7) * 0x00204081u) >> 21 & 15u) << (w * 4);
-            vr[r][w] &= ~((nan[r][w] >> 7) * 0xffu);
-          }
-          ((uint16_t *)(lds + buf + FOFF + kMeta))[(wave * 16 + mm * 4 + r) * 16 + (tid & 15)] = (uint16_t)bits;
+        if constexpr (VW == 4) {
+          const u32x4 x = *(const u32x4 *)(vp + vvo[r]);
+          vr[r][0] = x[0]; vr[r][1] = x[1]; vr[r][2] = x[2]; vr[r][3] = x[3];
         }
       }
-    }
-#pragma unroll
-    for (int w = 0; w < VW; ++w) {
-      const uint32_t x0 = __builtin_amdgcn_perm(vr[1][w], vr[0][w], 0x05010400), x1 = __builtin_amdgcn_perm(vr[3][w], vr[2][w], 0x05010400);
-      const uint32_t y0 = __builtin_amdgcn_perm(vr[1][w], vr[0][w], 0x07030602), y1 = __builtin_amdgcn_perm(vr[3][w], vr[2][w], 0x07030602);
-      const u32x2 f[4] = {{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x0, 1.0f, false)),
-                           __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x1, 1.0f, false))},
-                          {__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x0, 1.0f, true)),
-                           __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x1, 1.0f, true))},
-                          {__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(y0, 1.0f, false)),
-                           __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(y1, 1.0f, false))},
-                          {__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(y0, 1.0f, true)),
-                           __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(y1, 1.0f, true))}};
-#pragma unroll
-      for (int i = 0; i < 4; ++i) *(u32x2 *)(lds + (vw ^ (((w * 4 + i) >> 1) << 4)) + (w * 4 + i) * 128) = f[i];
-    }
-  };
-  auto edge_of = [&](int k) { return k * 64 + 63 > all_to; };
-
-  if (k_lo < k_hi) {
-    load(k_lo, k_lo);
-    store(0, edge_of(k_lo));
-  }
-  if (k_lo + 1 < k_hi) load(k_lo + 1, k_lo);
-  __syncthreads();
-  for (int k = k_lo; k < k_hi; ++k) {
-    const uint32_t buf = ((k - k_lo) & 1) * stage_bytes<D>(), next = stage_bytes<D>() - buf;
-    if (k + 1 < k_hi) {
-      store(next, edge_of(k + 1));
-      if (k + 2 < k_hi) load(k + 2, k_lo);
-    }
-    __builtin_amdgcn_sched_barrier(0);
-    if (alive && k * 64 <= wave_last) {
-      const uint32_t kb = buf + k_rd, vb = buf + v_rd;
-      f32x16 st[2] = {(f32x16){0}, (f32x16){0}};
-      // The order is pinned: left alone, the scheduler reads each fragment right before its product and waits for it.
-      // Four reads are on their way at any time.
-      u32x4 x[4];
-      auto k_frag = [&](int i) { return *(const u32x4 *)(lds + (kb ^ ((i >> 1) << 5)) + (i & 1) * 32 * KROW); };
-#pragma unroll
-      for (int i = 0; i < 4; ++i) x[i] = k_frag(i);
-#pragma unroll
-      for (int i = 0; i < 2 * DK; ++i) {
-        __builtin_amdgcn_sched_barrier(0);
-        st[i & 1] = E::mfma32(__builtin_bit_cast(typename E::frag, x[i & 3]), qf[i >> 1], st[i & 1]);
-        if (i + 4 < 2 * DK) x[i & 3] = k_frag(i + 4);
+    };
+    // LDS addresses.  16-byte chunk c of K row r lies at c ^ (r / (256 / KROW) & KMASK), chunk c of V^T row d at
+    // c ^ swz(d), which spreads what one instruction touches over the banks; a tile begins on 512 bytes, so that every
+    // address below is one of four lane constants ^ a compile-time constant + another.
+    auto swz = [](int d) { return ((d >> 1) ^ (d >> 4)) & 7; };
+    const uint32_t k_rd = c32 * KROW + ((hi ^ ((c32 >> KSH) & KMASK)) << 4);
+    const uint32_t v_rd = VOFF + c32 * 128 + ((hi ^ swz(c32)) << 4);
+    const uint32_t k_wr = (tid >> 2) * KROW + ((((tid & 3) * (KB / 8)) ^ (((tid >> 2) >> KSH) & KMASK)) << 4);
+    const uint32_t v_wr = VOFF + (tid & 15) * VB * 128 + (((wave * 2 + ((tid >> 4) & 1)) ^ swz((tid & 15) * VB)) << 4) + ((tid >> 5) & 1) * 8;
+    // codes in registers -> tile in LDS.  `edge`: some row does not attend some of these keys, so a NaN in V must be told
+    // from the others' results (found here, handled by the readers).
+    auto store = [&](uint32_t buf, bool edge) {
+      // (the batch still is the one these codes came from: load() of a later tile comes after)
+      if (wave == 0 && (uint32_t)(lane - staged_at) < 4) {
+        float *m = (float *)(lds + buf + FOFF) + (lane - staged_at);
+        m[0] = fmaxf(kscale, 1e-37f); // (not 0: a masked score times it has to stay -inf)
+        m[4] = (float)(vcode - kBase);
+        m[8] = unweight(vcode);
+        ((int32_t *)m)[12] = live;
       }
-      __builtin_amdgcn_sched_barrier(0);
-      const f32x4 factor = *(const f32x4 *)(lds + buf + FOFF), offset = *(const f32x4 *)(lds + buf + FOFF + 16);
-      const f32x4 back = *(const f32x4 *)(lds + buf + FOFF + 32);
-      const bool edge = edge_of(k);
-      bool whole_tile = !edge;
-      if (!edge) { // (also where every row attends every key a page may be missing)
-        const u32x4 nv = *(const u32x4 *)(lds + buf + FOFF + 48);
-        whole_tile = __builtin_amdgcn_readfirstlane(nv[0] & nv[1] & nv[2] & nv[3]) == 16;
-      }
-      if (!whole_tile) {
-        const u32x4 nv = *(const u32x4 *)(lds + buf + FOFF + 48);
-#pragma unroll
-        for (int s = 0; s < 4; ++s) {
-          const int32_t rel = nv[s] ? limit - k * 64 - s * 16 - hi * 4 : -1; // (keys past the end are past the limit)
-#pragma unroll
-          for (int r = 0; r < 8; ++r) {
-            const float x = st[s >> 1][(s & 1) * 8 + r];
-            st[s >> 1][(s & 1) * 8 + r] = (r >> 2) * 8 + (r & 3) <= rel ? x : -kInf;
-          }
-        }
-      }
-      // x = score * factor + offset, whose maximum is that of the scores
-      float top = -kInf;
-#pragma unroll
-      for (int s = 0; s < 4; ++s) {
-        float m = st[s >> 1][(s & 1) * 8];
-#pragma unroll
-        for (int r = 1; r < 8; ++r) m = fmaxf(m, st[s >> 1][(s & 1) * 8 + r]);
-        top = fmaxf(top, fmaf(m, factor[s], offset[s]));
-      }
-      if (__any(top > mref + kLazy)) {
-        const float mn = fmaxf(mref, fmaxf(top, __shfl_xor(top, 32)));
-        const float al = mn == -kInf ? 1.0f : __builtin_amdgcn_exp2f(mref - mn);
-        mref = mn;
-        lsum *= al;
-#pragma unroll
-        for (int i = 0; i < DT; ++i)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) acc[i][r] *= al;
-      }
-      const float ref = (mref == -kInf ? 0.0f : mref) - kLift;
-      // weights of a subtile between the products of the one before, V fragments four reads ahead
-      f16x8 pf[4];
-      float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-      auto weights = [&](int s, int r0, int n) {
-        const float c = offset[s] - ref;
-#pragma unroll
-        for (int r = r0; r < r0 + n; ++r) {
-          const float w = __builtin_amdgcn_exp2f(fmaf(st[s >> 1][(s & 1) * 8 + r], factor[s], c));
-          sum[s] += w; // (the sum of probabilities has to be fp32's: the log-sum-exp is a result)
-          pf[s][r] = (_Float16)w;
-        }
-      };
-      auto v_frag = [&](int i) { return *(const u32x4 *)(lds + (vb ^ (((i / DT) ^ (i % DT & 3)) << 5)) + i % DT * 32 * 128); };
-#pragma unroll
-      for (int i = 0; i < 4; ++i) x[i] = v_frag(i);
-      weights(0, 0, 8);
-#pragma unroll
-      for (int i = 0; i < 4 * DT; ++i) {
-        __builtin_amdgcn_sched_barrier(0);
-        acc[i % DT] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, x[i & 3]), pf[i / DT], acc[i % DT], 0, 0, 0);
-        if (i + 4 < 4 * DT) x[i & 3] = v_frag(i + 4);
-        if (i < 3 * DT) weights(i / DT + 1, i % DT * (8 / DT), 8 / DT);
-      }
-      __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-      for (int s = 0; s < 4; ++s) lsum = fmaf(sum[s], back[s], lsum);
-      if (edge) { // NaN in V, taken out of the tile: it reaches the rows that attend its key
-        for (int s = 0; s < 4; ++s) {
-          if (!__builtin_amdgcn_readfirstlane(*(const int32_t *)(lds + buf + FOFF + 64 + s * 4))) continue;
-          for (int j = 0; j < 16; ++j) {
-            if (k * 64 + s * 16 + j > limit) continue;
-            const uint16_t *bits = (const uint16_t *)(lds + buf + FOFF + kMeta) + (s * 16 + j) * 16;
-#pragma unroll
-            for (int i = 0; i < DT; ++i)
-#pragma unroll
-              for (int r = 0; r < 16; ++r) {
-                const int d = i * 32 + (r >> 2) * 8 + hi * 4 + (r & 3);
-                if (bits[d / VB] >> (d % VB) & 1) acc[i][r] = __builtin_nanf("");
-              }
-          }
-        }
-      }
-    }
-    __syncthreads();
-  }
-
-  lsum += __shfl_xor(lsum, 32);
-  const bool cut = k_lo > 0 || k_hi < nsteps;
-  // (the first tile of this workgroup takes slot 0, a later one that is cut can only be its last: slot 1)
-  const int which = u == u_first ? 0 : 1;
-  if (alive && row < R) {
-    if (!cut) {
-      const bool none = lsum == 0.0f && mref == -kInf;
-      const float inv = none ? 0.0f : kOut / lsum;
-      uint16_t *op = a.o + t * a.o_tok + hq * a.o_head + hi * 4;
-#pragma unroll
-      for (int i = 0; i < DT; ++i)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          uint16_t x[4];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) x[j] = E::out(acc[i][r * 4 + j] * inv);
-          *(u32x2 *)(op + i * 32 + r * 8) = (u32x2){(uint32_t)x[0] | (uint32_t)x[1] << 16, (uint32_t)x[2] | (uint32_t)x[3] << 16};
-        }
-      if (a.lse && hi == 0) a.lse[t * a.heads_q + hq] = none ? -kInf : mref - kLift + __builtin_log2f(lsum);
-    } else {
-      float *p = a.rows_part + (2 * (int64_t)wg + which) * part_floats<D>();
-      const int lr = wave * 32 + c32;
-#pragma unroll
-      for (int i = 0; i < DT; ++i)
-#pragma unroll
+      const uint32_t kw = buf + k_wr, vw = buf + v_wr;
+  #pragma unroll
+      for (int i = 0; i < KW; ++i)
+  #pragma unroll
+        for (int h = 0; h < 2; ++h)
+          *(u32x4 *)(lds + (kw ^ ((i * 2 + h) << 4))) = __builtin_bit_cast(u32x4, E::codes(kr[i][2 * h], kr[i][2 * h + 1]));
+      const int nv = staged_nv;
+      const int mm = (tid >> 4) & 3; // 4-key group of the 16
+      if (nv < 16) {
+  #pragma unroll
         for (int r = 0; r < 4; ++r)
-          *(f32x4 *)(p + lr * D + i * 32 + r * 8 + hi * 4) = (f32x4){acc[i][r * 4], acc[i][r * 4 + 1], acc[i][r * 4 + 2], acc[i][r * 4 + 3]};
-      if (hi == 0) { p[kRows * D + lr * 2] = mref; p[kRows * D + lr * 2 + 1] = lsum; }
+  #pragma unroll
+          for (int w = 0; w < VW; ++w) vr[r][w] = mm * 4 + r < nv ? vr[r][w] : 0;
+      }
+      if (edge) {
+        uint32_t nan[4][VW], any = 0;
+  #pragma unroll
+        for (int r = 0; r < 4; ++r)
+  #pragma unroll
+          for (int w = 0; w < VW; ++w) {
+            nan[r][w] = ((vr[r][w] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+            any |= nan[r][w];
+          }
+        const bool found = __any(any != 0);
+        if (lane == 0) *(int32_t *)(lds + buf + FOFF + 64 + wave * 4) = found;
+        if (found) {
+  #pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            uint32_t bits = 0;
+  #pragma unroll
+            for (int w = 0; w < VW; ++w) {
+              // bits 7, 15, 23, 31 -> 0 .. 3
+              bits |= (((nan[r][w] >> 7) * 0x00204081u) >> 21 & 15u) << (w * 4);
+              vr[r][w] &= ~((nan[r][w] >> 7) * 0xffu);
+            }
+            ((uint16_t *)(lds + buf + FOFF + kMeta))[(wave * 16 + mm * 4 + r) * 16 + (tid & 15)] = (uint16_t)bits;
+          }
+        }
+      }
+  #pragma unroll
+      for (int w = 0; w < VW; ++w) {
+        const uint32_t x0 = __builtin_amdgcn_perm(vr[1][w], vr[0][w], 0x05010400), x1 = __builtin_amdgcn_perm(vr[3][w], vr[2][w], 0x05010400);
+        const uint32_t y0 = __builtin_amdgcn_perm(vr[1][w], vr[0][w], 0x07030602), y1 = __builtin_amdgcn_perm(vr[3][w], vr[2][w], 0x07030602);
+        const u32x2 f[4] = {{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x0, 1.0f, false)),
+                             __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x1, 1.0f, false))},
+                            {__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x0, 1.0f, true)),
+                             __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x1, 1.0f, true))},
+                            {__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(y0, 1.0f, false)),
+                             __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(y1, 1.0f, false))},
+                            {__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(y0, 1.0f, true)),
+                             __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(y1, 1.0f, true))}};
+  #pragma unroll
+        for (int i = 0; i < 4; ++i) *(u32x2 *)(lds + (vw ^ (((w * 4 + i) >> 1) << 4)) + (w * 4 + i) * 128) = f[i];
+      }
+    };
+    auto edge_of = [&](int k) { return k * 64 + 63 > all_to; };
+
+    if (k_lo < k_hi) {
+      load(k_lo, k_lo);
+      store(0, edge_of(k_lo));
     }
-  }
-  if (a.rows_whole) return;
-  if (cut && k_lo == 0) {
-    const int32_t last = before + nsteps - 1, larger = extra * (each + 1); // the tile's last step, and the group that has it
-    const int32_t owner = last < larger ? last / (each + 1) : extra + (last - larger) / each;
-    if (tid == 0) *split = {b, owner - group, which, tile};
-    noted = true;
-  }
-  u += k_hi - k_lo;
-  if (u >= u_end) break;
-  before += nsteps;
-  if (++tile == sq.tiles) {
-    tile = 0;
-    do sq = seq_of(a, ++b);
-    while (sq.tiles == 0); // (u is less than all units)
-  }
+    if (k_lo + 1 < k_hi) load(k_lo + 1, k_lo);
+    __syncthreads();
+    for (int k = k_lo; k < k_hi; ++k) {
+      const uint32_t buf = ((k - k_lo) & 1) * stage_bytes<D>(), next = stage_bytes<D>() - buf;
+      if (k + 1 < k_hi) {
+        store(next, edge_of(k + 1));
+        if (k + 2 < k_hi) load(k + 2, k_lo);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      if (alive && k * 64 <= wave_last) {
+        const uint32_t kb = buf + k_rd, vb = buf + v_rd;
+        f32x16 st[2] = {(f32x16){0}, (f32x16){0}};
+        // The order is pinned: left alone, the scheduler reads each fragment right before its product and waits for it.
+        // Four reads are on their way at any time.
+        u32x4 x[4];
+        auto k_frag = [&](int i) { return *(const u32x4 *)(lds + (kb ^ ((i >> 1) << 5)) + (i & 1) * 32 * KROW); };
+  #pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = k_frag(i);
+  #pragma unroll
+        for (int i = 0; i < 2 * DK; ++i) {
+          __builtin_amdgcn_sched_barrier(0);
+          st[i & 1] = E::mfma32(__builtin_bit_cast(typename E::frag, x[i & 3]), qf[i >> 1], st[i & 1]);
+          if (i + 4 < 2 * DK) x[i & 3] = k_frag(i + 4);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        const f32x4 factor = *(const f32x4 *)(lds + buf + FOFF), offset = *(const f32x4 *)(lds + buf + FOFF + 16);
+        const f32x4 back = *(const f32x4 *)(lds + buf + FOFF + 32);
+        const bool edge = edge_of(k);
+        bool whole_tile = !edge;
+        if (!edge) { // (also where every row attends every key a page may be missing)
+          const u32x4 nv = *(const u32x4 *)(lds + buf + FOFF + 48);
+          whole_tile = __builtin_amdgcn_readfirstlane(nv[0] & nv[1] & nv[2] & nv[3]) == 16;
+        }
+        if (!whole_tile) {
+          const u32x4 nv = *(const u32x4 *)(lds + buf + FOFF + 48);
+  #pragma unroll
+          for (int s = 0; s < 4; ++s) {
+            const int32_t rel = nv[s] ? limit - k * 64 - s * 16 - hi * 4 : -1; // (keys past the end are past the limit)
+  #pragma unroll
+            for (int r = 0; r < 8; ++r) {
+              const float x = st[s >> 1][(s & 1) * 8 + r];
+              st[s >> 1][(s & 1) * 8 + r] = (r >> 2) * 8 + (r & 3) <= rel ? x : -kInf;
+            }
+          }
+        }
+        // x = score * factor + offset, whose maximum is that of the scores
+        float top = -kInf;
+  #pragma unroll
+        for (int s = 0; s < 4; ++s) {
+          float m = st[s >> 1][(s & 1) * 8];
+  #pragma unroll
+          for (int r = 1; r < 8; ++r) m = fmaxf(m, st[s >> 1][(s & 1) * 8 + r]);
+          top = fmaxf(top, fmaf(m, factor[s], offset[s]));
+        }
+        if (__any(top > mref + kLazy)) {
+          const float mn = fmaxf(mref, fmaxf(top, __shfl_xor(top, 32)));
+          const float al = mn == -kInf ? 1.0f : __builtin_amdgcn_exp2f(mref - mn);
+          mref = mn;
+          lsum *= al;
+  #pragma unroll
+          for (int i = 0; i < DT; ++i)
+  #pragma unroll
+            for (int r = 0; r < 16; ++r) acc[i][r] *= al;
+        }
+        const float ref = (mref == -kInf ? 0.0f : mref) - kLift;
+        // weights of a subtile between the products of the one before, V fragments four reads ahead
+        f16x8 pf[4];
+        float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        auto weights = [&](int s, int r0, int n) {
+          const float c = offset[s] - ref;
+  #pragma unroll
+          for (int r = r0; r < r0 + n; ++r) {
+            const float w = __builtin_amdgcn_exp2f(fmaf(st[s >> 1][(s & 1) * 8 + r], factor[s], c));
+            sum[s] += w; // (the sum of probabilities has to be fp32's: the log-sum-exp is a result)
+            pf[s][r] = (_Float16)w;
+          }
+        };
+        auto v_frag = [&](int i) { return *(const u32x4 *)(lds + (vb ^ (((i / DT) ^ (i % DT & 3)) << 5)) + i % DT * 32 * 128); };
+  #pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = v_frag(i);
+        weights(0, 0, 8);
+  #pragma unroll
+        for (int i = 0; i < 4 * DT; ++i) {
+          __builtin_amdgcn_sched_barrier(0);
+          acc[i % DT] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, x[i & 3]), pf[i / DT], acc[i % DT], 0, 0, 0);
+          if (i + 4 < 4 * DT) x[i & 3] = v_frag(i + 4);
+          if (i < 3 * DT) weights(i / DT + 1, i % DT * (8 / DT), 8 / DT);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+  #pragma unroll
+        for (int s = 0; s < 4; ++s) lsum = fmaf(sum[s], back[s], lsum);
+        if (edge) { // NaN in V, taken out of the tile: it reaches the rows that attend its key
+          for (int s = 0; s < 4; ++s) {
+            if (!__builtin_amdgcn_readfirstlane(*(const int32_t *)(lds + buf + FOFF + 64 + s * 4))) continue;
+            for (int j = 0; j < 16; ++j) {
+              if (k * 64 + s * 16 + j > limit) continue;
+              const uint16_t *bits = (const uint16_t *)(lds + buf + FOFF + kMeta) + (s * 16 + j) * 16;
+  #pragma unroll
+              for (int i = 0; i < DT; ++i)
+  #pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                  const int d = i * 32 + (r >> 2) * 8 + hi * 4 + (r & 3);
+                  if (bits[d / VB] >> (d % VB) & 1) acc[i][r] = __builtin_nanf("");
+                }
+            }
+          }
+        }
+      }
+      __syncthreads();
+    }
+
+    lsum += __shfl_xor(lsum, 32);
+    const bool cut = k_lo > 0 || k_hi < nsteps;
+    // (the first tile of this workgroup takes slot 0, a later one that is cut can only be its last: slot 1)
+    const int which = u == u_first ? 0 : 1;
+    if (alive && row < R) {
+      if (!cut) {
+        const bool none = lsum == 0.0f && mref == -kInf;
+        const float inv = none ? 0.0f : kOut / lsum;
+        uint16_t *op = a.o + t * a.o_tok + hq * a.o_head + hi * 4;
+  #pragma unroll
+        for (int i = 0; i < DT; ++i)
+  #pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            uint16_t x[4];
+  #pragma unroll
+            for (int j = 0; j < 4; ++j) x[j] = E::out(acc[i][r * 4 + j] * inv);
+            *(u32x2 *)(op + i * 32 + r * 8) = (u32x2){(uint32_t)x[0] | (uint32_t)x[1] << 16, (uint32_t)x[2] | (uint32_t)x[3] << 16};
+          }
+        if (a.lse && hi == 0) a.lse[t * a.heads_q + hq] = none ? -kInf : mref - kLift + __builtin_log2f(lsum);
+      } else {
+        float *p = a.rows_part + (2 * (int64_t)wg + which) * part_floats<D>();
+        const int lr = wave * 32 + c32;
+  #pragma unroll
+        for (int i = 0; i < DT; ++i)
+  #pragma unroll
+          for (int r = 0; r < 4; ++r)
+            *(f32x4 *)(p + lr * D + i * 32 + r * 8 + hi * 4) = (f32x4){acc[i][r * 4], acc[i][r * 4 + 1], acc[i][r * 4 + 2], acc[i][r * 4 + 3]};
+        if (hi == 0) { p[kRows * D + lr * 2] = mref; p[kRows * D + lr * 2 + 1] = lsum; }
+      }
+    }
+    if (a.rows_whole) return;
+    if (cut && k_lo == 0) {
+      const int32_t last = before + nsteps - 1, larger = extra * (each + 1); // the tile's last step, and the group that has it
+      const int32_t owner = last < larger ? last / (each + 1) : extra + (last - larger) / each;
+      if (tid == 0) *split = {b, owner - group, which, tile};
+      noted = true;
+    }
+    u += k_hi - k_lo;
+    if (u >= u_end) break;
+    before += nsteps;
+    if (++tile == sq.tiles) {
+      tile = 0;
+      do sq = seq_of(a, ++b);
+      while (sq.tiles == 0); // (u is less than all units)
+    }
   }
   if (!noted && tid == 0) split->b = -1;
 }
