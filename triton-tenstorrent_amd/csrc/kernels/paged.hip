@@ -37,7 +37,8 @@ __device__ __forceinline__ int32_t clampi(int32_t v, int32_t lo, int32_t hi) { r
 } // namespace
 
 // Every workgroup scans all sequences (the lengths are a few KB that the L2 holds) and then does its share of the
-// tokens, so that no workgroup waits for another.  Thread i owns `per` consecutive sequences; two scans, the tokens'
+// tokens, so that no workgroup waits for another and one launch is enough: a few KB in and out, the time is that of
+// dependent loads and two scans (16 sequences 4.8 us; 1000 sequences, 142619 tokens 7.0 us).  Thread i owns `per` consecutive sequences; two scans, the tokens'
 // (saturating at max_tokens) and the pages'.  A new token at the start of a page writes that page's table entry.
 extern "C" __global__ __launch_bounds__(1024) void paged_plan(PagedPlanArgs a) {
   __shared__ uint32_t part[16];
@@ -224,7 +225,8 @@ template <typename E> __device__ __forceinline__ void write_any(const PagedWrite
 }
 
 // ---- head dims 64, 128, 256, 16-byte aligned rows ----
-// Bound: HBM, 2 bytes read and 1 written a value.  A lane takes 8 values (16 bytes in, 8 out), so a row is D / 8 lanes and
+// Bound: HBM, 2 bytes read and 1 written a value; measured 55 us for 38171 prompt tokens of 8 heads of 128 (235 MB, 4.3 TB/s
+// where a copy reaches 6.7), 3.6 us for 64 single tokens.  Six workgroups a CU: at eight the registers spill (62 us).  A lane takes 8 values (16 bytes in, 8 out), so a row is D / 8 lanes and
 // a wavefront step RPS rows.  A workgroup looks at `tile` tokens for one head of K or of V; its wavefronts share the runs
 // that begin there:
 //   - a run of several tokens is one wavefront's, a long one all four's, held in registers between the maximum and the
@@ -483,7 +485,8 @@ __device__ __forceinline__ int owner_of(const int32_t *cu, int b, int32_t t) {
 }
 
 // One wavefront per (row, query head): lane = key for the scores of 64 keys, lane = head dims lane, lane + 64, ... for
-// the sum over V.  Any page size, strides and head dim up to 256; everything in fp32.
+// the sum over V.  Any page size, strides and head dim up to 256; everything in fp32.  It runs only where the kernels below
+// do not (71 ms for 6 sequences of 20000 to 131000 keys that take them 0.14).
 template <typename E> __device__ __forceinline__ void attn_any(const PagedAttnArgs &a, float *qs, uint16_t (*to_out)(float)) {
   const int lane = threadIdx.x;
   const int t = blockIdx.x, hq = blockIdx.y, D = a.c.head_dim, P = a.c.page_size, hk = hq / a.group;

@@ -3,7 +3,8 @@
 //
 // What bounds it: one pass over the cached codes, HBM.  A wavefront owns all queries and query heads of one cache head
 // (row r is query r / group, head r % group; empty rows of the MFMA tile cost nothing here) and streams keys from global memory
-// into registers, with no LDS between: every code is used once, by one wavefront.
+// into registers (6 sequences of 20000 to 131000 keys, 8 heads of 128, 782 MB: 131 us, 6.0 TB/s where a copy reaches 6.7; 48 of
+// 60 to 8000 keys: 56 us, 5.7 TB/s; the join 5 us), with no LDS between: every code is used once, by one wavefront.
 //   S^T[key, r] = K . Q^T       v_mfma_f32_16x16x32, A = 16 rows of K, B = Q; lane l ends with row l%16, keys (l/16)*4+r
 //   O^T[d, r]  += V^T . P^T     B = P^T is what the lane already holds; A = V^T, whose lane needs 8 keys of one d: it loads
 //                               D/16 consecutive codes of each of its keys and pairs neighbouring keys' bytes with

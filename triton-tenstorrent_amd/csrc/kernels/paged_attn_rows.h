@@ -9,7 +9,10 @@
 // two tiles ahead, turned to 16 bits on the way into LDS, V transposed there (v_perm_b32 pairs neighbouring keys' bytes
 // before the conversion, as in paged_attn_one.h), K and V without their scales, which join the scores as there.  LDS
 // holds two tiles; one barrier a tile.
-// Bound: MFMA and the exponentials (32 v_exp_f32 a lane and tile against 32 MFMAs of 32 cycles), LDS reads behind them.
+// Bound: instruction issue.  7169 prompt tokens, 32 heads of 128 over 8: 250 us, 848 TFLOP/s (a large product reaches 1593); the
+// MFMA pipes are busy a third of the time, an instruction is issued in 82 % of the cycles (exponentials, conversions,
+// staging).  Two workgroups on a CU, so that one's softmax runs beside the other's products; one wavefront a SIMD with
+// twice the rows moves its accumulators between the register files (488 us).
 //
 // Split: with row tiles enough to fill the chip twice, a workgroup takes one, late rows (which attend most keys) first.
 // With fewer, a group of workgroups, one for each cache head, takes an even share of the steps of all row tiles, and
