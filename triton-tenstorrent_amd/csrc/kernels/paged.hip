@@ -342,6 +342,7 @@ template <typename E, int D> __device__ __forceinline__ void write_rows(const Pa
   uint64_t many = __ballot(leads && !single);
   const uint64_t ones = __ballot(single), rest = __ballot(goes_on);
 
+  int at = 8; // the half of `tops` that the last shared run used
   for (int turn = 0; many; ++turn, many &= many - 1) {
     const int src = __builtin_ctzll(many);
     const int64_t t = first + src;
@@ -359,6 +360,7 @@ template <typename E, int D> __device__ __forceinline__ void write_rows(const Pa
     // a short run is one wavefront's, a long one all four's
     const bool shared = n > HOLD * RPS;
     if (!shared && (turn & 3) != wave) continue;
+    at ^= shared ? 8 : 0;
     const int r0 = shared ? wave * HOLD * RPS : 0, stride = shared ? 4 * HOLD * RPS : HOLD * RPS;
     uint8_t *base = codes + page * c_page, *sp = scales + page * s_page;
     const uint16_t *xr = x + t * x_tok + col;
@@ -375,16 +377,18 @@ template <typename E, int D> __device__ __forceinline__ void write_rows(const Pa
 #pragma unroll
       for (int i = 0; i < HOLD; ++i) amax = max(amax, top_of8(hold[i]));
     }
-    auto over_run = [&](uint32_t m, int at) { // the maximum over all lanes that share the run
+    // the maximum over all lanes that share the run; where it is stored again, two shared runs later, every wavefront has
+    // read it (there is a barrier between), so none is needed behind the stores of codes, which would wait for them
+    auto over_run = [&](uint32_t m, int to) {
       m = max64(m);
       if (shared) {
-        if (lane == 0) tops[at + wave] = m;
+        if (lane == 0) tops[to + wave] = m;
         __syncthreads();
-        m = max(max(tops[at], tops[at + 1]), max(tops[at + 2], tops[at + 3]));
+        m = max(max(tops[to], tops[to + 1]), max(tops[to + 2], tops[to + 3]));
       }
       return (uint32_t)__builtin_amdgcn_readfirstlane((int)m);
     };
-    amax = over_run(amax, 0);
+    amax = over_run(amax, at);
     const bool wild = amax >= E::kInfinite;
     if (wild) {
       amax = 0;
@@ -392,7 +396,7 @@ template <typename E, int D> __device__ __forceinline__ void write_rows(const Pa
 #pragma unroll
         for (int i = 0; i < HOLD; ++i)
           if (b + i * RPS < n) amax = max(amax, finite_top_of8<E>(*(const w_u32x4 *)(xr + (b + i * RPS) * x_tok)));
-      amax = over_run(amax, 4);
+      amax = over_run(amax, at + 4);
     }
     const int need = scale_of_top<E>(amax), s = row ? max(need, __builtin_amdgcn_readfirstlane(old)) : need;
     if (row && s > old && (!shared || wave == 0)) rescale_rows<D>(base, c_tok, row, old, s);
@@ -405,8 +409,7 @@ template <typename E, int D> __device__ __forceinline__ void write_rows(const Pa
         *(w_u32x2 *)(base + (row + r) * c_tok + col) = codes_of8<E>(hold[i], s, wild);
       }
     }
-    if (shared) __syncthreads(); // (tops; and every wavefront has read the old scale)
-    if (lane == 0 && (!shared || wave == 0)) *sp = (uint8_t)s;
+    if (lane == 0 && (!shared || wave == 0)) *sp = (uint8_t)s; // (every wavefront has read the old one: over_run's barrier)
   }
 
   // single tokens: list[i] = the lane that found the i-th
@@ -454,7 +457,7 @@ template <typename E, int D> __device__ __forceinline__ void write_rows(const Pa
 #define PAGED_WRITE(T, E, D)                                                                          \
   extern "C" __global__ __launch_bounds__(256, 6) void paged_write_##T##_d##D(PagedWriteArgs a) {      \
     __shared__ uint8_t list[256];                                                                     \
-    __shared__ uint32_t tops[8];                                                                      \
+    __shared__ uint32_t tops[16];                                                                     \
     write_rows<E, D>(a, list, tops);                                                                     \
   }
 } // namespace
