@@ -169,10 +169,14 @@ __device__ __forceinline__ int scale_for(uint32_t amax) {
 __device__ __forceinline__ float pow2_code(int s) { return __builtin_bit_cast(float, (uint32_t)s << 23); }
 // saturating (an infinity becomes +-448), NaN stays NaN
 __device__ __forceinline__ float sat448(float y) { return y != y ? y : fminf(fmaxf(y, -448.0f), 448.0f); }
+// The maximum over the wavefront, in a scalar register: within the rows of 16 lanes, then across them.
 __device__ __forceinline__ uint32_t max64(uint32_t v) {
-#pragma unroll
-  for (int d = 32; d; d >>= 1) v = max(v, (uint32_t)__shfl_xor((int)v, d));
-  return v;
+  v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x111, 0xf, 0xf, false)); // row_shr:1
+  v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x112, 0xf, 0xf, false)); // row_shr:2
+  v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x114, 0xf, 0xf, false)); // row_shr:4
+  v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x118, 0xf, 0xf, false)); // row_shr:8
+  return max(max((uint32_t)__builtin_amdgcn_readlane((int)v, 15), (uint32_t)__builtin_amdgcn_readlane((int)v, 31)),
+             max((uint32_t)__builtin_amdgcn_readlane((int)v, 47), (uint32_t)__builtin_amdgcn_readlane((int)v, 63)));
 }
 
 // One wavefront writes the runs that begin among its `tile` tokens, for one head of K or of V.  A run is a stretch of
@@ -324,16 +328,19 @@ template <typename E, int D> __device__ __forceinline__ void write_rows(const Pa
   uint8_t *codes = isv ? a.c.v + head * a.c.v_head : a.c.k + head * a.c.k_head;
   uint8_t *scales = isv ? a.c.vs + head * a.c.vs_head : a.c.ks + head * a.c.ks_head;
   const int sub = lane / LPR, col = lane % LPR * 8;
+  // a lane's offset from the first row of a step, in bytes; what else an address needs is the same for all lanes
+  const uint32_t x_off = (uint32_t)(sub * (int32_t)x_tok + col) * 2, c_off = (uint32_t)(sub * (int32_t)c_tok + col);
 
   // the runs that begin in this tile: lane i looks at token first + i (every wavefront comes to the same answer)
   const int64_t tt = first + lane;
-  int32_t slot = -1;
+  int32_t slot = -1, in_page = 0, row_of = 0;
   bool leads = false, single = false, goes_on = false;
   if (lane < a.tile && tt < a.tokens) {
     slot = a.slots[tt];
     const int32_t prev = tt ? a.slots[tt - 1] : -1, next = tt + 1 < a.tokens ? a.slots[tt + 1] : -1;
     if (slot >= 0 && slot < nslots) {
-      const int r = slot % P;
+      in_page = (int32_t)((uint32_t)slot / (uint32_t)P);
+      const int r = row_of = slot - in_page * P;
       goes_on = r && tt && prev == slot - 1;
       leads = !goes_on;
       single = leads && !(r + 1 < P && next == slot + 1);
@@ -347,8 +354,8 @@ template <typename E, int D> __device__ __forceinline__ void write_rows(const Pa
     const int src = __builtin_ctzll(many);
     const int64_t t = first + src;
     const int32_t s0 = __builtin_amdgcn_readlane(slot, src);
-    const int row = s0 % P;
-    const int64_t page = s0 / P;
+    const int row = __builtin_amdgcn_readlane(row_of, src);
+    const int64_t page = __builtin_amdgcn_readlane(in_page, src);
     // the run's tokens: those that go on behind it, past the tile's end if it reaches that
     int n = 1 + (src == 63 ? 0 : __builtin_ctzll(~(rest >> (src + 1))));
     while (src + n >= a.tile) {
@@ -363,19 +370,27 @@ template <typename E, int D> __device__ __forceinline__ void write_rows(const Pa
     at ^= shared ? 8 : 0;
     const int r0 = shared ? wave * HOLD * RPS : 0, stride = shared ? 4 * HOLD * RPS : HOLD * RPS;
     uint8_t *base = codes + page * c_page, *sp = scales + page * s_page;
-    const uint16_t *xr = x + t * x_tok + col;
-    const int old = row ? *sp : 0;
-    w_u32x4 hold[HOLD];
-    uint32_t amax = 0;
-    for (int b = r0; b < n; b += stride) {
+    const uint8_t *xr = (const uint8_t *)(x + t * x_tok);
+    // Rows r .. of the run, RPS a step.  What lies past its end stands for its last rows again, which leaves the maximum as it is:
+    // branches around single loads had the compiler wait for three of them before the fourth (54.5 us instead of 48.4 for 38171 prompt tokens).
+    auto load4 = [&](int r) {
+      struct { w_u32x4 x[HOLD]; } h;
 #pragma unroll
       for (int i = 0; i < HOLD; ++i) {
-        const int r = b + i * RPS + sub;
-        hold[i] = (w_u32x4){0, 0, 0, 0};
-        if (r < n) hold[i] = *(const w_u32x4 *)(xr + r * x_tok);
+        const int at = min(r + i * RPS, n - 1);
+        h.x[i] = *(const w_u32x4 *)(xr + at * x_tok * 2 + (at + sub < n ? x_off : (uint32_t)col * 2));
       }
+      return h;
+    };
+    const int old = row ? *sp : 0;
+    const auto first4 = load4(r0);
+    uint32_t amax = 0;
 #pragma unroll
-      for (int i = 0; i < HOLD; ++i) amax = max(amax, top_of8(hold[i]));
+    for (int i = 0; i < HOLD; ++i) amax = max(amax, top_of8(first4.x[i]));
+    for (int b = r0 + stride; b < n; b += stride) {
+      const auto h = load4(b);
+#pragma unroll
+      for (int i = 0; i < HOLD; ++i) amax = max(amax, top_of8(h.x[i]));
     }
     // the maximum over all lanes that share the run; where it is stored again, two shared runs later, every wavefront has
     // read it (there is a barrier between), so none is needed behind the stores of codes, which would wait for them
@@ -392,22 +407,24 @@ template <typename E, int D> __device__ __forceinline__ void write_rows(const Pa
     const bool wild = amax >= E::kInfinite;
     if (wild) {
       amax = 0;
-      for (int b = r0 + sub; b < n; b += stride)
+      for (int b = r0; b < n; b += stride) {
+        const auto h = load4(b);
 #pragma unroll
-        for (int i = 0; i < HOLD; ++i)
-          if (b + i * RPS < n) amax = max(amax, finite_top_of8<E>(*(const w_u32x4 *)(xr + (b + i * RPS) * x_tok)));
+        for (int i = 0; i < HOLD; ++i) amax = max(amax, finite_top_of8<E>(h.x[i]));
+      }
       amax = over_run(amax, at + 4);
     }
     const int need = scale_of_top<E>(amax), s = row ? max(need, __builtin_amdgcn_readfirstlane(old)) : need;
     if (row && s > old && (!shared || wave == 0)) rescale_rows<D>(base, c_tok, row, old, s);
-    for (int b = r0; b < n; b += stride) {
+    auto store4 = [&](int r, const w_u32x4 *h) {
 #pragma unroll
-      for (int i = 0; i < HOLD; ++i) {
-        const int r = b + i * RPS + sub;
-        if (r >= n) continue;
-        if (n > stride) hold[i] = *(const w_u32x4 *)(xr + r * x_tok); // a run longer than the registers is read twice
-        *(w_u32x2 *)(base + (row + r) * c_tok + col) = codes_of8<E>(hold[i], s, wild);
-      }
+      for (int i = 0; i < HOLD; ++i)
+        if (r + i * RPS + sub < n) *(w_u32x2 *)(base + (row + r + i * RPS) * c_tok + c_off) = codes_of8<E>(h[i], s, wild);
+    };
+    store4(r0, first4.x);
+    for (int b = r0 + stride; b < n; b += stride) { // a run longer than the registers is read twice
+      const auto h = load4(b);
+      store4(b, h.x);
     }
     if (lane == 0 && (!shared || wave == 0)) *sp = (uint8_t)s; // (every wavefront has read the old one: over_run's barrier)
   }
@@ -419,9 +436,8 @@ template <typename E, int D> __device__ __forceinline__ void write_rows(const Pa
   for (int i0 = wave * RPS; i0 < count; i0 += 4 * RPS) {
     const bool mine = i0 + sub < count;
     const int src = mine ? list[wave * 64 + i0 + sub] : 0;
-    const int32_t s0 = __shfl(slot, src);
-    const int row = s0 % P;
-    const int64_t page = s0 / P;
+    const int row = __shfl(row_of, src);
+    const int64_t page = __shfl(in_page, src);
     uint8_t *base = codes + page * c_page, *sp = scales + page * s_page;
     w_u32x4 v = {0, 0, 0, 0};
     int old = 0;

@@ -169,7 +169,8 @@ extern "C" int tt_paged_write(const void *k, const void *v, const int64_t k_stri
   const PagedCacheArgs &c = a.c;
   const int D = c.head_dim;
   const bool al = aligned16(k) && aligned16(v) && (a.k_tok | a.k_head | a.v_tok | a.v_head) % 8 == 0 && aligned(c.k, 8) &&
-                  aligned(c.v, 8) && (c.k_page | c.k_head | c.k_tok | c.v_page | c.v_head | c.v_tok) % 8 == 0;
+                  aligned(c.v, 8) && (c.k_page | c.k_head | c.k_tok | c.v_page | c.v_head | c.v_tok) % 8 == 0 &&
+                  std::max({a.k_tok, a.v_tok, c.k_tok, c.v_tok}) < (1 << 26); // (offsets inside 8 rows fit 32 bits)
   char name[64];
   int64_t wgs;
   if (al && (D == 64 || D == 128 || D == 256)) {
