@@ -229,8 +229,9 @@ template <typename E> __device__ __forceinline__ void write_any(const PagedWrite
 }
 
 // ---- head dims 64, 128, 256, 16-byte aligned rows ----
-// Bound: HBM, 2 bytes read and 1 written a value; measured 55 us for 38171 prompt tokens of 8 heads of 128 (235 MB, 4.3 TB/s
-// where a copy reaches 6.7), 3.6 us for 64 single tokens.  Six workgroups a CU: at eight the registers spill (62 us).  A lane takes 8 values (16 bytes in, 8 out), so a row is D / 8 lanes and
+// Bound: HBM, 2 bytes read and 1 written a value; measured 48 us for 38171 prompt tokens of 8 heads of 128 (235 MB, 4.8 TB/s
+// where a copy reaches 6.7; the chain of slots, values and barrier costs as much as the memory), 3.5 us for 64 single
+// tokens.  Six workgroups a CU: at eight the registers spill.  A lane takes 8 values (16 bytes in, 8 out), so a row is D / 8 lanes and
 // a wavefront step RPS rows.  A workgroup looks at `tile` tokens for one head of K or of V; its wavefronts share the runs
 // that begin there:
 //   - a run of several tokens is one wavefront's, a long one all four's, held in registers between the maximum and the
