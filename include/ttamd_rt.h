@@ -361,7 +361,8 @@ TTAMD_API int tt_attn_fwd(float sm_scale, float *M, int32_t Z, int32_t H, const 
  * cached value is its code times its page's scale.  Strides are in elements, of dimensions page, head and token (codes; the last dimension is
  * contiguous) and page and head (scales).  A sequence's tokens lie in the pages its row of the block table names:
  * position p in page table[p / page_size], row p % page_size.
- * All strides must be >= 0; num_pages, heads, page_size, head_dim >= 1, num_pages * page_size < 2^31, page_size * head_dim < 2^31. */
+ * All strides must be >= 0; num_pages, heads, page_size, head_dim >= 1, num_pages * page_size < 2^31,
+ * page_size * head_dim <= 2^31 - 64. */
 typedef struct tt_paged_cache {
   void *k, *v;
   void *k_scale, *v_scale;

@@ -693,3 +693,12 @@ def test_a_page_of_more_elements_than_31_bits_is_refused():
     assert rt.load().tt_paged_attn_workspace(1, 1, 1, 1, 1, c, ctypes.byref(n)) == rt.RT_ERR_UNSUPPORTED
     c = rt.pack_paged_cache(1, 1, 1, 1, *([0] * 10), 1, 1, 2**25 - 1, 64)
     assert rt.load().tt_paged_attn_workspace(1, 1, 1, 1, 1, c, ctypes.byref(n)) == rt.RT_OK
+
+
+@pytest.mark.parametrize("P,D", [(34087042, 63), (2**31 // 33, 33), (2**31 // 7, 7), (2**31 - 63, 1)])
+def test_a_page_whose_last_step_of_64_elements_would_pass_31_bits_is_refused(P, D):
+    # P * D is one of the last 63 values below 2^31; the largest page size below those is taken
+    n = ctypes.c_size_t()
+    ask = lambda P: rt.init(0).tt_paged_attn_workspace(1, 1, 1, 1, 1, rt.pack_paged_cache(1, 1, 1, 1, *([0] * 10), 1, 1, P, D), ctypes.byref(n))
+    assert 2**31 - 64 < P * D < 2**31 and ask(P) == rt.RT_ERR_UNSUPPORTED
+    assert ask((2**31 - 64) // D) == rt.RT_OK

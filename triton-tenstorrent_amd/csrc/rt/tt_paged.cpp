@@ -19,8 +19,9 @@ int check_cache(const char *who, const tt_paged_cache *c, PagedCacheArgs *out) {
                 c->page_size, c->head_dim);
   if ((int64_t)c->num_pages * c->page_size > INT32_MAX)
     return fail(RT_ERR_UNSUPPORTED, "%s: num_pages * page_size exceeds int32", who);
-  if ((int64_t)c->page_size * c->head_dim > INT32_MAX)
-    return fail(RT_ERR_UNSUPPORTED, "%s: page_size * head_dim exceeds int32", who);
+  // paged_write_any steps a 32-bit index through a page's elements, 64 at a time: its last step has to fit too
+  if ((int64_t)c->page_size * c->head_dim > INT32_MAX - 63)
+    return fail(RT_ERR_UNSUPPORTED, "%s: page_size * head_dim exceeds 2^31 - 64", who);
   if (c->head_dim > 256) return fail(RT_ERR_UNSUPPORTED, "%s: head dim %d (at most 256)", who, c->head_dim);
   for (int i = 0; i < 3; ++i)
     if (c->k_strides[i] < 0 || c->v_strides[i] < 0) return fail(RT_ERR_INVALID, "%s: negative cache stride", who);
