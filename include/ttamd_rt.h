@@ -408,7 +408,8 @@ TTAMD_API int tt_paged_write(const void *k, const void *v, const int64_t k_strid
  * contiguous fp32) is the base-2 log-sum-exp of the scaled scores.  Rows outside every sequence are left as they are.
  * max_q is an upper bound of the queries of one sequence; the rows of a sequence that has more are undefined.
  * Scores, softmax and sums are fp32; the weights of V (probability times the page's scale, relative to the row's
- * largest) are rounded to fp16.  The V scales of the pages that one query attends may differ by up to 2^100.
+ * largest) are rounded to fp16, and kept in 16 bits (two bf16) where the V scales that meet differ by more than 2^12.
+ * The V scales of the pages that one query attends may differ by up to 2^100, pages of zeros aside.
  * workspace: tt_paged_attn_workspace(...) bytes, 16-byte aligned (null if that is 0), used by this call only until the
  * stream has run it: calls that may overlap need one each.  grid = (tokens, heads_q, 1). */
 TTAMD_API int tt_paged_attn_workspace(int32_t B, int32_t max_pages, int32_t tokens, int32_t heads_q, int32_t max_q,

@@ -702,3 +702,55 @@ def test_a_page_whose_last_step_of_64_elements_would_pass_31_bits_is_refused(P, 
     ask = lambda P: rt.init(0).tt_paged_attn_workspace(1, 1, 1, 1, 1, rt.pack_paged_cache(1, 1, 1, 1, *([0] * 10), 1, 1, P, D), ctypes.byref(n))
     assert 2**31 - 64 < P * D < 2**31 and ask(P) == rt.RT_ERR_UNSUPPORTED
     assert ask((2**31 - 64) // D) == rt.RT_OK
+
+
+def compare_far(o, lse, want, n, D, dtype, apart):
+    """As `compare` (a weight is off by at most 2^-11 of itself, so a channel by 2^-11 of its own sum), without that one's absolute
+    term: only fp16 results, which can be subnormal, have half a step of 2^-24.  V's exponents enter scores as offsets of magnitude up to `apart`."""
+    wo, wl, spread, reach = want
+    o, lse = o.cpu().double().numpy(), lse.cpu().double().numpy()
+    ds = (D + 5) * U * reach + (apart + 54) * U
+    rel = 2 * (np.log(2.0) * ds + 2 * U + n * U)
+    tol = spread * (2.0**-11 + rel[..., None]) + torch.finfo(dtype).eps / 2 * (np.abs(wo) + spread * 2.0**-10)
+    tol += 2.0**-25 if dtype is torch.float16 else 0.0
+    assert np.isfinite(wl).all() and (np.abs(o - wo) <= tol).all(), (np.abs(o - wo) / tol).max()
+    ltol = ds + (n + 4) * U / np.log(2.0) + 2 * U * np.abs(wl) + 64 * U
+    assert (np.abs(lse - wl) <= ltol).all(), (np.abs(lse - wl) / ltol).max()
+
+
+@pytest.mark.parametrize("n,Hq,H,D,kernel", [(1, 4, 2, 64, "one"), (1, 4, 2, 128, "one"), (1, 32, 1, 64, "one"), (1, 32, 1, 128, "one"),
+                                             (1, 2, 2, 256, "one"), (5, 4, 2, 64, "few"), (16, 4, 2, 128, "few"), (8, 4, 2, 256, "few"),
+                                             (30, 4, 2, 64, "rows"), (30, 8, 2, 128, "rows"), (30, 4, 2, 256, "rows"), (3, 4, 2, 40, "any")])
+@pytest.mark.parametrize("apart", [7, 12, 13, 20, 30, 60, 100])
+def test_channels_that_only_pages_of_a_small_scale_fill(n, Hq, H, D, kernel, apart):
+    # half of the channels are zeros in every page of the large scale: what the small pages hold there is the result
+    fp16 = apart <= 20
+    dtype, top = (torch.float16, 133) if fp16 else (torch.bfloat16, 160)
+    q, codes, scales, table, lens, cu = make([1100, 90], [n, n], Hq, H, 16, D, dtype, seed=apart + n, q_scale=0.5)
+    rng = np.random.default_rng(apart)
+    small = rng.random(scales[1].shape) < 0.5
+    small[table[1, 0]], small[table[1, 1]] = False, True
+    scales[1] = np.where(small, top - apart, top)
+    codes[1, :, :, :, :D // 2] = np.where(~small[..., None, None] & (codes[1, :, :, :, :D // 2] != 0x7F), 0, codes[1, :, :, :, :D // 2])
+    o, lse = K.paged_attention(q.cuda(), device_cache(codes, scales), i32(table), i32(lens), i32(cu), 0.09, max_q=n, return_lse=True)
+    assert f"_{kernel}_" in rt.last_kernel_name() or "_join_" in rt.last_kernel_name()
+    want = orc.attention(q.double().numpy(), codes[0], codes[1], scales[0], scales[1], table, lens, cu, 0.09, True)
+    compare_far(o, lse, want, 1100, D, dtype, apart)
+    assert (want[2][:, :, :D // 2] > 0).all()
+
+
+@pytest.mark.parametrize("n,Hq,H,D", [(1, 4, 2, 64), (1, 4, 2, 128), (1, 2, 2, 256), (5, 4, 2, 128), (30, 8, 2, 128), (30, 4, 2, 64), (3, 4, 2, 40)])
+@pytest.mark.parametrize("top", [127, 135, 160, 200])
+def test_pages_of_zeros_beside_any_others(n, Hq, H, D, top):
+    # a page of zeros has the smallest scale there is; its keys count in the sum of probabilities like any others
+    q, codes, scales, table, lens, cu = make([1100, 90, 40], [n, n, n], Hq, H, 16, D, torch.bfloat16, seed=top + n)
+    rng = np.random.default_rng(top)
+    zero = rng.random(scales[1].shape) < 0.5
+    zero[table[1, :3]] = True
+    zero[table[0, 20:60]] = True            # whole shares of a long sequence
+    zero[table[2, :3]] = True               # nothing but zeros
+    scales[1] = np.where(zero, orc.MIN_SCALE, top)
+    codes[1] = np.where(zero[..., None, None] & (codes[1] != 0x7F), 0, codes[1])
+    o, lse = K.paged_attention(q.cuda(), device_cache(codes, scales), i32(table), i32(lens), i32(cu), 0.09, max_q=n, return_lse=True)
+    want = orc.attention(q.double().numpy(), codes[0], codes[1], scales[0], scales[1], table, lens, cu, 0.09, True)
+    compare_far(o, lse, want, 1100, D, torch.bfloat16, top - orc.MIN_SCALE)

@@ -13,8 +13,11 @@
 // e4m3 -> 16 bits is v_cvt_scalef32_pk_{bf16,f16}_fp8 (exact), K and V without their scales.  K's joins the factor on the
 // scores.  V's, a power of two 2^(e - 127), joins the exponent: with x = score + e - 121 the weight w = 2^(x - ref) is what
 // a key contributes relative to the row's largest contribution, the sum over V takes w and the sum of probabilities
-// w 2^(121 - e).  So weights can be held in fp16 (11 bits where bf16 has 8) whatever the scales' range: fp16 flushes
-// below 2^-32 of the largest contribution.
+// w 2^(121 - e).  So weights can be held in fp16 (11 bits where bf16 has 8): fp16 keeps all 11 down to 2^-22 of the largest
+// contribution and nothing below 2^-32.  That is nothing beside it, but all that there is in a channel where the larger
+// pages hold zeros.  So a sequence whose V scales a workgroup finds more than 2^kSpan apart (pages of ordinary values never
+// are; within 2^12, 2^-21 are left) goes to a second pass, FAR: a weight is the sum of two bf16 there, which reach as far as
+// fp32 does and leave 2^-17, and costs two products.
 //
 // Split: a group of workgroups, one for each cache head, takes an even share of the keys of all sequences, in units of
 // 64 * NS keys, whatever the lengths.  (All heads of a page are read at about the same time, by neighbouring workgroups:
@@ -26,6 +29,7 @@
 namespace one {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
@@ -39,6 +43,33 @@ constexpr int kBase = 121;     // scale code that leaves x = score: that of a pa
 __device__ __forceinline__ float unweight(int e) { return __builtin_bit_cast(float, (uint32_t)max(kBase + 127 - e, 1) << 23); }
 constexpr float kOut = 0x1p-6f; // 2^(kBase - 127): V of scale code kBase
 constexpr float kInf = __builtin_inff();
+constexpr int kSpan = 12;      // see above
+
+// A sum of probabilities times 2^d, d <= 0 (-inf: 0).  (2^d by itself would end at 2^-126, and a page of zeros, whose keys count
+// like any others, can lie 2^220 below the largest page.)
+__device__ __forceinline__ float lower(float l, float d) {
+  d = fmaxf(d, -512.0f);
+  const float n = floorf(d);
+  return __builtin_amdgcn_ldexpf(l * __builtin_amdgcn_exp2f(d - n), (int)n);
+}
+// Sums l and k of references m and r, brought to ref, the larger of these, by the powers f and w; where a power is near the end
+// of fp32, by lower().  (A row of NaN scores has reference -inf and a NaN sum: it has to stay, f and w are 1 there.)
+__device__ __forceinline__ float add_sums(float l, float m, float f, float k, float r, float w, float ref) {
+  if (__builtin_expect((m < ref - 100.0f && m != -kInf) || (r < ref - 100.0f && r != -kInf), 0))
+    return (m == -kInf ? l : lower(l, m - ref)) + (r == -kInf ? k : lower(k, r - ref));
+  return l * f + k * w;
+}
+
+// The smallest and the largest of V's scales that a wavefront has met; the same in all its lanes.
+struct Span {
+  int32_t low, high;
+  __device__ __forceinline__ Span(int32_t l = 255, int32_t h = 0) : low(l), high(h) {}
+  __device__ __forceinline__ void meet(int32_t live, int32_t vcode) {
+    low = min(low, 255 - (int32_t)max64(live > 0 ? 255 - vcode : 0));
+    high = max(high, (int32_t)max64(live > 0 ? vcode : 0));
+  }
+  __device__ __forceinline__ bool far() const { return high > low + kSpan; }
+};
 
 // Subtiles of 16 keys that a wavefront takes in one step.  Two leave room for three workgroups on a CU at head dim 128
 // and make finer units than four (513 keys, 8 heads: 7.2 us against 9.3); at head dim 64 two would be too few bytes in flight.
@@ -60,8 +91,7 @@ template <int UK, int ROWS, bool FEW> struct Walk {
   int per;
   int32_t base, total;
   Seq own;
-  __device__ __forceinline__ Walk(const PagedAttnArgs &args) : a(args) {
-    const int lane = threadIdx.x & 63;
+  __device__ __forceinline__ Walk(const PagedAttnArgs &args, int lane) : a(args) {
     per = (a.b + 63) / 64;
     int32_t n = 0;
     own = {0, 0, 0, 0};
@@ -105,6 +135,7 @@ template <int UK, int ROWS, bool FEW> struct Walk {
 struct Bf {
   typedef bf16x8 frag;
   static __device__ __forceinline__ f32x4 mfma(frag x, frag y, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, y, c, 0, 0, 0); }
+  static __device__ __forceinline__ f32x16 mfma32(frag x, frag y, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, y, c, 0, 0, 0); }
   static __device__ __forceinline__ frag codes(uint32_t lo, uint32_t hi) {
     const u32x4 r = {__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, false)),
                      __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, true)),
@@ -112,11 +143,15 @@ struct Bf {
                      __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, true))};
     return __builtin_bit_cast(frag, r);
   }
+  template <bool HI> static __device__ __forceinline__ uint32_t codes2(uint32_t x) {
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x, 1.0f, HI));
+  }
   static __device__ __forceinline__ uint16_t out(float f) { return out_bf16(f); }
 };
 struct Hf {
   typedef f16x8 frag;
   static __device__ __forceinline__ f32x4 mfma(frag x, frag y, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(x, y, c, 0, 0, 0); }
+  static __device__ __forceinline__ f32x16 mfma32(frag x, frag y, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(x, y, c, 0, 0, 0); }
   static __device__ __forceinline__ frag codes(uint32_t lo, uint32_t hi) {
     const u32x4 r = {__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.0f, false)),
                      __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.0f, true)),
@@ -124,8 +159,14 @@ struct Hf {
                      __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.0f, true))};
     return __builtin_bit_cast(frag, r);
   }
+  template <bool HI> static __device__ __forceinline__ uint32_t codes2(uint32_t x) {
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x, 1.0f, HI));
+  }
   static __device__ __forceinline__ uint16_t out(float f) { return out_f16(f); }
 };
+// What V and its weights are held in
+template <bool FAR> struct Weights { typedef Hf type; };
+template <> struct Weights<true> { typedef Bf type; };
 
 // Codes are read once: non-temporal loads where a row is whole 128-byte lines (782 MB of cache, head dim 128: 140 -> 126 us;
 // head dim 64, whose lines two rows share: no gain).
@@ -137,6 +178,13 @@ __device__ __forceinline__ int64_t lane64(int32_t lo, int32_t hi, int lane) {
   return (int64_t)(((uint64_t)(uint32_t)__builtin_amdgcn_readlane(hi, lane) << 32) | (uint32_t)__builtin_amdgcn_readlane(lo, lane));
 }
 
+// The kernel's argument block as a function that is called (not inlined) gets at it, and its wavefront's own values.
+typedef __attribute__((address_space(3))) uint8_t *Lds;
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ __forceinline__ PagedAttnArgs args_at(uint64_t p) {
+  return *(const __attribute__((address_space(4))) PagedAttnArgs *)((uint64_t)(uint32_t)uniform((int)(p >> 32)) << 32 | (uint32_t)uniform((int)p));
+}
+
 // Partial result p of the workspace: rows * D sums, then rows pairs (reference, sum).
 template <int D, int MT> constexpr int part_floats() { return 16 * MT * D + 32 * MT; }
 
@@ -145,13 +193,15 @@ template <int D, int MT> constexpr int part_floats() { return 16 * MT * D + 32 *
 struct Split { int32_t q0, more, slot, rows; }; // q0: first packed row of its queries, -1 = none; rows: queries times group
 
 // FEW: sequences may have several queries; without it exactly one, and nothing below looks at a row's own limit.
-template <class E, int D, int MT, bool FEW>
-__device__ __forceinline__ void body(const PagedAttnArgs &a, float *lds, int wg, int wgs) {
+// Returns whether a sequence was left to FAR, which computes those and passes over the others.
+template <class E, int D, int MT, bool FEW, bool FAR>
+__device__ __forceinline__ bool body(const PagedAttnArgs &a, float *lds, int wg, int wgs, int tid) {
+  typedef typename Weights<FAR>::type W;
   constexpr int NS = subtiles<D, MT>(), UK = 64 * NS, KL = D / 64, VW = D / 64; // 16-byte loads of K, dwords of V per row
   constexpr int VB = D / 16, IB = 64 / NS, LD = D + 4;                      // LD: padded LDS row of the merge
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c16 = lane & 15, g = lane >> 4;
-  const Walk<UK, 16 * MT, FEW> walk(a);
+  const Walk<UK, 16 * MT, FEW> walk(a, lane);
   Split *split = (Split *)(a.part + 2 * (int64_t)wgs * part_floats<D, MT>()) + wg;
   const int hk = wg % a.c.heads, group = wg / a.c.heads;
   int32_t u, u_end, before;
@@ -161,14 +211,14 @@ __device__ __forceinline__ void body(const PagedAttnArgs &a, float *lds, int wg,
   if (a.whole) { // one sequence each
     b = group;
     sq = seq_of<UK, 16 * MT, FEW>(a, b);
-    if (sq.units == 0) return;
+    if (sq.units == 0) return false;
     before = u = 0;
     u_end = sq.units;
   } else {
     const int32_t groups = min(wgs / a.c.heads, walk.total); // fewer units than groups: one each
     if (group >= groups) {
-      if (a.part && tid == 0) split->q0 = -1;
-      return;
+      if (!FAR && a.part && tid == 0) split->q0 = -1;
+      return false;
     }
     each = walk.total / groups;
     extra = walk.total - each * groups;
@@ -177,7 +227,8 @@ __device__ __forceinline__ void body(const PagedAttnArgs &a, float *lds, int wg,
     b = walk.find(u, &before, &sq);
   }
   const int32_t u_first = u;
-  bool noted = false;
+  bool noted = false, again = false;
+  int32_t *spans = (int32_t *)(lds + 4 * 16 * MT * LD + 4 * 16 * MT * 2); // [wave]: low, high
   const uint8_t *kh = a.c.k + hk * a.c.k_head, *vh = a.c.v + hk * a.c.v_head;
 
   const uint32_t klane = (uint32_t)(c16 * a.c.k_tok + g * 16);
@@ -207,6 +258,21 @@ __device__ __forceinline__ void body(const PagedAttnArgs &a, float *lds, int wg,
     live = ok ? (int32_t)min((int64_t)sq.len - key, (int64_t)16) : 0;
     kscale = pow2_code(a.c.ks[page * a.c.ks_page + hk * a.c.ks_head]) * a.qk_scale;
     vcode = ok ? a.c.vs[page * a.c.vs_page + hk * a.c.vs_head] : 0;
+  };
+
+  // the whole workgroup's span is wide (behind a barrier)
+  auto far_spans = [&]() {
+    const int32_t low = min(min(spans[0], spans[2]), min(spans[4], spans[6])), high = max(max(spans[1], spans[3]), max(spans[5], spans[7]));
+    return high > low + kSpan;
+  };
+  auto put_span = [&](const Span &x) {
+    if (lane == 0) { spans[wave * 2] = x.low; spans[wave * 2 + 1] = x.high; }
+  };
+  // the wavefront's span, with the batch at hand (in LDS: nothing of it is held during the loop over keys)
+  auto widen_span = [&]() {
+    Span x(spans[wave * 2], spans[wave * 2 + 1]);
+    x.meet(live, vcode);
+    put_span(x);
   };
 
   u32x4 kr[NS][KL];
@@ -239,13 +305,28 @@ __device__ __forceinline__ void body(const PagedAttnArgs &a, float *lds, int wg,
   };
 
   // one set of registers each for K and V: a step's loads go out as soon as the step before has used them up
+  bool skip = false; // FAR: a sequence that the first pass has done
   auto open = [&]() {
     c0 = u - before;
     n = min(sq.units - c0, u_end - u);
     table = a.table + (int64_t)b * a.table_stride;
+    if constexpr (FAR) {
+      Span span;
+      for (int it = 0; it < n; it += IB) {
+        batch(it);
+        span.meet(live, vcode);
+      }
+      __syncthreads();
+      put_span(span);
+      __syncthreads();
+      skip = !__builtin_amdgcn_readfirstlane(far_spans());
+      if (skip) return;
+    }
     batch(0);
-    load_k(0);
-    load_v(0);
+    if constexpr (!FAR) {
+      load_k(0);
+      load_v(0);
+    }
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
       const int row = m * 16 + c16, i = FEW ? min(row / a.group, sq.n - 1) : 0;
@@ -261,6 +342,18 @@ __device__ __forceinline__ void body(const PagedAttnArgs &a, float *lds, int wg,
   };
   open();
   for (;;) {
+    if (skip) {
+      u += n;
+      if (u >= u_end) break;
+      walk.step(u, &b, &before, &sq);
+      open();
+      continue;
+    }
+    if constexpr (!FAR) { // (while the first keys are on their way)
+      Span span;
+      span.meet(live, vcode);
+      put_span(span);
+    }
     f32x4 acc[MT][VB];
     float mref[MT], lsum[MT];
 #pragma unroll
@@ -271,6 +364,11 @@ __device__ __forceinline__ void body(const PagedAttnArgs &a, float *lds, int wg,
       for (int i = 0; i < VB; ++i) acc[m][i] = (f32x4){0, 0, 0, 0};
     }
     for (int it = 0; it < n; ++it) {
+      if constexpr (FAR) { // (nothing ahead: no more registers than the first pass has)
+        if (it > 0 && it % IB == 0) batch(it);
+        load_k(it);
+        load_v(it);
+      }
       int nv[NS], vc[NS];
       float ks[NS];
       int nmin = 16;
@@ -301,8 +399,11 @@ __device__ __forceinline__ void body(const PagedAttnArgs &a, float *lds, int wg,
 #pragma unroll
           for (int r = 0; r < 4; ++r) st[m][s][r] = fmaf(st[m][s][r], ks[s], (float)(vc[s] - kBase));
       }
-      if (it + 1 < n) {
-        if ((it + 1) % IB == 0) batch(it + 1);
+      if (!FAR && it + 1 < n) {
+        if ((it + 1) % IB == 0) {
+          if (it >= IB) widen_span(); // (not right behind its loads)
+          batch(it + 1);
+        }
         load_k(it + 1);
       }
       // keys behind the end or on no page, and those that some row does not attend
@@ -346,13 +447,14 @@ __device__ __forceinline__ void body(const PagedAttnArgs &a, float *lds, int wg,
           x = fmaxf(x, __shfl_xor(x, 32));
           const float mn = fmaxf(mref[m], x);
           const float al = mn == -kInf ? 1.0f : __builtin_amdgcn_exp2f(mref[m] - mn);
+          lsum[m] = !FAR ? lsum[m] * al : mn == -kInf ? lsum[m] : lower(lsum[m], mref[m] - mn);
           mref[m] = mn;
-          lsum[m] *= al;
 #pragma unroll
           for (int i = 0; i < VB; ++i) acc[m][i] *= al;
         }
       }
-      f16x8 pf[MT][NS / 2];
+      typename W::frag pf[MT][NS / 2];
+      [[maybe_unused]] typename W::frag rest[MT][NS / 2]; // FAR: what rounding to pf took away
 #pragma unroll
       for (int m = 0; m < MT; ++m) {
         const float ref = (mref[m] == -kInf ? 0.0f : mref[m]) - kLift;
@@ -362,9 +464,16 @@ __device__ __forceinline__ void body(const PagedAttnArgs &a, float *lds, int wg,
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
             w[r] = __builtin_amdgcn_exp2f(st[m][s][r] - ref);
-            pf[m][s >> 1][(s & 1) * 4 + r] = (_Float16)w[r];
+            if constexpr (FAR) {
+              const __bf16 h = (__bf16)w[r];
+              pf[m][s >> 1][(s & 1) * 4 + r] = h;
+              rest[m][s >> 1][(s & 1) * 4 + r] = (__bf16)(w[r] - (float)h);
+              lsum[m] += __builtin_amdgcn_exp2f(st[m][s][r] - ref + (float)(kBase - vc[s])); // (w can be too small for fp32, the probability is not)
+            } else {
+              pf[m][s >> 1][(s & 1) * 4 + r] = (_Float16)w[r];
+            }
           }
-          lsum[m] = fmaf((w[0] + w[1]) + (w[2] + w[3]), unweight(vc[s]), lsum[m]);
+          if constexpr (!FAR) lsum[m] = fmaf((w[0] + w[1]) + (w[2] + w[3]), unweight(vc[s]), lsum[m]);
         }
       }
       // the sum over V
@@ -378,46 +487,51 @@ __device__ __forceinline__ void body(const PagedAttnArgs &a, float *lds, int wg,
             const int s = 2 * p + (j >> 1), r = (j & 1) * 2;
             const uint32_t x = __builtin_amdgcn_perm(vr[s][r + 1][w], vr[s][r][w], 0x05010400);
             const uint32_t y = __builtin_amdgcn_perm(vr[s][r + 1][w], vr[s][r][w], 0x07030602);
-            f[0][j] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x, 1.0f, false));
-            f[1][j] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x, 1.0f, true));
-            f[2][j] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(y, 1.0f, false));
-            f[3][j] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(y, 1.0f, true));
+            f[0][j] = W::template codes2<false>(x);
+            f[1][j] = W::template codes2<true>(x);
+            f[2][j] = W::template codes2<false>(y);
+            f[3][j] = W::template codes2<true>(y);
           }
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            f16x8 x = __builtin_bit_cast(f16x8, (u32x4){f[i][0], f[i][1], f[i][2], f[i][3]});
+            typedef typename W::frag frag;
+            frag x = __builtin_bit_cast(frag, (u32x4){f[i][0], f[i][1], f[i][2], f[i][3]});
             if (FEW && __builtin_expect(nan, 0)) { // the sum runs without NaN, another product counts those that a row attends
-              f16x8 y;
+              frag y;
 #pragma unroll
               for (int j = 0; j < 8; ++j) {
-                y[j] = x[j] != x[j] ? (_Float16)1.0f : (_Float16)0.0f;
-                x[j] = x[j] != x[j] ? (_Float16)0.0f : x[j];
+                const bool bad = x[j] != x[j];
+                y[j] = bad ? 1.0f : 0.0f;
+                x[j] = bad ? 0.0f : (float)x[j];
               }
 #pragma unroll
               for (int m = 0; m < MT; ++m) {
-                f16x8 sees;
+                frag sees;
 #pragma unroll
-                for (int j = 0; j < 8; ++j) sees[j] = key0 + (2 * p + (j >> 2)) * 16 + g * 4 + (j & 3) <= limit[m] ? (_Float16)1.0f : (_Float16)0.0f;
-                const f32x4 bad = __builtin_amdgcn_mfma_f32_16x16x32_f16(y, sees, (f32x4){0, 0, 0, 0}, 0, 0, 0);
+                for (int j = 0; j < 8; ++j) sees[j] = key0 + (2 * p + (j >> 2)) * 16 + g * 4 + (j & 3) <= limit[m] ? 1.0f : 0.0f;
+                const f32x4 bad = W::mfma(y, sees, (f32x4){0, 0, 0, 0});
 #pragma unroll
                 for (int r = 0; r < 4; ++r)
                   if (bad[r] > 0.0f) acc[m][w * 4 + i][r] = __builtin_nanf("");
               }
             }
 #pragma unroll
-            for (int m = 0; m < MT; ++m)
-              acc[m][w * 4 + i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, pf[m][p], acc[m][w * 4 + i], 0, 0, 0);
+            for (int m = 0; m < MT; ++m) {
+              if constexpr (FAR) acc[m][w * 4 + i] = W::mfma(x, rest[m][p], acc[m][w * 4 + i]);
+              acc[m][w * 4 + i] = W::mfma(x, pf[m][p], acc[m][w * 4 + i]);
+            }
           }
         }
-      if (it + 1 < n) load_v(it + 1);
+      if (!FAR && it + 1 < n) load_v(it + 1);
     }
 
     // ---- the next sequence's loads, then the merge of the four wavefronts ----
+    if (!FAR && n > IB) widen_span();
     const int32_t q0 = sq.q0, rows = FEW ? sq.n * a.group : a.group;
     const bool whole = n == sq.units;
     // (the first sequence of this workgroup takes slot 0, a later one that is not whole can only be its last: slot 1)
     const int which = u == u_first ? 0 : 1;
-    if (!whole && c0 == 0) {
+    if (!FAR && !whole && c0 == 0) {
       const int32_t last = before + sq.units - 1, larger = extra * (each + 1); // its last unit, and the group that has that
       const int32_t owner = last < larger ? last / (each + 1) : extra + (last - larger) / each;
       if (tid == 0) *split = {q0, owner - group, which, rows};
@@ -445,6 +559,8 @@ __device__ __forceinline__ void body(const PagedAttnArgs &a, float *lds, int wg,
     }
     __syncthreads();
     float *slot = a.part + (2 * (int64_t)wg + which) * part_floats<D, MT>();
+    const bool left = !FAR && far_spans();
+    again |= left;
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
       const int row = m * 16 + (tid >> 4), d0 = (tid & 15) * VB;
@@ -459,12 +575,13 @@ __device__ __forceinline__ void body(const PagedAttnArgs &a, float *lds, int wg,
       for (int w = 0; w < 4; ++w) {
         const float mw = wml[(w * 16 * MT + row) * 2];
         const float f = mw == -kInf ? 1.0f : __builtin_amdgcn_exp2f(mw - mm); // (a row of NaN scores has reference -inf)
-        l += wml[(w * 16 * MT + row) * 2 + 1] * f;
+        const float lw = wml[(w * 16 * MT + row) * 2 + 1];
+        l += !FAR ? lw * f : mw == -kInf ? lw : lower(lw, mw - mm);
 #pragma unroll
         for (int i = 0; i < VB; ++i) o[i] += wo[(w * 16 * MT + row) * LD + d0 + i] * f;
       }
       if (whole) {
-        if (row < rows) {
+        if (row < rows && !left) {
           const int64_t t = q0 + (FEW ? row / a.group : 0);
           const int hq = hk * a.group + (FEW ? row % a.group : row);
           const bool none = l == 0.0f && mx == -kInf;
@@ -476,7 +593,7 @@ __device__ __forceinline__ void body(const PagedAttnArgs &a, float *lds, int wg,
                                     (uint32_t)E::out(o[i + 1] * inv) << 16;
           if (a.lse && d0 == 0) a.lse[t * a.heads_q + hq] = none ? -kInf : mx - kLift + __builtin_log2f(l);
         }
-      } else {
+      } else if (!left) {
 #pragma unroll
         for (int i = 0; i < VB; i += 4) *(f32x4 *)(slot + row * D + d0 + i) = (f32x4){o[i], o[i + 1], o[i + 2], o[i + 3]};
         if (d0 == 0) {
@@ -488,7 +605,22 @@ __device__ __forceinline__ void body(const PagedAttnArgs &a, float *lds, int wg,
     if (!more) break;
     __syncthreads();
   }
-  if (a.part && !noted && tid == 0) split->q0 = -1;
+  if (!FAR && a.part && !noted && tid == 0) split->q0 = -1;
+  return __builtin_amdgcn_readfirstlane(again);
+}
+// (a function of its own, out of the first pass's register allocation: inlined, 48 sequences of 60 to 8000 keys took 73 us instead of 69)
+// OCC, workgroups on a CU, keeps apart the functions of kernels that may use more registers.
+template <class E, int D, int MT, bool FEW, int OCC>
+__device__ __attribute__((noinline)) void far_pass(uint64_t args, Lds lds, int wg, int wgs) {
+  const PagedAttnArgs a = args_at(args);
+  body<E, D, MT, FEW, true>(a, (float *)lds, uniform(wg), uniform(wgs), threadIdx.x);
+}
+template <class E, int D, int MT, bool FEW, int OCC>
+__device__ __forceinline__ void both(const PagedAttnArgs &a, float *lds, int wg, int wgs) {
+  if (__builtin_expect(body<E, D, MT, FEW, false>(a, lds, wg, wgs, threadIdx.x), 0)) {
+    __syncthreads();
+    far_pass<E, D, MT, FEW, OCC>((uint64_t)__builtin_amdgcn_kernarg_segment_ptr(), (Lds)lds, wg, wgs);
+  }
 }
 
 // Adds the parts of the split sequence that workgroup wg of the launch before noted, if any: one of `join_pieces` pieces
@@ -524,9 +656,8 @@ template <class E, int D, int MT> __device__ __forceinline__ void join(const Pag
       for (int i = 0; i < 4; ++i) {
         if (p + i * deep >= parts) break;
         const float mn = fmaxf(m, pm[i]), ref = mn == -kInf ? 0.0f : mn;
-        // (a row of NaN scores has reference -inf and a NaN sum: it has to stay)
         const float f = m == -kInf ? 1.0f : __builtin_amdgcn_exp2f(m - ref), w = pm[i] == -kInf ? 1.0f : __builtin_amdgcn_exp2f(pm[i] - ref);
-        l = l * f + pl[i] * w;
+        l = add_sums(l, m, f, pl[i], pm[i], w, ref);
         o = o * f + po[i] * w;
         m = mn;
       }
@@ -541,7 +672,7 @@ template <class E, int D, int MT> __device__ __forceinline__ void join(const Pag
           const int y = tid + q * across * TPR;
           const float mn = fmaxf(m, lm[y]), ref = mn == -kInf ? 0.0f : mn;
           const float f = m == -kInf ? 1.0f : __builtin_amdgcn_exp2f(m - ref), w = lm[y] == -kInf ? 1.0f : __builtin_amdgcn_exp2f(lm[y] - ref);
-          l = l * f + ll[y] * w;
+          l = add_sums(l, m, f, ll[y], lm[y], w, ref);
           o = o * f + lds[y] * w;
           m = mn;
         }
@@ -559,18 +690,18 @@ template <class E, int D, int MT> __device__ __forceinline__ void join(const Pag
   }
 }
 
-template <int D, int MT> constexpr int lds_floats() { return 4 * 16 * MT * (D + 4) + 4 * 16 * MT * 2; }
+template <int D, int MT> constexpr int lds_floats() { return 4 * 16 * MT * (D + 4) + 4 * 16 * MT * 2 + 8; }
 
 } // namespace one
 
 #define PAGED_ONE(T, E, D, MT, OCC)                                                                           \
   extern "C" __global__ __launch_bounds__(256, OCC) void paged_attn_one_##T##_d##D##_r##MT(PagedAttnArgs a) {  \
     __shared__ __align__(16) float lds[one::lds_floats<D, MT>()];                                             \
-    one::body<one::E, D, MT, false>(a, lds, blockIdx.x, gridDim.x);                                           \
+    one::both<one::E, D, MT, false, OCC>(a, lds, blockIdx.x, gridDim.x);                                           \
   }                                                                                                           \
   extern "C" __global__ __launch_bounds__(256, 2) void paged_attn_few_##T##_d##D##_r##MT(PagedAttnArgs a) {    \
     __shared__ __align__(16) float lds[one::lds_floats<D, MT>()];                                             \
-    one::body<one::E, D, MT, true>(a, lds, blockIdx.x, gridDim.x);                                            \
+    one::both<one::E, D, MT, true, 2>(a, lds, blockIdx.x, gridDim.x);                                            \
   }                                                                                                           \
   extern "C" __global__ __launch_bounds__(256) void paged_attn_join_##T##_d##D##_r##MT(PagedAttnArgs a) {      \
     __shared__ one::f32x4 lds[256 + 128];                                                                     \

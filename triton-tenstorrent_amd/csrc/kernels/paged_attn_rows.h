@@ -21,7 +21,6 @@
 
 namespace rows {
 
-using one::f16x8;
 using one::kBase;
 using one::kInf;
 using one::kLazy;
@@ -30,15 +29,10 @@ using one::kOut;
 using one::unweight;
 using one::u32x2;
 using one::u32x4;
-typedef float f32x16 __attribute__((ext_vector_type(16)));
-typedef float f32x4 __attribute__((ext_vector_type(4)));
-
-struct Bf : one::Bf {
-  static __device__ __forceinline__ f32x16 mfma32(frag x, frag y, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, y, c, 0, 0, 0); }
-};
-struct Hf : one::Hf {
-  static __device__ __forceinline__ f32x16 mfma32(frag x, frag y, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(x, y, c, 0, 0, 0); }
-};
+using one::f32x16;
+using one::f32x4;
+using one::Bf;
+using one::Hf;
 
 constexpr int kRows = 128;
 
@@ -60,8 +54,7 @@ __device__ __forceinline__ int steps_of(const PagedAttnArgs &a, const Seq &sq, i
   return max((last_key(a, sq, r1 / a.group) + 64) / 64, 1);
 }
 
-__device__ __forceinline__ int32_t scan64(int32_t v) { // inclusive, over the wavefront
-  const int lane = threadIdx.x & 63;
+__device__ __forceinline__ int32_t scan64(int32_t v, int lane) { // inclusive, over the wavefront
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) {
     const int32_t o = __shfl_up(v, d);
@@ -74,7 +67,7 @@ __device__ __forceinline__ int32_t scan64(int32_t v) { // inclusive, over the wa
 // the sequences i * per and up.
 struct Walk {
   const PagedAttnArgs &a;
-  int per;
+  int lane, per;
   int32_t base, total;
   __device__ __forceinline__ int32_t units_of(const Seq &sq) const {
     if (a.rows_whole) return sq.tiles;
@@ -82,8 +75,7 @@ struct Walk {
     for (int i = 0; i < sq.tiles; ++i) n += steps_of(a, sq, i);
     return n;
   }
-  __device__ __forceinline__ Walk(const PagedAttnArgs &args) : a(args) {
-    const int lane = threadIdx.x & 63;
+  __device__ __forceinline__ Walk(const PagedAttnArgs &args, int lane) : a(args), lane(lane) {
     per = (a.b + 63) / 64;
     int32_t n = 0;
     bool large = false; // a sequence of many tiles, which all lanes count together
@@ -101,7 +93,7 @@ struct Walk {
       for (int d = 32; d; d >>= 1) m += __shfl_xor(m, d);
       if (lane == b) n = m;
     }
-    const int32_t v = scan64(n);
+    const int32_t v = scan64(n, lane);
     base = v - n;
     total = __builtin_amdgcn_readlane(v, 63);
   }
@@ -121,10 +113,9 @@ struct Walk {
   }
   // the tile of sequence sq that holds its step `at`, and the steps before that tile
   __device__ __forceinline__ int tile_of(const Seq &sq, int32_t at, int32_t *before) const {
-    const int lane = threadIdx.x & 63;
     *before = 0;
     for (int i0 = 0;; i0 += 64) {
-      const int32_t n = i0 + lane < sq.tiles ? steps_of(a, sq, i0 + lane) : 0, v = scan64(n);
+      const int32_t n = i0 + lane < sq.tiles ? steps_of(a, sq, i0 + lane) : 0, v = scan64(n, lane);
       const uint64_t past = __ballot(*before + v > at);
       if (past) {
         const int l = __builtin_ctzll(past);
@@ -150,27 +141,29 @@ constexpr int kMeta = 80;
 template <int D> constexpr int stage_bytes() { return (64 * D * 2 * 2 + kMeta + 64 * 16 * 2 + 511) / 512 * 512; }
 template <int D> constexpr int lds_bytes() { return 2 * stage_bytes<D>(); }
 
-template <class E, int D>
-__device__ __forceinline__ void body(const PagedAttnArgs &a, uint8_t *lds, int wg, int wgs) {
+// Returns whether a tile was left to FAR, as in paged_attn_one.h.
+template <class E, int D, bool FAR>
+__device__ __forceinline__ bool body(const PagedAttnArgs &a, uint8_t *lds, int wg, int wgs, int tid) {
+  typedef typename one::Weights<FAR>::type W;
   constexpr int DK = D / 16, DT = D / 32, KB = D / 4, VB = D / 16, KW = KB / 16, VW = VB / 4;
   constexpr int KROW = D * 2, VOFF = 64 * KROW, FOFF = 2 * VOFF;
   constexpr int KMASK = D == 64 ? 7 : 15, KSH = D == 64 ? 1 : 0; // chunk swizzle of K rows
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c32 = lane & 31, hi = lane >> 5;
-  const Walk walk(a);
+  const Walk walk(a, lane);
   const int heads = a.c.heads, hk = wg % heads, group = wg / heads;
   Split *split = (Split *)(a.rows_part + 2 * (int64_t)wgs * part_floats<D>()) + wg;
   int32_t u, u_end, before;
   int32_t each = 1, extra = 0; // steps of a group; the first `extra` groups have one more
   if (a.rows_whole) {
     u = walk.total - 1 - group; // late rows, which attend most keys, first
-    if (u < 0) return;
+    if (u < 0) return false;
     u_end = u + 1;
   } else {
     const int32_t groups = min(wgs / heads, walk.total);
     if (group >= groups) {
-      if (tid == 0) split->b = -1;
-      return;
+      if (!FAR && tid == 0) split->b = -1;
+      return false;
     }
     each = walk.total / groups;
     extra = walk.total - each * groups;
@@ -187,7 +180,7 @@ __device__ __forceinline__ void body(const PagedAttnArgs &a, uint8_t *lds, int w
     before += inside; // from here on: the units before the tile
   }
   const int32_t u_first = u;
-  bool noted = false;
+  bool noted = false, again = false;
 
   for (;;) {
     const int R = sq.n * a.group, row0 = tile * kRows;
@@ -228,6 +221,7 @@ __device__ __forceinline__ void body(const PagedAttnArgs &a, uint8_t *lds, int w
     // What lane (k % 16) * 4 + s knows of subtile s of step k (16 steps at a time).
     int32_t ko_lo, ko_hi, vo_lo, vo_hi, live, vcode;
     float kscale;
+    one::Span span; // the same in all wavefronts
     auto batch = [&](int k0) {
       const int64_t key = (int64_t)(k0 + (lane >> 2)) * 64 + (lane & 3) * 16;
       const uint32_t sub = (uint32_t)(key >> 4);
@@ -247,7 +241,10 @@ __device__ __forceinline__ void body(const PagedAttnArgs &a, uint8_t *lds, int w
     int staged_at, staged_nv; // of the codes in kr and vr: the lane that knows the tile's first subtile, the wavefront's live keys
     auto load = [&](int k, int k_first) {
       const int at = ((k - k_first) & 15) * 4;
-      if (((k - k_first) & 15) == 0) batch(k);
+      if (((k - k_first) & 15) == 0) {
+        if (!FAR && k != k_first) span.meet(live, vcode); // (not right behind their loads)
+        batch(k);
+      }
       staged_at = at;
       staged_nv = __builtin_amdgcn_readlane(live, at + wave);
       const uint8_t *kp = kh + one::lane64(ko_lo, ko_hi, at + wave), *vp = vh + one::lane64(vo_lo, vo_hi, at + wave);
@@ -328,31 +325,40 @@ __device__ __forceinline__ void body(const PagedAttnArgs &a, uint8_t *lds, int w
       for (int w = 0; w < VW; ++w) {
         const uint32_t x0 = __builtin_amdgcn_perm(vr[1][w], vr[0][w], 0x05010400), x1 = __builtin_amdgcn_perm(vr[3][w], vr[2][w], 0x05010400);
         const uint32_t y0 = __builtin_amdgcn_perm(vr[1][w], vr[0][w], 0x07030602), y1 = __builtin_amdgcn_perm(vr[3][w], vr[2][w], 0x07030602);
-        const u32x2 f[4] = {{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x0, 1.0f, false)),
-                             __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x1, 1.0f, false))},
-                            {__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x0, 1.0f, true)),
-                             __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x1, 1.0f, true))},
-                            {__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(y0, 1.0f, false)),
-                             __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(y1, 1.0f, false))},
-                            {__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(y0, 1.0f, true)),
-                             __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(y1, 1.0f, true))}};
+        const u32x2 f[4] = {{W::template codes2<false>(x0),
+                             W::template codes2<false>(x1)},
+                            {W::template codes2<true>(x0),
+                             W::template codes2<true>(x1)},
+                            {W::template codes2<false>(y0),
+                             W::template codes2<false>(y1)},
+                            {W::template codes2<true>(y0),
+                             W::template codes2<true>(y1)}};
   #pragma unroll
         for (int i = 0; i < 4; ++i) *(u32x2 *)(lds + (vw ^ (((w * 4 + i) >> 1) << 4)) + (w * 4 + i) * 128) = f[i];
       }
     };
     auto edge_of = [&](int k) { return k * 64 + 63 > all_to; };
 
-    if (k_lo < k_hi) {
+    bool far = false;
+    if constexpr (FAR) {
+      for (int k = k_lo; k < k_hi; k += 16) {
+        batch(k);
+        span.meet(live, vcode);
+      }
+      far = span.far();
+    }
+    const int k_to = FAR && !far ? k_lo : k_hi; // (no step of a tile that the first pass has done)
+    if (k_lo < k_to) {
       load(k_lo, k_lo);
       store(0, edge_of(k_lo));
     }
-    if (k_lo + 1 < k_hi) load(k_lo + 1, k_lo);
+    if (k_lo + 1 < k_to) load(k_lo + 1, k_lo);
     __syncthreads();
-    for (int k = k_lo; k < k_hi; ++k) {
+    for (int k = k_lo; k < k_to; ++k) {
       const uint32_t buf = ((k - k_lo) & 1) * stage_bytes<D>(), next = stage_bytes<D>() - buf;
-      if (k + 1 < k_hi) {
+      if (k + 1 < k_to) {
         store(next, edge_of(k + 1));
-        if (k + 2 < k_hi) load(k + 2, k_lo);
+        if (k + 2 < k_to) load(k + 2, k_lo);
       }
       __builtin_amdgcn_sched_barrier(0);
       if (alive && k * 64 <= wave_last) {
@@ -403,8 +409,8 @@ __device__ __forceinline__ void body(const PagedAttnArgs &a, uint8_t *lds, int w
         if (__any(top > mref + kLazy)) {
           const float mn = fmaxf(mref, fmaxf(top, __shfl_xor(top, 32)));
           const float al = mn == -kInf ? 1.0f : __builtin_amdgcn_exp2f(mref - mn);
+          lsum = !FAR ? lsum * al : mn == -kInf ? lsum : one::lower(lsum, mref - mn);
           mref = mn;
-          lsum *= al;
   #pragma unroll
           for (int i = 0; i < DT; ++i)
   #pragma unroll
@@ -412,15 +418,23 @@ __device__ __forceinline__ void body(const PagedAttnArgs &a, uint8_t *lds, int w
         }
         const float ref = (mref == -kInf ? 0.0f : mref) - kLift;
         // weights of a subtile between the products of the one before, V fragments four reads ahead
-        f16x8 pf[4];
+        typename W::frag pf[4];
+        [[maybe_unused]] typename W::frag rest[4]; // FAR: what rounding to pf took away
         float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
         auto weights = [&](int s, int r0, int n) {
           const float c = offset[s] - ref;
   #pragma unroll
           for (int r = r0; r < r0 + n; ++r) {
             const float w = __builtin_amdgcn_exp2f(fmaf(st[s >> 1][(s & 1) * 8 + r], factor[s], c));
-            sum[s] += w; // (the sum of probabilities has to be fp32's: the log-sum-exp is a result)
-            pf[s][r] = (_Float16)w;
+            if constexpr (FAR) {
+              const __bf16 h = (__bf16)w;
+              pf[s][r] = h;
+              rest[s][r] = (__bf16)(w - (float)h);
+              lsum += __builtin_amdgcn_exp2f(fmaf(st[s >> 1][(s & 1) * 8 + r], factor[s], -ref)); // (w can be too small for fp32, the probability is not)
+            } else {
+              sum[s] += w; // (the sum of probabilities has to be fp32's: the log-sum-exp is a result)
+              pf[s][r] = (_Float16)w;
+            }
           }
         };
         auto v_frag = [&](int i) { return *(const u32x4 *)(lds + (vb ^ (((i / DT) ^ (i % DT & 3)) << 5)) + i % DT * 32 * 128); };
@@ -430,13 +444,14 @@ __device__ __forceinline__ void body(const PagedAttnArgs &a, uint8_t *lds, int w
   #pragma unroll
         for (int i = 0; i < 4 * DT; ++i) {
           __builtin_amdgcn_sched_barrier(0);
-          acc[i % DT] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, x[i & 3]), pf[i / DT], acc[i % DT], 0, 0, 0);
+          if constexpr (FAR) acc[i % DT] = W::mfma32(__builtin_bit_cast(typename W::frag, x[i & 3]), rest[i / DT], acc[i % DT]);
+          acc[i % DT] = W::mfma32(__builtin_bit_cast(typename W::frag, x[i & 3]), pf[i / DT], acc[i % DT]);
           if (i + 4 < 4 * DT) x[i & 3] = v_frag(i + 4);
           if (i < 3 * DT) weights(i / DT + 1, i % DT * (8 / DT), 8 / DT);
         }
         __builtin_amdgcn_sched_barrier(0);
   #pragma unroll
-        for (int s = 0; s < 4; ++s) lsum = fmaf(sum[s], back[s], lsum);
+        for (int s = 0; s < 4 && !FAR; ++s) lsum = fmaf(sum[s], back[s], lsum);
         if (edge) { // NaN in V, taken out of the tile: it reaches the rows that attend its key
           for (int s = 0; s < 4; ++s) {
             if (!__builtin_amdgcn_readfirstlane(*(const int32_t *)(lds + buf + FOFF + 64 + s * 4))) continue;
@@ -457,11 +472,16 @@ __device__ __forceinline__ void body(const PagedAttnArgs &a, uint8_t *lds, int w
       __syncthreads();
     }
 
+    if constexpr (!FAR) {
+      span.meet(live, vcode);
+      far = span.far();
+      again |= far;
+    }
     lsum += __shfl_xor(lsum, 32);
     const bool cut = k_lo > 0 || k_hi < nsteps;
     // (the first tile of this workgroup takes slot 0, a later one that is cut can only be its last: slot 1)
     const int which = u == u_first ? 0 : 1;
-    if (alive && row < R) {
+    if (alive && row < R && far == FAR) {
       if (!cut) {
         const bool none = lsum == 0.0f && mref == -kInf;
         const float inv = none ? 0.0f : kOut / lsum;
@@ -487,8 +507,8 @@ __device__ __forceinline__ void body(const PagedAttnArgs &a, uint8_t *lds, int w
         if (hi == 0) { p[kRows * D + lr * 2] = mref; p[kRows * D + lr * 2 + 1] = lsum; }
       }
     }
-    if (a.rows_whole) return;
-    if (cut && k_lo == 0) {
+    if (a.rows_whole) return again;
+    if (!FAR && cut && k_lo == 0) {
       const int32_t last = before + nsteps - 1, larger = extra * (each + 1); // the tile's last step, and the group that has it
       const int32_t owner = last < larger ? last / (each + 1) : extra + (last - larger) / each;
       if (tid == 0) *split = {b, owner - group, which, tile};
@@ -503,7 +523,18 @@ __device__ __forceinline__ void body(const PagedAttnArgs &a, uint8_t *lds, int w
       while (sq.tiles == 0); // (u is less than all units)
     }
   }
-  if (!noted && tid == 0) split->b = -1;
+  if (!FAR && !noted && tid == 0) split->b = -1;
+  return again;
+}
+template <class E, int D> __device__ __attribute__((noinline)) void far_pass(uint64_t args, one::Lds lds, int wg, int wgs) {
+  const PagedAttnArgs a = one::args_at(args);
+  body<E, D, true>(a, (uint8_t *)lds, one::uniform(wg), one::uniform(wgs), threadIdx.x);
+}
+template <class E, int D> __device__ __forceinline__ void both(const PagedAttnArgs &a, uint8_t *lds, int wg, int wgs) {
+  if (__builtin_expect(body<E, D, false>(a, lds, wg, wgs, threadIdx.x), 0)) {
+    __syncthreads();
+    far_pass<E, D>((uint64_t)__builtin_amdgcn_kernarg_segment_ptr(), (one::Lds)lds, wg, wgs);
+  }
 }
 
 // Adds the parts of the split tile that workgroup wg of the launch before noted, if any: rows 16 part .. + 15.
@@ -536,9 +567,8 @@ template <class E, int D> __device__ __forceinline__ void join(const PagedAttnAr
     for (int i = 0; i < 4; ++i) {
       if (p + i >= parts) break;
       const float mn = fmaxf(m, pm[i]), ref = mn == -kInf ? 0.0f : mn;
-      // (a row of NaN scores has reference -inf and a NaN sum: it has to stay)
       const float f = m == -kInf ? 1.0f : __builtin_amdgcn_exp2f(m - ref), w = pm[i] == -kInf ? 1.0f : __builtin_amdgcn_exp2f(pm[i] - ref);
-      l = l * f + pl[i] * w;
+      l = one::add_sums(l, m, f, pl[i], pm[i], w, ref);
 #pragma unroll
       for (int v = 0; v < VB / 4; ++v) o[v] = o[v] * f + po[i][v] * w;
       m = mn;
@@ -563,9 +593,9 @@ template <class E, int D> __device__ __forceinline__ void join(const PagedAttnAr
     constexpr int bytes = rows::lds_bytes<D>() > one::lds_floats<D, MT>() * 4 ? rows::lds_bytes<D>() : one::lds_floats<D, MT>() * 4; \
     __shared__ __align__(512) uint8_t lds[bytes];                                                             \
     if ((int)blockIdx.x < a.rows_groups)                                                                      \
-      rows::body<rows::E, D>(a, lds, blockIdx.x, a.rows_groups);                                              \
+      rows::both<rows::E, D>(a, lds, blockIdx.x, a.rows_groups);                                              \
     else                                                                                                      \
-      one::body<one::E, D, MT, true>(a, (float *)lds, blockIdx.x - a.rows_groups, gridDim.x - a.rows_groups); \
+      one::both<one::E, D, MT, true, OCC>(a, (float *)lds, blockIdx.x - a.rows_groups, gridDim.x - a.rows_groups); \
   }                                                                                                           \
   /* 8 workgroups for each that may have split a row tile, then join_pieces for each that may have split a sequence */ \
   extern "C" __global__ __launch_bounds__(256) void paged_attn_rows_join_##T##_d##D##_r##MT(PagedAttnArgs a) { \
