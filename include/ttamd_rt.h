@@ -404,7 +404,7 @@ TTAMD_API int tt_paged_write(const void *k, const void *v, const int64_t k_strid
  * cache: rows cu_q[b] .. cu_q[b+1]-1 belong to sequence b, which holds lens[b] keys.  heads_q is a multiple of
  * cache->heads; query head h reads cache head h / (heads_q / heads).  With causal, query i of n attends the keys at
  * positions <= lens[b] - n + i, otherwise all lens[b] keys; keys on a page outside the cache count as absent.  A query
- * that attends no key gives 0 and lse = -inf.  o (strides as q's) has q's type; lse (null, or [tokens, heads_q]
+ * that attends no key, or whose scores all are -inf, gives 0 and lse = -inf.  o (strides as q's) has q's type; lse (null, or [tokens, heads_q]
  * contiguous fp32) is the base-2 log-sum-exp of the scaled scores.  Rows outside every sequence are left as they are.
  * max_q is an upper bound of the queries of one sequence; the rows of a sequence that has more are undefined.
  * Scores, softmax and sums are fp32; the weights of V (probability times the page's scale, relative to the row's

@@ -104,10 +104,10 @@ def attention(q, kc, vc, ks, vs, table, lens, cu, sm_scale, causal):
             for i in range(n):
                 t = cu[b] + i
                 sees = key <= (L - n + i if causal else L - 1)
-                if not sees.any():
+                s = k[sees] @ q[t, h] * sm_scale
+                if (s == -np.inf).all():            # also where it sees no key
                     o[t, h], lse[t, h], spread[t, h] = 0.0, -np.inf, 0.0
                     continue
-                s = k[sees] @ q[t, h] * sm_scale
                 m = s.max()
                 p = np.exp(s - m)
                 l = p.sum()

@@ -754,3 +754,23 @@ def test_pages_of_zeros_beside_any_others(n, Hq, H, D, top):
     o, lse = K.paged_attention(q.cuda(), device_cache(codes, scales), i32(table), i32(lens), i32(cu), 0.09, max_q=n, return_lse=True)
     want = orc.attention(q.double().numpy(), codes[0], codes[1], scales[0], scales[1], table, lens, cu, 0.09, True)
     compare_far(o, lse, want, 1100, D, torch.bfloat16, top - orc.MIN_SCALE)
+
+
+@pytest.mark.parametrize("n,Hq,H,D", [(1, 4, 2, 64), (1, 4, 2, 128), (1, 2, 2, 256), (5, 4, 2, 128), (8, 4, 2, 256), (30, 8, 2, 128), (30, 4, 2, 64),
+                                      (3, 4, 2, 40)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("sm_scale", [0.1, -0.1])
+def test_a_query_whose_scores_all_are_minus_infinity_gives_what_one_without_a_key_does(n, Hq, H, D, dtype, sm_scale):
+    q, codes, scales, table, lens, cu = make([100, 0, 700], [n, n, n], Hq, H, 16, D, dtype, seed=D)
+    at = codes[0, ..., 0] != 0x7F
+    codes[0, ..., 0][at] = 0x38             # component 0 of every key is 1 times its scale
+    sign = -np.sign(sm_scale)
+    for row, x in ((0, sign), (2 * n, sign), (3 * n - 1, -sign)):
+        q[row, 1, 0] = x * float("inf")
+    o, lse = K.paged_attention(q.cuda(), device_cache(codes, scales), i32(table), i32(lens), i32(cu), sm_scale, max_q=n, return_lse=True)
+    nan, none = torch.zeros(3 * n, Hq, dtype=torch.bool), torch.zeros(3 * n, Hq, dtype=torch.bool)
+    none[n:2 * n], none[0, 1], none[2 * n, 1] = True, True, True
+    nan[3 * n - 1, 1], none[3 * n - 1, 1] = True, False     # every score is +inf
+    o, lse = o.cpu(), lse.cpu()
+    assert torch.equal(torch.isnan(o).all(-1), nan) and torch.equal(torch.isnan(o).any(-1), nan) and torch.equal(torch.isnan(lse), nan)
+    assert torch.equal(torch.isneginf(lse), none) and (o[none] == 0).all()

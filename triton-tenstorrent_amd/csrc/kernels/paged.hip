@@ -519,7 +519,6 @@ template <typename E> __device__ __forceinline__ void attn_any(const PagedAttnAr
   __syncthreads();
   const int32_t *table = a.table + b * a.table_stride;
   float m = -__builtin_inff(), l = 0.0f, acc[4] = {0, 0, 0, 0};
-  bool seen = false;
   for (int64_t k0 = 0; k0 <= last; k0 += 64) {
     const int64_t key = k0 + lane;
     int32_t page = -1;
@@ -537,10 +536,9 @@ template <typename E> __device__ __forceinline__ void attn_any(const PagedAttnAr
 #pragma unroll
     for (int d = 32; d; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
     if (!__any(live)) continue;
-    seen = true;
-    const float m_new = fmaxf(m, top);
-    const float p = live ? __builtin_amdgcn_exp2f(s - m_new) : 0.0f;
-    const float alpha = __builtin_amdgcn_exp2f(m - m_new);
+    const float m_new = fmaxf(m, top), ref = m_new == -__builtin_inff() ? 0.0f : m_new;
+    const float p = live ? __builtin_amdgcn_exp2f(s - ref) : 0.0f;
+    const float alpha = __builtin_amdgcn_exp2f(m - ref);
     l = l * alpha + p;
     m = m_new;
 #pragma unroll
@@ -558,10 +556,11 @@ template <typename E> __device__ __forceinline__ void attn_any(const PagedAttnAr
   }
 #pragma unroll
   for (int d = 32; d; d >>= 1) l += __shfl_xor(l, d);
+  const bool none = l == 0.0f && m == -__builtin_inff(); // no key, or no score above -inf
 #pragma unroll
   for (int r = 0; r < 4; ++r)
-    if (lane + r * 64 < D) a.o[t * a.o_tok + hq * a.o_head + lane + r * 64] = to_out(seen ? acc[r] / l : 0.0f);
-  if (a.lse && lane == 0) a.lse[(int64_t)t * a.heads_q + hq] = seen ? m + __builtin_log2f(l) : -__builtin_inff();
+    if (lane + r * 64 < D) a.o[t * a.o_tok + hq * a.o_head + lane + r * 64] = to_out(none ? 0.0f : acc[r] / l);
+  if (a.lse && lane == 0) a.lse[(int64_t)t * a.heads_q + hq] = none ? -__builtin_inff() : m + __builtin_log2f(l);
 }
 
 __device__ __forceinline__ uint16_t out_bf16(float f) { return __builtin_bit_cast(uint16_t, (__bf16)f); }

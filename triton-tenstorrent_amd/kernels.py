@@ -439,7 +439,7 @@ def paged_attention(q: torch.Tensor, cache: PagedCache, block_table: torch.Tenso
     ``cu_q[b]:cu_q[b+1]`` belong to sequence b with ``lens[b]`` keys (the new ones among them: write first, then attend).
     ``causal``: query i of n attends the keys at positions <= lens[b] - n + i; otherwise all (an encoder's states).
     ``heads_q`` is a multiple of the cache's heads.  ``max_q``: an upper bound of the queries of one sequence (None: the
-    number of rows); 1 for a decode step takes the kernel for single tokens.  A query without a key gives 0 (lse -inf);
+    number of rows); 1 for a decode step takes the kernel for single tokens.  A query without a key, or with no score above -inf, gives 0 (lse -inf);
     rows outside every sequence are left as they are in ``out``.  Returns ``out``, or (``out``, lse [tokens, heads_q] in
     base 2) with ``return_lse``."""
     out = torch.empty_like(q) if out is None else out
