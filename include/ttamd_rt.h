@@ -114,7 +114,8 @@ TTAMD_API int rt_builtin_module(const char *which, rt_module *out);
 TTAMD_API int rt_get_kernel(rt_module m, const char *name, rt_kernel *out);
 /* command.set_arg... + finalize(grid, block, shared) + schedule.run()
  * (backend/driver.py:117-168), asynchronous on `stream`.  args[i] points at
- * the i-th kernel parameter value. */
+ * the i-th kernel parameter value.  A dimension may have 2^32 - 1 threads
+ * (workgroups times their threads). */
 TTAMD_API int rt_launch(rt_kernel k, const uint32_t grid[3], const uint32_t block[3],
               uint32_t shared_bytes, void *stream, void **args, size_t nargs);
 TTAMD_API int rt_sync(void *stream);

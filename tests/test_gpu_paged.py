@@ -774,3 +774,40 @@ def test_a_query_whose_scores_all_are_minus_infinity_gives_what_one_without_a_ke
     o, lse = o.cpu(), lse.cpu()
     assert torch.equal(torch.isnan(o).all(-1), nan) and torch.equal(torch.isnan(o).any(-1), nan) and torch.equal(torch.isnan(lse), nan)
     assert torch.equal(torch.isneginf(lse), none) and (o[none] == 0).all()
+
+
+def test_more_workgroups_than_a_launch_takes_are_refused():
+    # (all of it in memory that exists: no token has a slot, no row a sequence)
+    H, T = 64, 2**19
+    cache = K.paged_cache(1, H, 1, 16)
+    x = torch.zeros(T + 1, H, 1, dtype=torch.bfloat16, device="cuda")
+    none = torch.full((T + 1, ), -1, **I32)
+    with pytest.raises(NotImplementedError, match="grid"):
+        K.paged_write(x, x, none, cache)                    # 2^24 + 16 workgroups
+    K.paged_write(x[:-2], x[:-2], none[:-2], cache)
+    T = 2**26
+    q = torch.zeros(T, 1, 1, dtype=torch.bfloat16, device="cuda")
+    with pytest.raises(NotImplementedError, match="grid"):
+        K.paged_attention(q, K.paged_cache(1, 1, 1, 16), i32([[0]]), i32([0]), i32([0, 0]), 1.0)
+
+
+def test_more_pairs_of_sequence_and_head_than_a_launch_takes():
+    H, B = 17, 2**20                                        # 2^24 + 2^20 pairs: the kernel for any shape, a workgroup for each row
+    q, codes, scales, table, lens, cu = make([13, 9], [1, 1], H, H, 16, 64, torch.bfloat16)
+    wide = torch.full((B, 1), -1, **I32)
+    many, ends = torch.zeros(B, **I32), torch.zeros(B + 1, **I32)
+    for i, b in ((0, 5), (1, B - 1)):
+        wide[b, 0], many[b] = int(table[i, 0]), int(lens[i])
+        ends[b + 1:] += 1
+    o, lse = K.paged_attention(q.cuda(), device_cache(codes, scales), wide, many, ends, 0.1, max_q=1, return_lse=True)
+    want = orc.attention(q.double().numpy(), codes[0], codes[1], scales[0], scales[1], table, lens, cu, 0.1, True)
+    compare(o, lse, want, 13, 64, torch.bfloat16)
+
+
+def test_rt_launch_refuses_a_dimension_of_more_threads_than_32_bits_count():
+    lib, m, k = rt.init(0), ctypes.c_void_p(), ctypes.c_void_p()
+    rt.check(lib.rt_builtin_module(b"paged", ctypes.byref(m)))
+    rt.check(lib.rt_get_kernel(m, b"paged_plan", ctypes.byref(k)))
+    three = lambda *v: (ctypes.c_uint32 * 3)(*v)
+    for grid, block in (((2**24, 1, 1), (256, 1, 1)), ((2**32 - 1, 1, 1), (2, 1, 1)), ((1, 2**31, 1), (1, 2, 1)), ((1, 1, 2**26), (1, 1, 64))):
+        assert lib.rt_launch(k, three(*grid), three(*block), 0, None, None, 0) == rt.RT_ERR_UNSUPPORTED

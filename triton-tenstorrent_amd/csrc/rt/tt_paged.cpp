@@ -10,6 +10,9 @@
 using namespace ttamd;
 
 namespace {
+// A launch may have 2^32 - 1 threads in x: workgroups of `threads`.
+constexpr int64_t most_groups(int64_t threads) { return UINT32_MAX / threads; }
+
 bool aligned(const void *p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
 
 int check_cache(const char *who, const tt_paged_cache *c, PagedCacheArgs *out) {
@@ -82,7 +85,7 @@ Route route_of(const PagedCacheArgs &c, int32_t B, int32_t max_pages, int32_t to
     // Also where the table allows more units than 32 bits count.
     const int64_t pairs = (int64_t)B * c.heads;
     if (most <= (pairs >= slots * c.heads / 2 ? 16 : 8) || most * std::min(B, tokens) > INT32_MAX) {
-      if (pairs > INT32_MAX / 16) return Route();
+      if (pairs > most_groups(256)) return Route();
       r.one_whole = true;
       r.one_groups = (uint32_t)pairs;
     }
@@ -185,7 +188,7 @@ extern "C" int tt_paged_write(const void *k, const void *v, const int64_t k_stri
     wgs = cdiv64((int64_t)tokens * c.heads * 2, 4);
     snprintf(name, sizeof(name), "paged_write_any_%s", dtype == TT_BF16 ? "bf16" : "f16");
   }
-  if (wgs > INT32_MAX) return fail(RT_ERR_UNSUPPORTED, "%s: tokens * heads exceeds the grid", who);
+  if (wgs > most_groups(256)) return fail(RT_ERR_UNSUPPORTED, "%s: tokens * heads exceeds the grid", who);
   return launch("paged", name, dim3((uint32_t)wgs), dim3(256), 0, stream, args, 1);
 }
 
@@ -260,7 +263,7 @@ extern "C" int tt_paged_attn(const void *q, const int64_t q_strides[2], const tt
       a.rows_part = (float *)((char *)workspace + r.one_bytes);
       a.rows_groups = (int32_t)r.rows_groups;
     }
-    if (r.rows_groups + r.one_groups > INT32_MAX / 8) return fail(RT_ERR_UNSUPPORTED, "%s: tokens * heads exceeds the grid", who);
+    if (r.rows_groups + r.one_groups > most_groups(256)) return fail(RT_ERR_UNSUPPORTED, "%s: tokens * heads exceeds the grid", who);
     if ((rc = launch("paged", name, dim3((uint32_t)(r.rows_groups + r.one_groups)), dim3(256), 0, stream, args, 1))) return rc;
     if (r.rows_whole) a.rows_groups = 0; // nothing to join there
     const uint32_t joins = 8 * (uint32_t)a.rows_groups + (r.one_join ? r.one_groups * r.join_pieces : 0);
@@ -268,6 +271,7 @@ extern "C" int tt_paged_attn(const void *q, const int64_t q_strides[2], const tt
     snprintf(name, sizeof(name), "paged_attn_%s_%s_d%d_r%d", r.rows ? "rows_join" : "join", type, c.head_dim, r.one_tiles);
     return launch("paged", name, dim3(joins), dim3(256), 0, stream, args, 1);
   }
+  if (tokens > most_groups(64)) return fail(RT_ERR_UNSUPPORTED, "%s: %d tokens exceed the grid", who, tokens);
   return launch("paged", dtype == TT_BF16 ? "paged_attn_any_bf16" : "paged_attn_any_f16",
                 dim3((uint32_t)tokens, (uint32_t)heads_q), dim3(64), 0, stream, args, 1);
 }

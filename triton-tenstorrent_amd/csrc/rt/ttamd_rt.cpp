@@ -288,6 +288,11 @@ int rt_launch(rt_kernel k, const uint32_t grid[3], const uint32_t block[3], uint
   if ((uint64_t)block[0] * block[1] * block[2] > 1024)
     return fail(RT_ERR_INVALID, "rt_launch(%s): more than 1024 threads per workgroup",
                 k->name.c_str());
+  // (a dimension of 2^32 threads and more is launched without an error, with what is left of it modulo 2^32)
+  for (int i = 0; i < 3; ++i)
+    if ((uint64_t)grid[i] * block[i] > UINT32_MAX)
+      return fail(RT_ERR_UNSUPPORTED, "rt_launch(%s): %u workgroups of %u threads in one dimension (2^32 threads or more)",
+                  k->name.c_str(), grid[i], block[i]);
   RT_HIP(hipModuleLaunchKernel(k->fn, grid[0], grid[1], grid[2], block[0], block[1], block[2],
                                shared_bytes, (hipStream_t)stream, args, nullptr));
   return RT_OK;
