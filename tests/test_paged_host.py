@@ -179,3 +179,30 @@ def test_a_users_kernel_of_the_same_name_is_not_bound_to_it():
         assert b"paged" not in record       # the empty kernel, by its body
     except RuntimeError:
         pass
+
+
+@pytest.mark.parametrize("n", [2**31, 2**32 + 1, 2**32 + 16, -2**31 - 1])
+def test_numbers_of_more_than_31_bits_are_refused_not_cut(lib, n):
+    with pytest.raises(rt.InvalidLaunch, match="31 bits"):
+        K.paged_attn_kernel[(6, 8)](*attn_args(max_q=n), CAUSAL=True)
+    with pytest.raises(rt.InvalidLaunch, match="31 bits"):
+        K.paged_plan_kernel[(4, )](*plan_args(), PAGE_SIZE=n)
+    assert not lib.calls
+
+
+def test_tensors_of_more_than_31_bits_are_refused_not_cut(lib):
+    n = 2**32 + 4
+    for args in (plan_args(free_pages=Fake((n, ), I32)), plan_args(slot_map=Fake((n, ), I32)), plan_args(block_table=Fake((4, n), I32))):
+        with pytest.raises(rt.InvalidLaunch, match="31 bits"):
+            K.paged_plan_kernel[(4, )](*args, PAGE_SIZE=16)
+    long = Fake((n, 2, 64), BF16)
+    with pytest.raises(rt.InvalidLaunch, match="31 bits"):
+        K.paged_write_kernel[(4, )](long, long, Fake((n, ), I32), *cache())
+    with pytest.raises(rt.InvalidLaunch, match="31 bits"):
+        K.paged_write_kernel[(7, )](Fake((7, 2, 64), BF16), Fake((7, 2, 64), BF16), Fake((7, ), I32), *cache(pages=n))
+    long = Fake((n, 8, 64), BF16)
+    with pytest.raises(rt.InvalidLaunch, match="31 bits"):
+        K.paged_attn_kernel[(4, 8)](*attn_args(q=long, out=long), CAUSAL=True)
+    with pytest.raises(rt.InvalidLaunch, match="31 bits"):
+        K.paged_attn_kernel[(6, 8)](*attn_args(table=Fake((3, n), I32)), CAUSAL=True)
+    assert not lib.calls

@@ -688,6 +688,11 @@ def _paged_vector(who: str, name: str, t, n: int, dtype):
     return ptr
 
 
+def _refuse_wide(who: str, *values):
+    # handed over as they are, they would lose their upper bits
+    _refuse(who, f"one of {values} is negative or does not fit 31 bits")
+
+
 def _paged_half(who: str, name: str, t, torch):
     """The tt_dtype of a 16-bit float tensor."""
     if t.dtype is torch.bfloat16:
@@ -708,6 +713,8 @@ def _paged_cache(who: str, k, v, k_scale, v_scale, torch):
     if v.shape != shape or k_scale.shape != shape[:2] or v_scale.shape != shape[:2]:
         _refuse(who, f"cache shapes {tuple(shape)}, {tuple(v.shape)}, {tuple(k_scale.shape)}, {tuple(v_scale.shape)}: K and V have one "
                      "shape [pages, heads, page size, head dim], their scales its first two dimensions")
+    if (shape[0] | shape[1] | shape[2] | shape[3]) >> 31:
+        _refuse_wide(who, *shape)
     return rt.pack_paged_cache(pk, pv, pks, pvs, *sk[:3], *sv[:3], *sks, *svs, *shape), shape
 
 
@@ -717,6 +724,8 @@ def _paged_plan_launch(lib, page_size: int, args, grid, stream):
     ctx_lens, new_lens, table, free_pages, free_start, lens, cu_new, slot_map, free_end = args
     pt, st = _paged_tensor(who, "block_table", table, 2, i32)
     B, width = table.shape
+    if (page_size | B | width | free_pages.shape[0] | slot_map.shape[0]) >> 31:
+        _refuse_wide(who, page_size, B, width, free_pages.shape[0], slot_map.shape[0])
     rc = lib.tt_paged_plan(
         _paged_vector(who, "ctx_lens", ctx_lens, B, i32), _paged_vector(who, "new_lens", new_lens, B, i32), pt,
         st[0] if B > 1 else width, B, width, _paged_tensor(who, "free_pages", free_pages, 1, i32)[0], free_pages.shape[0],
@@ -739,6 +748,8 @@ def _paged_write_launch(lib, args, grid, stream):
     T, h, d = k.shape
     if h != H or d != D or k.shape != v.shape:
         _refuse(who, f"k is {tuple(k.shape)}, v is {tuple(v.shape)}; the cache takes [tokens, {H}, {D}]")
+    if T >> 31:
+        _refuse_wide(who, T)
     rc = lib.tt_paged_write(pk, pv, rt.pack_strides2(sk[0], sk[1]), rt.pack_strides2(sv[0], sv[1]),
                             _paged_vector(who, "slot_map", slot_map, T, torch.int32), T, cache, code, grid, stream)
     if rc:
@@ -759,6 +770,8 @@ def _paged_attn_launch(lib, causal: bool, args, grid, stream):
     if q.shape != out.shape or d != D or Hq == 0 or Hq % H:
         _refuse(who, f"q {tuple(q.shape)}, out {tuple(out.shape)} over a cache of {H} heads of {D}: both are [tokens, a multiple of {H}, {D}]")
     B, width = table.shape
+    if (T | Hq | B | width | max_q) >> 31:
+        _refuse_wide(who, T, Hq, B, width, max_q)
     pl = None
     if lse is not None:
         pl, sl = _paged_tensor(who, "lse", lse, 2, torch.float32)
