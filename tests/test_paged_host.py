@@ -1,4 +1,5 @@
 """Host side of the paged 8-bit cache, no GPU: what the launch functions hand to the C ABI, and what they refuse."""
+import json
 import struct
 
 import pytest
@@ -205,4 +206,25 @@ def test_tensors_of_more_than_31_bits_are_refused_not_cut(lib):
         K.paged_attn_kernel[(4, 8)](*attn_args(q=long, out=long), CAUSAL=True)
     with pytest.raises(rt.InvalidLaunch, match="31 bits"):
         K.paged_attn_kernel[(6, 8)](*attn_args(table=Fake((3, n), I32)), CAUSAL=True)
+    assert not lib.calls
+
+
+@pytest.mark.parametrize("name", sorted(drv.OWN_KERNELS))
+def test_a_users_kernel_of_an_own_name_is_bound_by_its_body(name):
+    text = "module {\n  tt.func public @%s(%%arg0: !tt.ptr<f32>) attributes {noinline = false} {\n%s    tt.return\n  }\n}\n"
+    options = type("O", (), {"arch": "gfx950"})
+    assert json.loads(compiler.TTBackend.make_binary(text % (name, ""), {}, options))["kernel"] == "empty_kernel"
+    with pytest.raises(RuntimeError, match=f"'{name}' has no prebuilt"):
+        compiler.TTBackend.make_binary(text % (name, "    %0 = tt.get_program_id x : i32\n"), {}, options)
+
+
+def test_the_wrappers_refuse_tensors_on_the_cpu(lib):
+    q = torch.zeros(2, 4, 64, dtype=BF16)
+    c = K.paged_cache(4, 2, 64, 16, device="cpu")
+    i = lambda *v: torch.tensor(v, dtype=I32)
+    for call in (lambda: K.paged_attention(q, c, i(0, 1).view(2, 1), i(1, 1), i(0, 1, 2), 1.0, max_q=1),
+                 lambda: K.paged_write(q[:, :2], q[:, :2], i(0, 1), c),
+                 lambda: K.paged_plan(i(0, 0), i(1, 1), i(-1, -1).view(2, 1), i(0, 1), 16, 2)):
+        with pytest.raises(rt.InvalidLaunch, match="on the GPU"):
+            call()
     assert not lib.calls
