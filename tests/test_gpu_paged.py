@@ -811,3 +811,148 @@ def test_rt_launch_refuses_a_dimension_of_more_threads_than_32_bits_count():
     three = lambda *v: (ctypes.c_uint32 * 3)(*v)
     for grid, block in (((2**24, 1, 1), (256, 1, 1)), ((2**32 - 1, 1, 1), (2, 1, 1)), ((1, 2**31, 1), (1, 2, 1)), ((1, 1, 2**26), (1, 1, 64))):
         assert lib.rt_launch(k, three(*grid), three(*block), 0, None, None, 0) == rt.RT_ERR_UNSUPPORTED
+
+
+# ---- the kernel for a few queries of a sequence, and it beside the one for many, where masks and codes are special ----
+FEW = [(5, 4, 2, 64), (16, 4, 2, 64), (5, 4, 2, 128), (16, 4, 2, 128), (8, 4, 2, 256), (3, 33, 3, 64), (3, 30, 3, 64)]   # n, Hq, H, D
+
+
+def few_or_rows(n, Hq, H, D):
+    """Queries times group up to 32 rows (16 at head dim 256) are the few-queries kernel's."""
+    return "_few_" if n * Hq // H <= (16 if D == 256 else 32) else "_rows_"
+
+
+def attend(q, codes, scales, table, lens, cu, sm_scale=0.1, **kw):
+    return K.paged_attention(q.cuda(), device_cache(codes, scales), i32(table), i32(lens), i32(cu), sm_scale, return_lse=True, **kw)
+
+
+def oracle_of(q, codes, scales, table, lens, cu, sm_scale=0.1, causal=True):
+    return orc.attention(q.double().numpy(), codes[0], codes[1], scales[0], scales[1], table, lens, cu, sm_scale, causal)
+
+
+@pytest.mark.parametrize("n,Hq,H,D", FEW)
+@pytest.mark.parametrize("causal", [True, False])
+def test_few_pages_outside_the_cache_count_as_absent(n, Hq, H, D, causal):
+    q, codes, scales, table, lens, cu = make([300, 150, 64, 4000], [n] * 4, Hq, H, 32, D, torch.bfloat16, seed=40)
+    table[0, 3], table[0, 5], table[1, 0], table[2, :], table[3, 60] = -1, 10**6, codes.shape[1], -1, -5
+    o, lse = attend(q, codes, scales, table, lens, cu, max_q=n, causal=causal)
+    compare(o, lse, oracle_of(q, codes, scales, table, lens, cu, causal=causal), 4000, D, torch.bfloat16)
+    short = (q[:3 * n], codes, scales, table[:3, :12].copy(), lens[:3], cu[:4])
+    o, lse = attend(*short, max_q=n, causal=causal)
+    assert few_or_rows(n, Hq, H, D) in rt.last_kernel_name()
+    compare(o, lse, oracle_of(*short, causal=causal), 300, D, torch.bfloat16)
+
+
+@pytest.mark.parametrize("n,Hq,H,D", FEW)
+def test_few_lengths_past_the_table_and_below_zero(n, Hq, H, D):
+    q, codes, scales, table, lens, cu = make([96, 96], [n, n], Hq, H, 32, D, torch.float16, seed=41)
+    table = np.ascontiguousarray(table[:, :3])
+    o, lse = attend(q, codes, scales, table, [96, 2**31 - 1], cu, max_q=n)
+    assert few_or_rows(n, Hq, H, D) in rt.last_kernel_name()
+    compare(o, lse, oracle_of(q, codes, scales, table, [96, 96], cu), 96, D, torch.float16)
+    o, lse = attend(q, codes, scales, table, [96, -5], cu, max_q=n)
+    assert (o[n:] == 0).all() and torch.isneginf(lse[n:]).all()
+    compare(o[:n], lse[:n], tuple(x[:n] for x in oracle_of(q, codes, scales, table, [96, 96], cu)), 96, D, torch.float16)
+
+
+@pytest.mark.parametrize("n,Hq,H,D", FEW)
+def test_few_strided_queries_and_results_and_rows_of_no_sequence(n, Hq, H, D):
+    q, codes, scales, table, lens, cu = make([90, 300], [n, n], Hq, H, 32, D, torch.bfloat16, seed=42)
+    rows = 2 * n + 7
+    wide = torch.full((rows, Hq * D + 24), float("nan"), dtype=torch.bfloat16, device="cuda")
+    qv = wide[:, :Hq * D].view(rows, Hq, D)
+    qv[:2 * n] = q.cuda()
+    want = oracle_of(q, codes, scales, table, lens, cu)
+    for off in (0, 8, 3):       # 3: rows off the alignment the fast kernels need
+        hold = torch.full((Hq, rows, D + off), 7.0, dtype=torch.bfloat16, device="cuda")
+        out = hold[:, :, off:].transpose(0, 1)
+        o, lse = K.paged_attention(qv, device_cache(codes, scales), i32(table), i32(lens), i32(cu), 0.1, max_q=n, return_lse=True, out=out)
+        assert (few_or_rows(n, Hq, H, D) if off != 3 else "_any_") in rt.last_kernel_name()
+        compare(o[:2 * n], lse[:2 * n], want, 300, D, torch.bfloat16)
+        assert (hold[:, :, :off] == 7).all() and (out[2 * n:] == 7).all()
+
+
+def check_nan(lens, n_q, Hq, H, P, D, bad, causal, apart=0, kernel=None, dtype=torch.bfloat16):
+    """bad: (sequence, position, 0 for K or 1 for V): one NaN code, in channel 5 of head 0."""
+    q, codes, scales, table, lens, cu = make(lens, n_q, Hq, H, P, D, dtype, seed=43)
+    if apart:
+        scales[1] = np.where(np.random.default_rng(3).random(scales[1].shape) < 0.5, 130 - apart, 130)
+        scales[1][table[0, 0]], scales[1][table[0, 1]] = 130, 130 - apart
+    for b, pos, j in bad:
+        codes[j, table[b, pos // P], 0, pos % P, 5] = 0x7F if pos % 2 else 0xFF
+    o, lse = attend(q, codes, scales, table, lens, cu, max_q=int(max(n_q)), causal=causal)
+    if kernel:
+        assert kernel in rt.last_kernel_name()
+    clean = codes.copy()
+    clean[:, table[table >= 0]] = np.where((clean[:, table[table >= 0]] & 127) == 127, 0, clean[:, table[table >= 0]])
+    wo = oracle_of(q, clean, scales, table, lens, cu, causal=causal)[0]
+    o = o.double().cpu().numpy()
+    for b, L in enumerate(lens):
+        for i in range(n_q[b]):
+            last = L - n_q[b] + i if causal else L - 1
+            hits = {j for bb, pos, j in bad if bb == b and pos <= last}
+            for h in range(Hq):
+                row = np.isnan(o[cu[b] + i, h])
+                if h * H // Hq or not hits:
+                    assert not row.any(), (b, i, h)
+                elif 0 in hits:
+                    assert row.all(), (b, i, h)
+                else:
+                    assert row[5] and not np.delete(row, 5).any(), (b, i, h)
+                if not hits:        # (the oracle's rows that see no bad key: compared roughly, a NaN that was counted as a key would show)
+                    assert np.allclose(o[cu[b] + i, h], wo[cu[b] + i, h], rtol=0.05, atol=0.02 * np.abs(wo[cu[b] + i, h]).max())
+
+
+@pytest.mark.parametrize("n,Hq,H,D", FEW)
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("apart", [0, 40])
+def test_few_nan_codes_reach_the_queries_that_attend_them_only(n, Hq, H, D, causal, apart):
+    # (sequence 1: NaN in V at the last keys, which only the last queries attend; sequence 2: in K too; 3: none)
+    bad = [(0, 30, 1), (1, 69, 1), (1, 68, 1), (1, 66, 1), (2, 97, 1), (2, 99, 0)]
+    check_nan([60, 70, 100, 33], [n] * 4, Hq, H, 16, D, bad, causal, apart, few_or_rows(n, Hq, H, D))
+
+
+@pytest.mark.parametrize("Hq,H,D", [(4, 2, 64), (8, 2, 128), (4, 2, 256)])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("apart", [0, 40])
+def test_nan_codes_where_few_and_many_queries_share_a_launch(Hq, H, D, causal, apart):
+    bad = [(0, 97, 1), (0, 30, 1), (1, 69, 1), (2, 130, 1), (2, 199, 1), (3, 0, 0)]
+    check_nan([100, 70, 200, 40, 90], [4, 1, 150, 3, 60], Hq, H, 16, D, bad, causal, apart, "_rows_")
+
+
+@pytest.mark.parametrize("n_q", [[1, 1, 1], [5, 3, 4], [60, 40, 90], [60, 1, 4]])
+@pytest.mark.parametrize("apart", [0, 40])
+def test_results_over_the_queries(n_q, apart):
+    # out may be q itself: a row is read before it is written, also where a second pass follows
+    q, codes, scales, table, lens, cu = make([100, 2000, 90], n_q, 8, 2, 16, 128, torch.bfloat16, seed=44)
+    if apart:
+        scales[1] = np.where(np.random.default_rng(4).random(scales[1].shape) < 0.5, 130 - apart, 130)
+    args = (device_cache(codes, scales), i32(table), i32(lens), i32(cu), 0.1)
+    o, lse = K.paged_attention(q.cuda(), *args, max_q=max(n_q), return_lse=True)
+    x = q.cuda()
+    o2, lse2 = K.paged_attention(x, *args, max_q=max(n_q), return_lse=True, out=x)
+    assert o2 is x and torch.equal(o, o2) and torch.equal(lse, lse2)
+
+
+# ---- the write's infinities and NaN, in runs of every kind ----
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("D,P", [(64, 64), (128, 64), (256, 64), (64, 256), (128, 256), (256, 256), (40, 64)])
+def test_write_of_special_values_in_runs_that_wavefronts_share(dtype, D, P):
+    H = 2
+    codes, scales = filled(9, H, P, D, seed=D + P)
+    spec = [(0, 0, P), (1, 0, P), (2, 0, P), (3, 7, P - 7), (4, 0, P), (5, P // 2, P // 2), (6, 0, P - 1), (7, 3, 1)]
+    slots, g = runs(spec, P), torch.Generator().manual_seed(D * P)
+    at = np.cumsum([0] + [n for _, _, n in spec])
+    x = torch.randn(2, len(slots), H, D, generator=g)
+    x[:, at[3]:at[4]] *= 3e4 if dtype is torch.bfloat16 else 1e3       # the scale grows behind earlier rows
+    x[:, at[5]:at[6]] *= 1e-3                                          # and here it does not
+    x = x.to(dtype)
+    inf, nan = float("inf"), float("nan")
+    x[0, at[0] + P // 2 + 3, 0, 5], x[1, at[0] + P - 1, 1, D - 1] = inf, -inf      # one wavefront's rows only; runs 1 and 6 have none
+    x[:, at[2]:at[3], 0, ::3], x[0, at[2]:at[3], 1] = nan, inf                     # nothing finite in K's head 1
+    x[0, at[3] + 1, 0, 0], x[1, at[3], 0, 1] = nan, inf
+    x[:, at[4]:at[5]] = torch.finfo(dtype).max
+    x[1, at[4] + P // 4, 1, 2] = -inf
+    x[:, at[5]] = -inf
+    x[0, at[7], 1, 3], x[1, at[7]] = inf, nan
+    check_write(x.cuda(), slots, codes, scales)
