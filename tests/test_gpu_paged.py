@@ -956,3 +956,25 @@ def test_write_of_special_values_in_runs_that_wavefronts_share(dtype, D, P):
     x[:, at[5]] = -inf
     x[0, at[7], 1, 3], x[1, at[7]] = inf, nan
     check_write(x.cuda(), slots, codes, scales)
+
+
+def test_plan_of_sequences_taken_back():
+    # (drafts that were rejected: the entries behind the shorter length are replaced, the page that it ends in stays)
+    table = np.array([[5, 6, 7, -1], [8, 9, -1, -1], [3, 2, 1, -1]])
+    run_plan([5, 4, 0], [4, 3, 5], table, np.arange(20, 30), 4, 12)
+
+
+@pytest.mark.parametrize("Hq,H,D", [(4, 2, 64), (2, 1, 128)])
+@pytest.mark.parametrize("most", [1, 4, 150])
+def test_many_sequences_of_scales_far_apart(Hq, H, D, most):
+    # over 64 sequences, each lane of a scan several; some workgroups meet near and far ones
+    rng = np.random.default_rng(6)
+    lens = rng.integers(0, 200, 150)
+    n = np.minimum(rng.integers(0, 2, 150), lens)
+    n[[3, 70, 149]] = np.minimum([150, 37, 20], lens[[3, 70, 149]])
+    n = np.minimum(n, most)
+    q, codes, scales, table, lens, cu = make(list(lens), list(n), Hq, H, 32, D, torch.bfloat16, seed=7)
+    far = rng.random(scales[1].shape) < 0.2
+    scales[1] = np.where(far, 60, 130)
+    o, lse = attend(q, codes, scales, table, lens, cu, max_q=most)
+    compare(o, lse, oracle_of(q, codes, scales, table, lens, cu), 200, D, torch.bfloat16)
