@@ -617,6 +617,12 @@ __device__ __attribute__((noinline)) void far_pass(uint64_t args, Lds lds, int w
 }
 template <class E, int D, int MT, bool FEW, int OCC>
 __device__ __forceinline__ void both(const PagedAttnArgs &a, float *lds, int wg, int wgs) {
+  { // One word of each line of the arguments, asked for at once: with a call in the kernel the compiler loads them in three
+    // or four turns, each a wait for memory otherwise (62 rows over 16 encoder states: 20.3 us instead of 19.3).
+    static_assert(sizeof(PagedAttnArgs) > 64 * 4, "a word of the fifth line");
+    const __attribute__((address_space(4))) uint32_t *p = (const __attribute__((address_space(4))) uint32_t *)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" :: "s"(p[0]), "s"(p[16]), "s"(p[32]), "s"(p[48]), "s"(p[64]));
+  }
   if (__builtin_expect(body<E, D, MT, FEW, false>(a, lds, wg, wgs, threadIdx.x), 0)) {
     __syncthreads();
     far_pass<E, D, MT, FEW, OCC>((uint64_t)__builtin_amdgcn_kernarg_segment_ptr(), (Lds)lds, wg, wgs);
