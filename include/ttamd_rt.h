@@ -358,8 +358,8 @@ TTAMD_API int tt_attn_fwd(float sm_scale, float *M, int32_t Z, int32_t H, const 
 /* ----------------------------------------------------------------------- */
 
 /* The cache of one layer: for K and for V, e4m3 codes [num_pages, heads, page_size, head_dim] and one scale for each
- * (page, head), held as its exponent: code s (a byte, 1..247; tt_paged_write makes 27..247) stands for 2^(s - 127), and a
- * cached value is its code times its page's scale.  Strides are in elements, of dimensions page, head and token (codes; the last dimension is
+ * (page, head), held as its exponent: code s (a byte, 27..247, as tt_paged_write makes them) stands for 2^(s - 127), and
+ * a cached value is its code times its page's scale.  Strides are in elements, of dimensions page, head and token (codes; the last dimension is
  * contiguous) and page and head (scales).  A sequence's tokens lie in the pages its row of the block table names:
  * position p in page table[p / page_size], row p % page_size.
  * All strides must be >= 0; num_pages, heads, page_size, head_dim >= 1, num_pages * page_size < 2^31,
@@ -378,7 +378,9 @@ typedef struct tt_paged_cache {
  *   cu_new[b]   first row of sequence b among the packed new tokens; cu_new[B] = their number
  *   lens[b]     ctx_lens[b] + the new tokens that were taken
  *   block_table entries for the pages that ctx_lens[b] does not reach yet are taken from free_pages in sequence order,
- *               from index *free_start (null: 0); earlier entries are read and stay as they are
+ *               from index *free_start (null: 0); earlier entries are read and stay as they are.  A sequence is taken back
+ *               by a smaller ctx_lens[b]: entries behind the pages that this one reaches are then replaced like empty ones,
+ *               and the pages they named are the caller's to give back to free_pages
  *   slot_map[t] page * page_size + row of new token t; -1 for t >= cu_new[B] and for tokens without a page
  *   free_end[0] *free_start + the pages that were needed; more than num_free says that the list ran out (the entries
  *               and slots it could not fill are -1)

@@ -4,7 +4,7 @@
 // What bounds it: one pass over the cached codes, HBM.  A wavefront owns all queries and query heads of one cache head
 // (row r is query r / group, head r % group; empty rows of the MFMA tile cost nothing here) and streams keys from global memory
 // into registers (6 sequences of 20000 to 131000 keys, 8 heads of 128, 782 MB: 131 us, 6.0 TB/s where a copy reaches 6.7; 48 of
-// 60 to 8000 keys: 56 us, 5.7 TB/s; the join 5 us), with no LDS between: every code is used once, by one wavefront.
+// 60 to 8000 keys: 55 to 65 us from one set of inputs to another, at best 5.9 TB/s; the join 5 us), with no LDS between: every code is used once, by one wavefront.
 //   S^T[key, r] = K . Q^T       v_mfma_f32_16x16x32, A = 16 rows of K, B = Q; lane l ends with row l%16, keys (l/16)*4+r
 //   O^T[d, r]  += V^T . P^T     B = P^T is what the lane already holds; A = V^T, whose lane needs 8 keys of one d: it loads
 //                               D/16 consecutive codes of each of its keys and pairs neighbouring keys' bytes with
@@ -17,7 +17,7 @@
 // contribution and nothing below 2^-32.  That is nothing beside it, but all that there is in a channel where the larger
 // pages hold zeros.  So a sequence whose V scales a workgroup finds more than 2^kSpan apart (pages of ordinary values never
 // are; within 2^12, 2^-21 are left) goes to a second pass, FAR: a weight is the sum of two bf16 there, which reach as far as
-// fp32 does and leave 2^-17, and costs two products.
+// fp32 does and leave 2^-16, and costs two products.
 //
 // Split: a group of workgroups, one for each cache head, takes an even share of the keys of all sequences, in units of
 // 64 * NS keys, whatever the lengths.  (All heads of a page are read at about the same time, by neighbouring workgroups:
@@ -72,7 +72,8 @@ struct Span {
 };
 
 // Subtiles of 16 keys that a wavefront takes in one step.  Two leave room for three workgroups on a CU at head dim 128
-// and make finer units than four (513 keys, 8 heads: 7.2 us against 9.3); at head dim 64 two would be too few bytes in flight.
+// and make finer units than four (calls in a captured graph: 513 keys, 8 heads 8.6 us against 12.5; 48 sequences of 60 to 8000
+// keys 73 against 94); at head dim 64 two would be too few bytes in flight.
 template <int D, int MT> constexpr int subtiles() { return D * MT >= 128 ? 2 : 4; }
 
 // Sequence b as this kernel sees it: no units where it is not this kernel's (no query, or too many).
@@ -168,8 +169,8 @@ struct Hf {
 template <bool FAR> struct Weights { typedef Hf type; };
 template <> struct Weights<true> { typedef Bf type; };
 
-// Codes are read once: non-temporal loads where a row is whole 128-byte lines (782 MB of cache, head dim 128: 140 -> 126 us;
-// head dim 64, whose lines two rows share: no gain).
+// Codes are read once: non-temporal loads where a row is whole 128-byte lines (782 MB of cache, head dim 128, a call
+// in a captured graph: 162 -> 155 us; head dim 64, whose lines two rows share: no gain).
 template <int D, typename T> __device__ __forceinline__ T stream(const T *p) {
   if constexpr (D >= 128) return __builtin_nontemporal_load(p);
   return *p;

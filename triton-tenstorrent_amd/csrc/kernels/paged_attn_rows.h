@@ -9,7 +9,8 @@
 // two tiles ahead, turned to 16 bits on the way into LDS, V transposed there (v_perm_b32 pairs neighbouring keys' bytes
 // before the conversion, as in paged_attn_one.h), K and V without their scales, which join the scores as there.  LDS
 // holds two tiles; one barrier a tile.
-// Bound: instruction issue.  7169 prompt tokens, 32 heads of 128 over 8: 250 us, 848 TFLOP/s (a large product reaches 1593); the
+// Bound: instruction issue.  7169 prompt tokens, 32 heads of 128 over 8: 250 us, 848 TFLOP/s (a large product reaches 1593; both
+// vary by 6 % from one machine to another); the
 // MFMA pipes are busy a third of the time, an instruction is issued in 82 % of the cycles (exponentials, conversions,
 // staging).  Two workgroups on a CU, so that one's softmax runs beside the other's products; one wavefront a SIMD with
 // twice the rows moves its accumulators between the register files (488 us).
@@ -417,7 +418,8 @@ __device__ __forceinline__ bool body(const PagedAttnArgs &a, uint8_t *lds, int w
             for (int r = 0; r < 16; ++r) acc[i][r] *= al;
         }
         const float ref = (mref == -kInf ? 0.0f : mref) - kLift;
-        // weights of a subtile between the products of the one before, V fragments four reads ahead
+        // weights of a subtile between the products of the one before, V fragments four reads ahead (the sums of weights too as
+        // it is written; the compiler moves those, 32 additions, behind the last product)
         typename W::frag pf[4];
         [[maybe_unused]] typename W::frag rest[4]; // FAR: what rounding to pf took away
         float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};

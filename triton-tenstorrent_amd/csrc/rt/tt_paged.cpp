@@ -76,12 +76,15 @@ Route route_of(const PagedCacheArgs &c, int32_t B, int32_t max_pages, int32_t to
     r.one_tiles = few / 16;
     const int64_t unit = D * r.one_tiles >= 128 ? 128 : 256;
     const int64_t most = std::max<int64_t>(cdiv64(keys, unit), 1);
-    // a workgroup for each head of a group; the groups fill the chip once (two or three workgroups a CU) or have a unit each
+    // A workgroup for each head of a group; the groups fill the chip once (two or three workgroups a CU) or have a unit each.
+    // (Behind row tiles of head dim 256, with one workgroup on a CU, they come in two turns.)
     const int64_t slots = std::max((D * r.one_tiles > 128 || max_q > 1 ? 2 : 3) * cus / c.heads, 1);
     r.one_groups = (uint32_t)(std::min<int64_t>(most * std::min(B, tokens), slots) * c.heads);
     // A workgroup for each (sequence, head) instead, without parts to join, where the table allows no long sequence: up to
-    // 8 units take less than the second launch costs (8 heads of 512 keys: 7.4 us against 11.5; 2048 keys: 20), up to 16
-    // where there are pairs enough to keep the chip busy (512 pairs of 2048 keys: 44.6 us against 56).
+    // 8 units, up to 16 where there are pairs enough to keep the chip busy.  Calls in a captured graph, 8 heads of 128, whole
+    // sequences against split ones: 1 sequence of 6 units 9.4 us against 10.3, of 8 units 13.7 against 10.5; 8 sequences of 8
+    // units 14.9 against 16.4, of 10 units 17.5 against 16.6; 64 sequences of 16 units 50 against 65.  (The host, which knows
+    // the table's width only, cannot tell one short sequence in a wide table from a long one.)
     // Also where the table allows more units than 32 bits count.
     const int64_t pairs = (int64_t)B * c.heads;
     if (most <= (pairs >= slots * c.heads / 2 ? 16 : 8) || most * std::min(B, tokens) > INT32_MAX) {
@@ -98,7 +101,11 @@ Route route_of(const PagedCacheArgs &c, int32_t B, int32_t max_pages, int32_t to
   r.workspace = r.one_bytes;
   if (r.rows) {
     const int64_t items = ((int64_t)tokens * group / 128 + std::min(B, tokens)) * c.heads, slots = (D == 256 ? 1 : 2) * cus;
-    // (the last condition: more steps than 32 bits count)
+    // `items` is what the launch may have to hold: a tile for each sequence, also for those that turn out to be the other
+    // kernel's.  As a bound of the work it is high beside many single tokens, but the rows by themselves are a worse one (the
+    // rule with tokens * group / 128 in its place: a piece of a prompt beside 120, 199 and 256 single tokens 319, 504 and 561 us
+    // instead of 330, 548 and 596, beside 159 441 instead of 426; 128 sequences of up to 20 tokens 111 instead of 95, 200
+    // 151 instead of 138).  (The last condition: more steps than 32 bits count.)
     r.rows_whole = items >= 2 * slots || keys <= 64 || items / c.heads * cdiv64(keys, 64) > INT32_MAX;
     r.rows_groups = r.rows_whole ? items : std::max<int64_t>(slots / c.heads, 1) * c.heads;
     if (!r.rows_whole) r.workspace += (size_t)r.rows_groups * (2 * (128 * D + 256) * sizeof(float) + 16);
@@ -178,8 +185,11 @@ extern "C" int tt_paged_write(const void *k, const void *v, const int64_t k_stri
   char name[64];
   int64_t wgs;
   if (al && (D == 64 || D == 128 || D == 256)) {
-    // Tokens per workgroup.  16 single tokens are what its wavefronts do at once at head dim 128; once that gives more
-    // workgroups than the chip holds (8 a CU), 64 leave fewer that only find out that a run began before them.
+    // Tokens per workgroup.  16 single tokens are what its wavefronts do at once at head dim 128; where that gives more
+    // workgroups than the chip takes at a time (6 or 7 a CU), 64 leave fewer that only find out that a run began before them.
+    // In a captured graph, 8 heads of 128, 16 against 64: 256 single tokens 3.9 us against 5.9, 1024 4.8 against 6.2, 2048
+    // 7.1 against 7.1; a prompt of 2090 tokens 8.3 against 5.7 (and of 1045, which the host cannot tell from single ones, 6.5
+    // against 4.6).
     a.tile = cdiv64(tokens, 16) * c.heads * 2 > 8 * props()->multiprocessor_count ? 64 : 16;
     wgs = cdiv64(tokens, a.tile) * c.heads * 2;
     snprintf(name, sizeof(name), "paged_write_%s_d%d", dtype == TT_BF16 ? "bf16" : "f16", D);

@@ -366,8 +366,8 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, causal: bool, s
 # ---- a paged key/value cache in 8 bits --------------------------------------
 class PagedCache(NamedTuple):
     """The cache of one layer.  ``k``, ``v``: e4m3 codes [pages, heads, page_size, head_dim] (any strides, the last
-    dimension contiguous); ``k_scale``, ``v_scale``: uint8 [pages, heads], exponents: code s stands for 2^(s - 127), and
-    a cached value is its code times its page's scale."""
+    dimension contiguous); ``k_scale``, ``v_scale``: uint8 [pages, heads], exponents: code s (27 .. 247) stands for
+    2^(s - 127), and a cached value is its code times its page's scale."""
     k: torch.Tensor
     v: torch.Tensor
     k_scale: torch.Tensor
@@ -404,7 +404,9 @@ def paged_plan(ctx_lens: torch.Tensor, new_lens: torch.Tensor, block_table: torc
     ``block_table`` (int32 [B, max_pages]) is extended in place with pages from ``free_pages`` (int32), taken in sequence
     order from index ``free_start`` (int32 [1]; None: 0).  ``max_tokens`` is the size of the slot map, at least the sum of
     ``new_lens``; with a larger one the surplus slots are -1, so that a captured step serves batches of several sizes.
-    ``free_end`` is where the next step's ``free_start`` begins; past ``len(free_pages)`` it says that pages ran out."""
+    ``free_end`` is where the next step's ``free_start`` begins; past ``len(free_pages)`` it says that pages ran out.
+    Entries behind the pages that ``ctx_lens[b]`` reaches are replaced, whatever they hold: the pages of tokens that were
+    taken back (a smaller ``ctx_lens[b]``) are the caller's to give back."""
     B = block_table.shape[0]
     made = torch.empty(2 * B + 2 + max_tokens, dtype=torch.int32, device=block_table.device)
     plan = PagedPlan(*made.split_with_sizes((B, B + 1, max_tokens, 1)))     # one allocation
