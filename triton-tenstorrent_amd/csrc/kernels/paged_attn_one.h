@@ -704,11 +704,11 @@ template <int D, int MT> constexpr int lds_floats() { return 4 * 16 * MT * (D + 
 #define PAGED_ONE(T, E, D, MT, OCC)                                                                           \
   extern "C" __global__ __launch_bounds__(256, OCC) void paged_attn_one_##T##_d##D##_r##MT(PagedAttnArgs a) {  \
     __shared__ __align__(16) float lds[one::lds_floats<D, MT>()];                                             \
-    one::both<one::E, D, MT, false, OCC>(a, lds, blockIdx.x, gridDim.x);                                           \
+    one::both<one::E, D, MT, false, OCC>(a, lds, blockIdx.x, gridDim.x);                                      \
   }                                                                                                           \
   extern "C" __global__ __launch_bounds__(256, 2) void paged_attn_few_##T##_d##D##_r##MT(PagedAttnArgs a) {    \
     __shared__ __align__(16) float lds[one::lds_floats<D, MT>()];                                             \
-    one::both<one::E, D, MT, true, 2>(a, lds, blockIdx.x, gridDim.x);                                            \
+    one::both<one::E, D, MT, true, 2>(a, lds, blockIdx.x, gridDim.x);                                         \
   }                                                                                                           \
   extern "C" __global__ __launch_bounds__(256) void paged_attn_join_##T##_d##D##_r##MT(PagedAttnArgs a) {      \
     __shared__ one::f32x4 lds[256 + 128];                                                                     \

@@ -326,14 +326,10 @@ __device__ __forceinline__ bool body(const PagedAttnArgs &a, uint8_t *lds, int w
       for (int w = 0; w < VW; ++w) {
         const uint32_t x0 = __builtin_amdgcn_perm(vr[1][w], vr[0][w], 0x05010400), x1 = __builtin_amdgcn_perm(vr[3][w], vr[2][w], 0x05010400);
         const uint32_t y0 = __builtin_amdgcn_perm(vr[1][w], vr[0][w], 0x07030602), y1 = __builtin_amdgcn_perm(vr[3][w], vr[2][w], 0x07030602);
-        const u32x2 f[4] = {{W::template codes2<false>(x0),
-                             W::template codes2<false>(x1)},
-                            {W::template codes2<true>(x0),
-                             W::template codes2<true>(x1)},
-                            {W::template codes2<false>(y0),
-                             W::template codes2<false>(y1)},
-                            {W::template codes2<true>(y0),
-                             W::template codes2<true>(y1)}};
+        const u32x2 f[4] = {{W::template codes2<false>(x0), W::template codes2<false>(x1)},
+                            {W::template codes2<true>(x0), W::template codes2<true>(x1)},
+                            {W::template codes2<false>(y0), W::template codes2<false>(y1)},
+                            {W::template codes2<true>(y0), W::template codes2<true>(y1)}};
   #pragma unroll
         for (int i = 0; i < 4; ++i) *(u32x2 *)(lds + (vw ^ (((w * 4 + i) >> 1) << 4)) + (w * 4 + i) * 128) = f[i];
       }
